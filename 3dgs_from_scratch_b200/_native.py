@@ -90,6 +90,11 @@ SIGNATURES = {
     "gs_ssim_forward": (I, [I, I, I, P, P, I, P, SZ, P, P]),
     "gs_ssim_backward": (I, [I, I, I, P, P, P, P, P, P]),
     "gs_l1_ssim_loss_grad": (I, [I, I, P, P, I, F, P, P, P, SZ, P]),
+    "gs_gated_scan_saved_bytes": (SZ, [I64, I, I, I, I]),
+    "gs_gated_scan_scratch_bytes": (SZ, [I64, I, I, I, I, I]),
+    "gs_gated_scan_forward": (I, [I64, I, I, I, I, I, P, I64, P, I64, P, P, I, P, P, P, P, SZ, P]),
+    "gs_gated_scan_backward": (I, [I64, I, I, I, I, I, P, I64, P, I64, P, P, I, P, P, I64, P, P, P,
+                                   P, P, SZ, P]),
     "gs_preprocess_backward": (I, [I, P, P, P, P, P, P, P, P, P, I, I, I, I, I, P, P, I, P, I, P,
                                    P, P, P, P, P, P]),
     "gs_preprocess_forward_views": (I, [I, I, P, P, P, P, P, P, P, P, P, F, F, F, F, F, I, I, I,
@@ -99,6 +104,9 @@ SIGNATURES = {
     "gs_preprocess_backward_views": (I, [I, I, P, P, P, P, P, P, P, P, P, I, I, I, I, I, P, P, I,
                                          P, I, P, P, P, P, P, P, P]),
 }
+
+# GS_TYPE_* by torch dtype name
+TYPES = {"float32": 0, "bfloat16": 1, "float16": 2}
 
 _lib = None
 _lock = threading.Lock()

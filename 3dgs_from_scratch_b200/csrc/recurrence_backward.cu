@@ -1,0 +1,242 @@
+// recurrence_backward.cu -- the gated recurrence's gradients (see
+// recurrence.cuh for the tiles).
+//
+// With u_t = dh_t + g_{t+1} u_{t+1} the gradient that reaches h_t, the chain
+// runs over v_t = g_t u_t, what row t hands to row t - 1, so that a row needs
+// only its own gate:
+//   v_t = g_t (dh_t + v_{t+1}), v after the last row = dfinal;
+//   dx_t = u_t = dh_t + v_{t+1};  dg_t = sum over the gate's channels of u_t h_{t-1};
+//   dinitial = v of the first row.
+// The states h_{t-1} are recomputed in 32 bits from x, the gates and the state
+// that the forward kept before each tile: the rounded h of a 16-bit run would
+// cost the gates' gradient its last bits, and reading it costs as much as
+// reading x.
+#include "recurrence.cuh"
+
+namespace gs {
+namespace scan {
+
+template <typename XT, typename GT, int V, int R, bool SHARED, bool CHAINS>
+__global__ void __launch_bounds__(kThreads) backward_kernel(const Args A) {
+  __shared__ Tile<V, R> S;
+  __shared__ float sums[SHARED && !CHAINS ? kThreads * R : 1];
+  const int cblk = blockIdx.x % A.channel_blocks;
+  const int64_t tile = A.tiles - 1 - blockIdx.x / A.channel_blocks;
+  const Place p = place_of<V, R, SHARED>(A, tile, cblk);
+  Pack<XT, V> x[R], dh[R];
+  Gates<GT, V, SHARED> g[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (i < p.rows) {
+      const int64_t row = row_of<R>(A, p, i);
+      if (!CHAINS)
+        x[i] = load_pack<XT, V>(reinterpret_cast<const XT *>(A.x) + row * A.x_stride + p.c);
+      if (A.dh != nullptr) {
+        dh[i] = load_pack<XT, V>(reinterpret_cast<const XT *>(A.dh) + row * A.dh_stride + p.c);
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) dh[i].e[v] = from_f32<XT>(0.f);
+      }
+      g[i].load(A, row, p.g);
+    }
+  tile_info(A, tile, S.info);
+  float P[V], L[V], tp, tl;
+  float before[R][V];  // the state before each row
+  if (!CHAINS) {
+    reduce_segment<XT, GT, V, R, SHARED>(A, p, S.info, x, g, P, L);
+    put_segment<V, R>(A, p, S, segment_cut<R>(p, S.info, 1), P, L);
+    __syncthreads();
+    fold_segments<V, R, false>(A, S, tp, tl);
+    __syncthreads();
+    if (p.on) {
+      float h[V];
+      enter_segment<V, R>(A, p, S, A.saved, h);
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        if (i >= p.rows) break;
+        const int in = S.info[p.sg * R + i];
+        if (in >= 0 && (in & 1)) load_state<V>(A.initial, A, in >> 2, p.c, h);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          before[i][v] = h[v];
+          h[v] = in < 0 ? 0.f : fmaf(g[i](v), h[v], to_f32<XT>(x[i].e[v]));
+        }
+      }
+    }
+    __syncthreads();
+  }
+  reduce_segment_back<XT, GT, V, R, SHARED>(A, p, S.info, dh, g, P, L);
+  put_segment<V, R>(A, p, S, segment_cut<R>(p, S.info, 2), P, L);
+  __syncthreads();
+  const bool cut = fold_segments<V, R, true>(A, S, tp, tl);
+  if (CHAINS) {
+    const int c = cblk * A.tx * V + threadIdx.x;
+    if (threadIdx.x < A.tx * V && c < A.channels) A.chains[tile * A.channels + c] = make_float2(tp, tl);
+    if (cblk == 0 && threadIdx.x == 0) A.cuts[tile] = cut;
+    return;
+  }
+  __syncthreads();
+  const int c1 = (cblk + 1) * A.tx * V < A.channels ? (cblk + 1) * A.tx * V : A.channels;
+  empty_sequences(A, tile, cblk * A.tx * V, c1, A.dfinal, A.dinitial);
+  if (p.on) {
+    float after[V];
+    enter_segment<V, R>(A, p, S, A.carry, after);
+#pragma unroll
+    for (int i = R - 1; i >= 0; --i) {
+      if (i >= p.rows) continue;
+      const int in = S.info[p.sg * R + i];
+      const int64_t row = row_of<R>(A, p, i);
+      float u[V], dg[V], sum = 0.f;
+      if (in < 0) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) u[v] = dg[v] = after[v] = 0.f;
+      } else {
+        if (in & 2) load_state<V>(A.dfinal, A, in >> 2, p.c, after);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          u[v] = to_f32<XT>(dh[i].e[v]) + after[v];
+          dg[v] = u[v] * before[i][v];
+          after[v] = g[i](v) * u[v];
+          sum += dg[v];
+        }
+        if ((in & 1) && A.dinitial != nullptr) store_state<V>(A.dinitial, A, in >> 2, p.c, after);
+      }
+      store_pack<XT, V>(reinterpret_cast<XT *>(A.dx) + row * A.channels + p.c, u);
+      if (SHARED) sums[(p.sg * R + i) * A.tx + p.tx] = sum;
+      else store_pack<GT, V>(reinterpret_cast<GT *>(A.dgate) + row * A.gates + p.c, dg);
+    }
+  }
+  if (!SHARED) return;
+  // The sums of the threads that share a gate, in their order.
+  __syncthreads();
+  const int c0 = cblk * A.tx * V, first = c0 / A.per_gate, count = (c1 - 1) / A.per_gate - first + 1;
+  const int64_t left = A.rows - p.t0;
+  const int rows = left < A.tile_rows ? (int)left : A.tile_rows;
+  for (int k = threadIdx.x; k < rows * count; k += kThreads) {
+    const int i = k / count, gate = first + k % count;
+    const int lo = gate * A.per_gate > c0 ? gate * A.per_gate : c0;
+    const int hi = (gate + 1) * A.per_gate < c1 ? (gate + 1) * A.per_gate : c1;
+    float sum = 0.f;
+    for (int c = lo; c < hi; c += V) sum += sums[i * A.tx + (c - c0) / V];
+    const int64_t t = p.t0 + i, row = A.reverse ? A.rows - 1 - t : t;
+    if (A.partial == nullptr) {
+      reinterpret_cast<GT *>(A.dgate)[row * A.gates + gate] = from_f32<GT>(sum);
+    } else {
+      const int slot = cblk - gate * A.per_gate / (A.tx * V);
+      A.partial[((int64_t)slot * A.rows + row) * A.gates + gate] = sum;
+    }
+  }
+}
+
+// The gates whose channels lie in several blocks: their parts added in order.
+template <typename GT>
+__global__ void __launch_bounds__(kThreads) join_gates_kernel(const Args A, int width) {
+  const int64_t n = A.rows * A.gates, stride = (int64_t)gridDim.x * kThreads;
+  for (int64_t k = (int64_t)blockIdx.x * kThreads + threadIdx.x; k < n; k += stride) {
+    const int gate = (int)(k % A.gates);
+    const int first = gate * A.per_gate / width, last = ((gate + 1) * A.per_gate - 1) / width;
+    float sum = 0.f;
+    for (int s = 0; s <= last - first; ++s) sum += A.partial[s * n + k];
+    reinterpret_cast<GT *>(A.dgate)[k] = from_f32<GT>(sum);
+  }
+}
+
+template <typename XT, typename GT, int V, int R, bool SHARED>
+static void launch_backward(const Args &A, cudaStream_t st) {
+  const unsigned grid = (unsigned)(A.tiles * A.channel_blocks);
+  if (A.carry != nullptr) {
+    backward_kernel<XT, GT, V, R, SHARED, true><<<grid, kThreads, 0, st>>>(A);
+    count_launch();
+    launch_carry(A, true, st);
+  }
+  backward_kernel<XT, GT, V, R, SHARED, false><<<grid, kThreads, 0, st>>>(A);
+  count_launch();
+  if (A.partial != nullptr && A.rows > 0) {
+    const int64_t want = (A.rows * A.gates + kThreads - 1) / kThreads;
+    join_gates_kernel<GT><<<(unsigned)(want < 1184 ? want : 1184), kThreads, 0, st>>>(A, A.tx * V);
+    count_launch();
+  }
+}
+
+template <typename XT, typename GT>
+static void pick_backward(const Args &A, int vec, cudaStream_t st) {
+  constexpr int kPer = 16 / (int)(sizeof(XT) > sizeof(GT) ? sizeof(XT) : sizeof(GT));
+  constexpr int kShared = 16 / (int)sizeof(XT);
+  const bool shared = A.per_gate > 1;
+  if (vec == 1 && shared) launch_backward<XT, GT, 1, kRowsScalar, true>(A, st);
+  else if (vec == 1) launch_backward<XT, GT, 1, kRowsScalar, false>(A, st);
+  else if (shared) launch_backward<XT, GT, kShared, kRowsVector, true>(A, st);
+  else launch_backward<XT, GT, kPer, kRowsVector, false>(A, st);
+}
+
+}  // namespace scan
+}  // namespace gs
+
+using namespace gs;
+using namespace gs::scan;
+
+extern "C" int gs_gated_scan_backward(int64_t rows, int sequences, int channels, int gates,
+                                      int x_type, int gate_type, const void *x,
+                                      int64_t x_row_stride, const void *gate,
+                                      int64_t gate_row_stride, const float *initial,
+                                      const int32_t *offsets, int reverse, const float *saved,
+                                      const void *grad_h, int64_t grad_h_row_stride,
+                                      const float *grad_final, void *grad_x, void *grad_gate,
+                                      float *grad_initial, void *scratch, size_t scratch_bytes,
+                                      void *stream) {
+  const int rc = check_shape(rows, sequences, channels, gates, x_type, gate_type, offsets);
+  if (rc) return rc;
+  if (rows > 0 && (x == nullptr || gate == nullptr || saved == nullptr || grad_x == nullptr ||
+                   grad_gate == nullptr))
+    return GS_ERR_INVALID_ARGUMENT;
+  const Plan p = make_plan(rows, channels, gates, x_type, gate_type);
+  const int xb = type_bytes(x_type), gb = type_bytes(gate_type);
+  const bool shared = channels != gates;
+  if (!suits(x, x_row_stride, xb, p.vec) || !suits(grad_x, channels, xb, p.vec) ||
+      !suits(grad_h, grad_h_row_stride, xb, p.vec) ||
+      !suits(gate, gate_row_stride, gb, shared ? 1 : p.vec) ||
+      !suits(grad_gate, gates, gb, shared ? 1 : p.vec) ||
+      (((uintptr_t)initial | (uintptr_t)grad_initial | (uintptr_t)grad_final | (uintptr_t)offsets |
+        (uintptr_t)saved) & 3))
+    return GS_ERR_INVALID_ARGUMENT;
+  Args A{};
+  fill_plan(A, p);
+  A.rows = rows;
+  A.sequences = sequences;
+  A.channels = channels;
+  A.gates = gates;
+  A.per_gate = channels / gates;
+  A.period = offsets == nullptr ? rows / sequences : 0;
+  A.offsets = offsets;
+  A.reverse = reverse != 0;
+  A.x = x;
+  A.x_stride = x_row_stride;
+  A.gate = gate;
+  A.gate_stride = gate_row_stride;
+  A.dh = grad_h;
+  A.dh_stride = grad_h_row_stride;
+  A.initial = initial;
+  A.dfinal = grad_final;
+  A.dx = grad_x;
+  A.dgate = grad_gate;
+  A.dinitial = grad_initial;
+  A.saved = const_cast<float *>(saved);
+  if (p.tiles > 1 || p.slots > 1) {
+    if (scratch == nullptr || ((uintptr_t)scratch & 15)) return GS_ERR_INVALID_ARGUMENT;
+    if (scratch_bytes < gs_gated_scan_scratch_bytes(rows, channels, gates, x_type, gate_type, 1))
+      return GS_ERR_CAPACITY;
+  }
+  if (p.tiles > 1) place_chains(A, p, scratch);
+  if (p.slots > 1)
+    A.partial = reinterpret_cast<float *>(static_cast<char *>(scratch) + chain_bytes(p, channels));
+  A.status = device_status_word();
+  if (A.status == nullptr) return GS_ERR_CUDA;
+  const bool same = x_type == gate_type;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (x_type == GS_TYPE_F32) pick_backward<float, float>(A, p.vec, st);
+  else if (x_type == GS_TYPE_BF16 && same) pick_backward<__nv_bfloat16, __nv_bfloat16>(A, p.vec, st);
+  else if (x_type == GS_TYPE_BF16) pick_backward<__nv_bfloat16, float>(A, p.vec, st);
+  else if (same) pick_backward<__half, __half>(A, p.vec, st);
+  else pick_backward<__half, float>(A, p.vec, st);
+  return launch_status();
+}

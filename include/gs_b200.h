@@ -42,6 +42,11 @@ extern "C" {
 #define GS_ERR_CAPACITY 4           /* scratch too small / count beyond 2^30 */
 #define GS_ERR_PEER 5               /* another rank reported an error in this step */
 
+/* ---- element types (gs_gated_scan_*, gs_orthogonalize, gs_muon_step) ---- */
+#define GS_TYPE_F32 0
+#define GS_TYPE_BF16 1
+#define GS_TYPE_F16 2
+
 /* Tile edge in pixels; the reference hard-codes 16 (src/cuda/wrapper.py:267). */
 #define GS_TILE 16
 
@@ -565,6 +570,57 @@ GS_API int gs_densify_apply(int n, const uint8_t *codes, const int32_t *pos_keep
  * the group's Adam moments (if given) zeroed. */
 GS_API int gs_reset_opacities(int n, float *opacity_logits, float *exp_avg, float *exp_avg_sq,
                               float threshold, void *stream);
+
+/* ---- gated linear recurrence -----------------------------------------------
+ * No counterpart in the reference. Over every sequence of a packed tensor of
+ * `rows` rows and `channels` channels,
+ *   h_t = g_t h_{t-1} + x_t,   h before the first row = initial,
+ * the gates per row dividing the channels: channel c takes gate
+ * c / (channels / gates). Sequence s is the rows offsets[s] .. offsets[s+1]-1
+ * (sequences + 1 ascending int32 row numbers in device memory; sequences may
+ * be empty), or with offsets NULL each rows / sequences rows. reverse = 1 runs
+ * every sequence from its last row to its first.
+ *
+ * x, h and grad_* of them are of type x_type, the gates of x_type or
+ * GS_TYPE_F32. initial and final_state (and their gradients) are fp32
+ * (sequences, channels); the recurrence is computed in fp32 and h rounded
+ * once. x, gate and grad_h have a stride of elements from row to row; outputs
+ * are contiguous. Rows outside every sequence are not read into a result and
+ * are written as zeros. Pointers and row strides are multiples of 16 bytes
+ * (8 where an 16-bit x goes with fp32 gates of one per channel) when the
+ * channels (with shared gates: the channels per gate) fill whole vectors of
+ * that size, otherwise of the element. rows <= INT32_MAX,
+ * sequences <= 2^28. Offsets that do not ascend within [0, rows] record
+ * GS_ERR_INVALID_ARGUMENT in the device status word; what is written then is
+ * undefined, but within the buffers. */
+
+/* What the forward keeps for the backward (the state before each of its
+ * tiles), and the scratch of either direction (0: none; 16-byte aligned). */
+GS_API size_t gs_gated_scan_saved_bytes(int64_t rows, int channels, int gates, int x_type,
+                                        int gate_type);
+GS_API size_t gs_gated_scan_scratch_bytes(int64_t rows, int channels, int gates, int x_type,
+                                          int gate_type, int backward);
+
+/* initial NULL: zeros. final_state NULL: not written. saved NULL: no backward
+ * follows. */
+GS_API int gs_gated_scan_forward(int64_t rows, int sequences, int channels, int gates, int x_type,
+                                 int gate_type, const void *x, int64_t x_row_stride,
+                                 const void *gate, int64_t gate_row_stride, const float *initial,
+                                 const int32_t *offsets, int reverse, void *h, float *final_state,
+                                 float *saved, void *scratch, size_t scratch_bytes, void *stream);
+
+/* The gradients of sum(grad_h h) + sum(grad_final final_state) (NULL: zeros),
+ * on the inputs and `saved` of the forward. grad_gate is summed over the
+ * channels that share a gate, in a fixed order. grad_initial NULL: not
+ * written. */
+GS_API int gs_gated_scan_backward(int64_t rows, int sequences, int channels, int gates, int x_type,
+                                  int gate_type, const void *x, int64_t x_row_stride,
+                                  const void *gate, int64_t gate_row_stride, const float *initial,
+                                  const int32_t *offsets, int reverse, const float *saved,
+                                  const void *grad_h, int64_t grad_h_row_stride,
+                                  const float *grad_final, void *grad_x, void *grad_gate,
+                                  float *grad_initial, void *scratch, size_t scratch_bytes,
+                                  void *stream);
 
 #ifdef __cplusplus
 }

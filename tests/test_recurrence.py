@@ -1,0 +1,380 @@
+"""The gated linear recurrence against its definition in 64 bits, row by row.
+
+Tolerances. With u = 2^-24, a state is a sum of products of at most 2 n + 2
+rounded operations each (n rows in its sequence: one product and one sum a
+row, whatever the order in which runs of rows are joined, and one more for
+each of the few levels of joining), so its error is at most
+(2 n + 16) u times the same recurrence run on absolute values. The gradient's
+chain has the same form, and a gate's gradient is a sum over D channels of
+products of the two: (4 n + 32 + D) u times the sum of absolute values.
+Rounding to the output's type adds half a step, eps / 2 of the value.
+"""
+import importlib
+
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def walk(x, g, init, bounds, reverse):
+    """h and the final states by the definition; x, g (rows, channels) in 64 bits."""
+    h, final = torch.zeros_like(x), init.clone()
+    for s, (a, b) in enumerate(bounds):
+        state = init[s].clone()
+        for t in (range(b - 1, a - 1, -1) if reverse else range(a, b)):
+            state = g[t] * state + x[t]
+            h[t] = state
+        final[s] = state
+    return h, final
+
+
+def walk_back(g, dh, dfinal, init, h, bounds, reverse):
+    dx, dg, dinit = torch.zeros_like(dh), torch.zeros_like(dh), torch.zeros_like(init)
+    for s, (a, b) in enumerate(bounds):
+        order = list(range(b - 1, a - 1, -1) if reverse else range(a, b))
+        v = dfinal[s].clone()
+        for k in range(len(order) - 1, -1, -1):
+            t = order[k]
+            dx[t] = dh[t] + v
+            dg[t] = dx[t] * (h[order[k - 1]] if k else init[s])
+            v = g[t] * dx[t]
+        dinit[s] = v
+    return dx, dg, dinit
+
+
+def bounds_of(rows, sequences, offsets):
+    if offsets is None:
+        n = rows // sequences
+        return [(s * n, (s + 1) * n) for s in range(sequences)]
+    return [(offsets[s], offsets[s + 1]) for s in range(len(offsets) - 1)]
+
+
+def near(name, got, ref, scale, ops, dtype):
+    got, half = got.detach().double().cpu(), torch.finfo(dtype).eps / 2
+    tol = 1.01 * ops * U * scale + half * (ref.abs() + ops * U * scale) + torch.finfo(dtype).tiny * half * 2
+    bad = (got - ref).abs() > tol
+    assert not bool(bad.any()), (f"{name}: {int(bad.sum())} of {bad.numel()} off, the first at "
+                                 f"{bad.nonzero()[0].tolist()}: {got[bad][0]} and not {ref[bad][0]}")
+
+
+def check(gs, rows, sequences, channels, gates, *, offsets=None, dtype=F32, gate_dtype=F32,
+          reverse=False, seed=0, with_initial=True, wrap=None, low=0.5, train=True):
+    gen = torch.Generator().manual_seed(seed)
+    per = channels // gates
+    x = torch.randn(rows, channels, generator=gen).to(dtype)
+    gate = (low + (1 - low) * torch.rand(rows, gates, generator=gen))
+    gate[torch.rand(rows, gates, generator=gen) < 0.05] = 0.0
+    gate[torch.rand(rows, gates, generator=gen) < 0.05] *= -1.0
+    gate = gate.to(gate_dtype)
+    init = torch.randn(sequences, channels, generator=gen) if with_initial else None
+    dh = torch.randn(rows, channels, generator=gen).to(dtype)
+    dfinal = torch.randn(sequences, channels, generator=gen)
+    bounds = bounds_of(rows, sequences, offsets)
+    shape = (rows,) if offsets is not None or sequences == 1 and wrap != "batch" else (sequences, rows // sequences)
+    on = {k: v.to(DEV) for k, v in (("x", x), ("gate", gate), ("dh", dh))}
+    on = {k: v.reshape(*shape, v.shape[-1]) for k, v in on.items()}
+    if wrap == "strided":  # columns of a wider tensor
+        wide = torch.zeros(*shape, 2 * channels + 2 * gates, dtype=dtype, device=DEV)
+        wide[..., :channels] = on["x"]
+        on["x"] = wide[..., :channels]
+        wide = torch.full((*shape, channels + 8), float("nan"), dtype=dtype, device=DEV)
+        wide[..., 3:3 + channels] = on["dh"]
+        on["dh"] = wide[..., 3:3 + channels]
+    leaves = [on["x"].detach().requires_grad_(train), on["gate"].detach().requires_grad_(train)]
+    if with_initial:
+        leaves.append(init.to(DEV).requires_grad_(train))
+    offs = None if offsets is None else torch.tensor(offsets, dtype=torch.int32, device=DEV)
+    h, final = gs.gated_scan(leaves[0], leaves[1], initial=leaves[2] if with_initial else None,
+                             offsets=offs, reverse=reverse)
+    assert h.dtype == dtype and final.dtype == F32 and h.shape == on["x"].shape
+    X, G, DH = x.double(), gate.double().repeat_interleave(per, 1), dh.double()
+    I = (init if with_initial else torch.zeros(sequences, channels)).double()
+    n = max([b - a for a, b in bounds], default=0)
+    ops = 2 * n + 16
+    H, FIN = walk(X, G, I, bounds, reverse)
+    HA, FA = walk(X.abs(), G.abs(), I.abs(), bounds, reverse)
+    near("h", h.reshape(rows, channels), H, HA, ops, dtype)
+    near("final", final, FIN, FA, ops, F32)
+    if not train:
+        return
+    grads = torch.autograd.grad((h, final), leaves, (on["dh"], dfinal.to(DEV)))
+    DX, DG, DI = walk_back(G, DH, dfinal.double(), I, H, bounds, reverse)
+    DXA, DGA, DIA = walk_back(G.abs(), DH.abs(), dfinal.double().abs(), I.abs(), HA, bounds, reverse)
+    near("dx", grads[0].reshape(rows, channels), DX, DXA, ops, dtype)
+    fold = lambda t: t.reshape(rows, gates, per).sum(2)  # noqa: E731
+    near("dgate", grads[1].reshape(rows, gates), fold(DG), fold(DGA), 4 * n + 32 + per, gate_dtype)
+    if with_initial:
+        near("dinitial", grads[2], DI, DIA, ops, F32)
+
+
+@gpu
+@pytest.mark.parametrize("rows,sequences", [(1, 1), (7, 7), (64, 2), (129, 1), (900, 3), (1500, 1)])
+@pytest.mark.parametrize("channels,gates", [(1, 1), (3, 1), (16, 16), (35, 1), (72, 72), (64, 4)])
+def test_batches_of_even_sequences(gs, rows, sequences, channels, gates):
+    check(gs, rows, sequences, channels, gates, seed=rows + channels)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,gate_dtype", [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)])
+@pytest.mark.parametrize("channels,gates", [(40, 40), (40, 1), (40, 5), (21, 21), (21, 7), (520, 2), (301, 1)])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_types_and_ragged_sequences(gs, dtype, gate_dtype, channels, gates, reverse):
+    # empty ones at both ends and in the middle, one row, ends inside and at the edge of tiles,
+    # rows behind the last
+    offsets = [0, 0, 1, 129, 129, 129, 257, 320, 321, 700, 700]
+    check(gs, 713, 10, channels, gates, offsets=offsets, dtype=dtype, gate_dtype=gate_dtype,
+          reverse=reverse, seed=channels)
+
+
+@gpu
+@pytest.mark.parametrize("reverse", [False, True])
+def test_rows_before_the_first_sequence_and_no_rows_inside(gs, reverse):
+    check(gs, 300, 2, 24, 24, offsets=[130, 135, 200], reverse=reverse)
+    check(gs, 300, 3, 24, 3, offsets=[300, 300, 300, 300], reverse=reverse)
+    check(gs, 5, 2, 24, 1, offsets=[2, 2, 2], reverse=reverse)
+
+
+@gpu
+def test_many_short_sequences(gs):
+    gen = torch.Generator().manual_seed(4)
+    cuts = torch.randint(0, 2000, (1499,), generator=gen).sort().values.tolist()
+    check(gs, 2000, 1500, 12, 12, offsets=[0] + cuts + [2000])
+    check(gs, 4096, 4096, 20, 4, train=True)  # one row each
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_strided_rows(gs, dtype):
+    for channels, gates in ((32, 32), (30, 3)):
+        check(gs, 400, 4, channels, gates, dtype=dtype, gate_dtype=dtype, wrap="strided")
+        check(gs, 400, 2, channels, gates, offsets=[0, 150, 390], dtype=dtype, wrap="strided")
+
+
+@gpu
+def test_no_initial_state_and_a_batch_of_one(gs):
+    check(gs, 260, 2, 16, 16, with_initial=False)
+    check(gs, 260, 1, 16, 2, with_initial=False, wrap="batch", reverse=True)
+
+
+@gpu
+def test_long_memory(gs):
+    check(gs, 6000, 1, 8, 8, low=0.999, seed=2)
+    check(gs, 6000, 2, 9, 1, low=0.999, seed=3, reverse=True)
+
+
+@gpu
+def test_other_layouts_give_the_same(gs):
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.randn(5, 70, 24, generator=gen, device=DEV)
+    g = torch.rand(5, 70, 24, generator=gen, device=DEV)
+    h, final = gs.gated_scan(x, g)
+    tx = x.transpose(0, 1).contiguous().transpose(0, 1)       # rows of a time-major tensor
+    tg = g.mT.contiguous().mT                                  # channels apart
+    h2, f2 = gs.gated_scan(tx, tg)
+    assert torch.equal(h, h2) and torch.equal(final, f2)
+    ge = g[..., :1].expand(-1, -1, 24)                         # a broadcast gate
+    leaf = g[..., :1].clone().requires_grad_(True)
+    h3, _ = gs.gated_scan(x, leaf.expand(-1, -1, 24))
+    h4, _ = gs.gated_scan(x, ge.contiguous())
+    assert torch.equal(h3, h4)
+    shared = g[..., :1].clone().requires_grad_(True)
+    h5, _ = gs.gated_scan(x, shared)
+    up = torch.randn(5, 70, 24, generator=gen, device=DEV)
+    (d1,), (d2,) = torch.autograd.grad(h3, leaf, up), torch.autograd.grad(h5, shared, up)
+    sizes = gs.gated_scan(x.abs(), shared.detach())[0].max() * gs.gated_scan(up.abs(), shared.detach())[0].max()
+    assert torch.equal(h3, h5)
+    assert float((d1 - d2).detach().abs().max()) <= 2 * (4 * 70 + 32 + 24) * U * 24 * float(sizes)
+    offs = torch.arange(0, 351, 70, device=DEV)                # int64 offsets of the same sequences
+    h6, f6 = gs.gated_scan(x.reshape(350, 24), g.reshape(350, 24), offsets=offs)
+    assert torch.equal(h6.reshape(5, 70, 24), h) and torch.equal(f6, final)
+    tail = torch.randn(351 * 24, device=DEV)[1:350 * 24 + 1].reshape(350, 24)  # not at 16 bytes
+    h7, _ = gs.gated_scan(tail, g.reshape(350, 24), offsets=offs)
+    h8, _ = gs.gated_scan(tail.clone(), g.reshape(350, 24), offsets=offs)
+    assert torch.equal(h7, h8)
+
+
+@gpu
+def test_a_row_at_a_time_continues_a_sequence(gs):
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(6, 40, 48, generator=gen, device=DEV)
+    g = torch.rand(6, 40, 48, generator=gen, device=DEV)
+    whole, end = gs.gated_scan(x, g)
+    state = torch.zeros(6, 48, device=DEV)
+    tol = 2 * (2 * 40 + 16) * U * float(gs.gated_scan(x.abs(), g)[0].max())
+    for t in range(40):
+        h, state = gs.gated_scan(x[:, t:t + 1], g[:, t:t + 1], initial=state)
+        assert torch.allclose(h[:, 0], whole[:, t], rtol=0, atol=tol)
+    assert torch.allclose(state, end, rtol=0, atol=tol)
+
+
+@gpu
+def test_nan_and_infinity_stay_in_their_sequence(gs):
+    for reverse in (False, True):
+        x = torch.ones(600, 16, device=DEV)
+        g = torch.full((600, 16), 0.5, device=DEV)
+        x[210, 3], x[100, 5], g[395, 7] = float("nan"), float("inf"), float("inf")
+        x[590:], g[590:] = float("nan"), float("nan")   # behind the last sequence
+        offs = torch.tensor([0, 200, 400, 590], dtype=torch.int32, device=DEV)
+        x.requires_grad_(True), g.requires_grad_(True)
+        h, final = gs.gated_scan(x, g, offsets=offs, reverse=reverse)
+        grads = torch.autograd.grad((h, final), (x, g), (torch.ones_like(h), torch.ones_like(final)))
+        whole = torch.isfinite(h)
+        for s, c in ((0, 5), (1, 3), (1, 7)):
+            assert not bool(whole[200 * s:200 * (s + 1), c].all()) and not bool(torch.isfinite(final[s, c]))
+            whole[200 * s:200 * (s + 1), c] = True
+        assert bool(whole.all()) and float(h[590:].abs().max()) == 0.0
+        for d in grads:
+            assert float(d[590:].abs().max()) == 0.0
+            assert bool(torch.isfinite(d[:, [0, 1, 2, 4, 6]]).all())
+
+
+@gpu
+def test_gradients_by_differences(gs):
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(90, 6, generator=gen, device=DEV)
+    g = 0.2 + 0.7 * torch.rand(90, 2, generator=gen, device=DEV)
+    init = torch.randn(4, 6, generator=gen, device=DEV)
+    offs = torch.tensor([0, 33, 33, 70, 88], device=DEV)
+    wh = torch.randn(90, 6, generator=gen, device=DEV)
+    wf = torch.randn(4, 6, generator=gen, device=DEV)
+
+    def loss(x, g, init):
+        h, final = gs.gated_scan(x, g, initial=init, offsets=offs, reverse=True)
+        return (h.double() * wh).sum() + (final.double() * wf).sum()
+
+    leaves = [t.clone().requires_grad_(True) for t in (x, g, init)]
+    grads = torch.autograd.grad(loss(*leaves), leaves)
+    for k, t in enumerate((x, g, init)):
+        way = torch.randn(t.shape, generator=gen, device=DEV)
+        step = 2.0 ** (-9 if k == 1 else -7)
+        ahead, back = [[v.clone() for v in (x, g, init)] for _ in range(2)]
+        ahead[k] += step * way
+        back[k] -= step * way
+        slope = float(loss(*ahead) - loss(*back)) / (2 * step)
+        told = float((grads[k].double() * way).sum())
+        # x and initial enter linearly; the gates' third derivative is what differences leave
+        assert abs(slope - told) <= (2e-2 if k == 1 else 2e-3) * (1 + abs(told)), (k, slope, told)
+
+
+@gpu
+def test_only_one_output_used_and_missing_gradients(gs):
+    x = torch.randn(3, 50, 8, device=DEV, requires_grad=True)
+    g = torch.rand(3, 50, 8, device=DEV)
+    h, final = gs.gated_scan(x, g)
+    (a,) = torch.autograd.grad(final.sum(), x, retain_graph=True)
+    (b,) = torch.autograd.grad(h.sum(), x, retain_graph=True)
+    (c,) = torch.autograd.grad(h.sum() + final.sum(), x)
+    assert torch.allclose(a + b, c, rtol=1e-5, atol=1e-5)
+    with torch.no_grad():
+        h, final = gs.gated_scan(x, g)
+    assert not h.requires_grad and not final.requires_grad
+
+
+@gpu
+def test_the_same_bits_every_time_and_from_a_graph(gs):
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.randn(20000, 40, generator=gen, device=DEV, requires_grad=True)
+    g = torch.rand(20000, 1, generator=gen, device=DEV, requires_grad=True)
+    offs = torch.tensor([0, 9000, 9001, 20000], dtype=torch.int32, device=DEV)
+    up = torch.randn(20000, 40, generator=gen, device=DEV)
+
+    def step():
+        h, final = gs.gated_scan(x, g, offsets=offs)
+        return (h, final) + torch.autograd.grad(h, (x, g), up)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ref = [t.clone() for t in step()]
+        again = step()
+        assert all(torch.equal(a, b) for a, b in zip(ref, again))
+        del again
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(3):
+        for t in out:
+            t.detach().fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(ref, out))
+
+
+@gpu
+def test_offsets_that_do_not_ascend_are_reported(gs):
+    """The kernels index within the buffers whatever the offsets hold (checked by reading: a
+    sequence number is below the count, a row below rows); the fault is in the status word."""
+    nat = importlib.import_module("3dgs_from_scratch_b200._native")
+    x = torch.randn(200, 8, device=DEV)
+    for offsets in ([0, 120, 60, 200], [0, 50, 201], [-3, 50, 200], [0, 2 ** 33, 200]):
+        assert nat.query("gs_check_status", nat.stream_ptr()) == 0
+        gs.gated_scan(x, x, offsets=torch.tensor(offsets, device=DEV))
+        assert nat.query("gs_check_status", nat.stream_ptr()) == nat.GS_ERR_INVALID_ARGUMENT
+        gs.gated_scan(x, x, offsets=torch.tensor([0, 60, 200], device=DEV))
+        assert nat.query("gs_check_status", nat.stream_ptr()) == 0
+
+
+@gpu
+def test_no_rows_and_no_sequences(gs):
+    x = torch.zeros(0, 6, device=DEV, requires_grad=True)
+    init = torch.randn(2, 6, device=DEV, requires_grad=True)
+    h, final = gs.gated_scan(x, x.detach(), initial=init, offsets=torch.zeros(3, dtype=torch.int32, device=DEV))
+    assert h.shape == (0, 6) and torch.equal(final, init)
+    dx, dinit = torch.autograd.grad(final.sum(), (x, init))
+    assert dx.shape == (0, 6) and bool((dinit == 1).all())
+    h, final = gs.gated_scan(torch.zeros(0, 5, 6, device=DEV), torch.zeros(0, 5, 2, device=DEV))
+    assert h.shape == (0, 5, 6) and final.shape == (0, 6)
+
+
+def test_refuses_what_it_cannot_run(gs):
+    x, g = torch.zeros(4, 6), torch.zeros(4, 6)
+    for bad in (lambda: gs.gated_scan(x, g),                                       # not on a GPU
+                lambda: gs.gated_scan(x[0], g[0]),
+                lambda: gs.gated_scan(x, g[:3]),
+                lambda: gs.gated_scan(x, torch.zeros(4, 4)),                       # 4 gates, 6 channels
+                lambda: gs.gated_scan(x, torch.zeros(4, 0)),
+                lambda: gs.gated_scan(x.double(), g.double()),
+                lambda: gs.gated_scan(x, g.half()),
+                lambda: gs.gated_scan(x[None], g[None], offsets=torch.zeros(2, dtype=torch.int32))):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@gpu
+def test_refuses_wrong_states_and_offsets(gs):
+    x, g = torch.zeros(4, 6, device=DEV), torch.zeros(4, 6, device=DEV)
+    offs = torch.tensor([0, 2, 4], device=DEV)
+    for kw in (dict(initial=torch.zeros(2, 6, device=DEV)), dict(initial=torch.zeros(1, 6)),
+               dict(initial=torch.zeros(1, 6, device=DEV, dtype=torch.int32)),
+               dict(offsets=offs.cpu()), dict(offsets=offs[:1]), dict(offsets=offs.float()),
+               dict(offsets=offs[None])):
+        with pytest.raises(ValueError):
+            gs.gated_scan(x, g, **kw)
+
+
+def test_entry_points_refuse_bad_arguments(gs):
+    lib = gs.load_native()
+    nat = importlib.import_module("3dgs_from_scratch_b200._native")
+    bad, P, at = nat.GS_ERR_INVALID_ARGUMENT, None, 0x10000
+
+    def fwd(rows=8, seqs=2, channels=8, gates=8, xt=0, gt=0, x=at, xs=8, gate=at, gst=8, init=P,
+            offs=P, h=at, scratch=P, nbytes=0):
+        return lib.gs_gated_scan_forward(rows, seqs, channels, gates, xt, gt, x, xs, gate, gst, init,
+                                         offs, 0, h, P, P, scratch, nbytes, P)
+
+    for kw in (dict(rows=-1), dict(rows=2 ** 31), dict(seqs=0), dict(seqs=3), dict(channels=0), dict(gates=0),
+               dict(gates=3), dict(xt=3), dict(xt=1, gt=2), dict(xt=0, gt=1), dict(x=P), dict(gate=P),
+               dict(h=P), dict(x=at + 4), dict(xs=9), dict(gst=10), dict(h=at + 8), dict(init=at + 2),
+               dict(offs=at + 2), dict(rows=2 ** 20)):       # many tiles and no scratch
+        assert fwd(**kw) == bad, kw
+    assert lib.gs_gated_scan_backward(8, 2, 8, 8, 0, 0, at, 8, at, 8, P, P, 0, P, at, 8, P, at, at, P,
+                                      P, 0, P) == bad         # nothing kept by the forward
+    assert lib.gs_gated_scan_saved_bytes(-1, 8, 8, 0, 0) == 0
+    assert lib.gs_gated_scan_saved_bytes(100, 8, 8, 0, 0) == 8 * 4
+    assert lib.gs_gated_scan_scratch_bytes(100, 8, 8, 0, 0, 0) == 0
+    assert lib.gs_gated_scan_scratch_bytes(1 << 20, 8, 8, 0, 0, 1) > 0
