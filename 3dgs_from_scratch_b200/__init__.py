@@ -11,11 +11,13 @@ importlib.import_module("3dgs_from_scratch_b200").
 from . import _native
 from . import cuda_rasterizer
 from . import scenes
+from .muon import muon_step, orthogonalize
 from .recurrence import gated_scan
 from .wrapper import ProjectPointsFunction, RasterizeFunction, SphericalHarmonicsFunction, render
 
 __all__ = ["render", "ProjectPointsFunction", "SphericalHarmonicsFunction", "RasterizeFunction",
-           "cuda_rasterizer", "scenes", "gated_scan", "load_native", "native_path"]
+           "cuda_rasterizer", "scenes", "gated_scan",
+           "orthogonalize", "muon_step", "load_native", "native_path"]
 
 
 def load_native():

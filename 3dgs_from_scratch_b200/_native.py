@@ -31,6 +31,7 @@ P = ctypes.c_void_p
 I = ctypes.c_int
 I64 = ctypes.c_int64
 F = ctypes.c_float
+D = ctypes.c_double
 SZ = ctypes.c_size_t
 
 # name -> (restype, argtypes); mirrors include/gs_b200.h
@@ -95,6 +96,9 @@ SIGNATURES = {
     "gs_gated_scan_forward": (I, [I64, I, I, I, I, I, P, I64, P, I64, P, P, I, P, P, P, P, SZ, P]),
     "gs_gated_scan_backward": (I, [I64, I, I, I, I, I, P, I64, P, I64, P, P, I, P, P, I64, P, P, P,
                                    P, P, SZ, P]),
+    "gs_orthogonalize_scratch_bytes": (SZ, [I, I, I, I]),
+    "gs_orthogonalize": (I, [I, I, I, I, P, I64, I64, I64, P, I, F, F, F, F, P, SZ, P]),
+    "gs_muon_step": (I, [I, I, I, I, P, P, P, D, D, I, D, D, I, F, F, F, F, P, SZ, P]),
     "gs_preprocess_backward": (I, [I, P, P, P, P, P, P, P, P, P, I, I, I, I, I, P, P, I, P, I, P,
                                    P, P, P, P, P, P]),
     "gs_preprocess_forward_views": (I, [I, I, P, P, P, P, P, P, P, P, P, F, F, F, F, F, I, I, I,

@@ -1,0 +1,666 @@
+// orthogonalize.cu -- an update matrix brought near its orthogonal factor by
+// Newton-Schulz products, and the optimizer step built on it.
+//
+// X0 = U / max(|U|_F, eps) (transposed where U is tall, so that X is m x n
+// with m <= n), then `steps` times
+//   A = X X^T;  B = b A + c A A;  X = a X + B X,
+// an odd quintic p(s) = a s + b s^3 + c s^5 on X's singular values.
+//
+// Numbers. The products run on the tensor cores with fp16 operands and fp32
+// accumulators. A value is held as hi + lo, two fp16 numbers (22 bits), scaled
+// by 2^12 so that neither leaves fp16's range: |X|_2 and |B|_2 stay below 8
+// (checked by the host for the given coefficients), and a typical entry of
+// even the largest matrix is far above the smallest normal number.
+//   full (fp32 and fp16 results): every product is hi hi + hi lo + lo hi. The
+//     tensor core cuts its fp32 sums off instead of rounding them, a bias that
+//     grows with the number of additions (2.6e-5 of the result at 4096 x 4096
+//     with one accumulator for all of K); so each 256 elements of K start a
+//     fresh accumulator, and these parts are added in registers, rounded.
+//   half (bf16 results, 2^-9 a rounding): A and B are computed from and held
+//     as hi alone. Their errors (2^-12) multiply each singular direction by
+//     1 + small and mix left directions only, so a small singular value keeps
+//     its relative accuracy; X's own rounding would not do that (it adds to
+//     every direction alike, and the small ones grow 3.4-fold a step), so X
+//     keeps hi + lo in a X + B X. Two products there, one in A and in A A.
+//
+// Layout. Every matrix lies in the workspace as 128 x 64 blocks of fp16, each
+// the 16 KB image of 128 rows of 128 bytes in the tensor core's 128-byte
+// swizzle (16-byte chunk j of row r at chunk j ^ (r & 7)). A block is fetched
+// with one contiguous bulk copy, and the same image serves as a K-major
+// operand (rows along M or N) and, 64 of its rows at a time, as an MN-major
+// one (rows along K): X needs no transposed copy, and of the symmetric A and
+// B only the blocks on and above the diagonal are computed and stored, the
+// others read as their mirror images.
+//
+// Padding to whole blocks is zero from the start and stays zero.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "tcgen05.cuh"
+
+namespace gs {
+namespace ns {
+
+constexpr int kBlockBytes = 128 * 64 * 2;
+constexpr int kEpilogueWarps = 8;  // two for each quarter of tensor memory's lanes
+constexpr int kMaxStages = 8;
+constexpr float kScale = 4096.f, kUnscale = 1.f / 4096.f;
+
+enum Kind { kGram, kSquare, kApply };
+
+struct Matrix {        // planes of blocks [row block][column block]
+  char *hi, *lo;       // lo may be null
+  int64_t batch_bytes;
+  int column_blocks;
+};
+
+struct Out {
+  void *p;             // the result, or the weights that it updates; null: none
+  int type;            // GS_TYPE_*
+  int update;          // p = decay p - step X instead of p = X; skipped like the momentum
+                       // while the device status word is set
+  int tall;            // X is the transpose
+  int rows, cols;      // of X
+  int64_t batch_stride;
+  float decay, step;
+};
+
+struct Args {
+  Matrix x, y, sq, poly;  // X, the next X, A, B
+  int row_blocks, column_blocks;  // of 128 rows and of 64 columns, X
+  int k_blocks_n, k_blocks_m;     // 64-wide K blocks that hold data
+  int stages;
+  float a, b, c;
+  Out out;
+  uint32_t *status;
+};
+
+__device__ __forceinline__ char *block_at(char *plane, const Matrix &M, int batch, int rb, int cb) {
+  return plane + (int64_t)batch * M.batch_bytes + ((int64_t)rb * M.column_blocks + cb) * kBlockBytes;
+}
+
+// Byte of the 16-byte chunk that holds columns col..col+7 of row r in a block.
+__device__ __forceinline__ int chunk_at(int r, int col) {
+  return r * 128 + ((((col & 63) >> 3) ^ (r & 7)) << 4);
+}
+
+// One plane's rows of an operand: `rows` rows from `row` on, K block kb, into
+// shared memory. Above or on the diagonal (of blocks of `tri`) of a symmetric
+// matrix, and always for X, as K-major rows; below it as the mirror image,
+// MN-major. Returns the bytes that will arrive.
+__device__ __forceinline__ uint32_t fetch_rows(char *plane, const Matrix &M, int batch, int row,
+                                               int rows, int kb, bool mirrored, char *dst,
+                                               uint64_t *bar) {
+  if (!mirrored) {
+    if (rows < 128) {
+      bulk_load(dst, block_at(plane, M, batch, row / 128, kb) + (row % 128) * 128, rows * 128, bar);
+    } else {
+      for (int u = 0; u < rows / 128; ++u)
+        bulk_load(dst + u * kBlockBytes, block_at(plane, M, batch, row / 128 + u, kb), kBlockBytes, bar);
+    }
+  } else {
+    for (int u = 0; u < rows / 64; ++u)
+      bulk_load(dst + u * (kBlockBytes / 2),
+                block_at(plane, M, batch, kb / 2, row / 64 + u) + (kb & 1) * (kBlockBytes / 2),
+                kBlockBytes / 2, bar);
+  }
+  return rows * 128;
+}
+
+__device__ __forceinline__ uint64_t operand(uint32_t addr, bool mn, int k) {
+  // 16 elements of K further: 32 bytes along a row, or 16 rows of 128 bytes
+  return mn ? tc::descriptor(addr + k * 2048, kBlockBytes / 2, 1024)
+            : tc::descriptor(addr + k * 32, 16, 1024);
+}
+
+__device__ __forceinline__ void split8(const float *v, uint4 &hi, uint4 &lo) {
+  __half h[8], l[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    h[i] = __float2half_rn(v[i]);
+    l[i] = __float2half_rn(v[i] - __half2float(h[i]));
+  }
+  hi = *reinterpret_cast<uint4 *>(h);
+  lo = *reinterpret_cast<uint4 *>(l);
+}
+
+__device__ __forceinline__ void add8(const uint4 &q, float (&v)[8]) {
+  const __half *h = reinterpret_cast<const __half *>(&q);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] += __half2float(h[i]);
+}
+
+__device__ __forceinline__ void store_result(const Out &o, int batch, int row, int col, float v) {
+  if (row >= o.rows || col >= o.cols) return;
+  const int64_t at = (int64_t)batch * o.batch_stride +
+                     (o.tall ? (int64_t)col * o.rows + row : (int64_t)row * o.cols + col);
+  if (o.update) {
+    float *w = reinterpret_cast<float *>(o.p);
+    w[at] = fmaf(o.decay, w[at], -o.step * v);
+  } else if (o.type == GS_TYPE_F32) {
+    reinterpret_cast<float *>(o.p)[at] = v;
+  } else if (o.type == GS_TYPE_BF16) {
+    reinterpret_cast<__nv_bfloat16 *>(o.p)[at] = __float2bfloat16_rn(v);
+  } else {
+    reinterpret_cast<__half *>(o.p)[at] = __float2half_rn(v);
+  }
+}
+
+template <int BN, int KIND, bool FULL>
+struct Shape {
+  static constexpr int kPlanesA = FULL ? 2 : 1;
+  static constexpr int kPlanesB = FULL || KIND == kApply ? 2 : 1;
+  static constexpr int kStage = (kPlanesA * 128 + kPlanesB * BN) * 128;
+  static constexpr int kTri = BN > 128 ? BN : 128;
+  static constexpr int kChunk = FULL ? 4 : 1 << 30;        // K blocks of an accumulator
+  // Where there is room, hi lo + lo hi have an accumulator of their own: far
+  // fewer cut-off additions to the large one (128 x 64 in fp32: the result's
+  // error 2.3e-6 -> 1.2e-6, as fp32 products have).
+  static constexpr bool kCross = FULL && BN <= 128;
+  static constexpr int kWidth = kCross ? 2 * BN : BN;        // columns of tensor memory
+  static constexpr int kColumns = FULL ? 2 * kWidth : kWidth;  // two take turns
+  // A copy warp, an MMA warp and the epilogue. Where an epilogue thread holds
+  // 128 sums, a whole warpgroup goes to the first two, so that it can hand its
+  // registers over: 384 threads x 168 = 128 x 40 + 256 x 232.
+  static constexpr bool kHandOver = FULL && BN == 256;
+  static constexpr int kEpilogue = kHandOver ? 4 : 2;      // its first warp
+  static constexpr int kThreads = 32 * (kEpilogue + kEpilogueWarps);
+};
+
+template <int BN, int KIND, bool FULL>
+__global__ void __launch_bounds__(Shape<BN, KIND, FULL>::kThreads, 1) product_kernel(const Args A) {
+  using S = Shape<BN, KIND, FULL>;
+  extern __shared__ char raw[];
+  char *smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], ready[2], drained[2];
+  __shared__ uint32_t tmem_base, failed;
+  const int warp = threadIdx.x / 32, batch = blockIdx.y;
+  int i, j;  // the tile: rows 128 i.., columns BN j..
+  if (KIND == kApply) {
+    i = blockIdx.x % A.row_blocks;
+    j = blockIdx.x / A.row_blocks;
+  } else {  // column j of tiles holds the rows down to its diagonal block
+    int left = blockIdx.x, rows;
+    for (j = 0;; ++j) {
+      rows = (j * BN / S::kTri + 1) * (S::kTri / 128);
+      if (left < rows) break;
+      left -= rows;
+    }
+    i = left;
+  }
+  const int k_blocks = KIND == kGram ? A.k_blocks_n : A.k_blocks_m;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < A.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&ready[s], 1);
+      mbar_init(&drained[s], kEpilogueWarps);
+    }
+    failed = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tc::tmem_alloc(&tmem_base, S::kColumns);
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = tmem_base;
+  // Whether a K block of a symmetric matrix lies below the diagonal of rows.
+  const auto below = [&](int row, int kb) { return KIND != kGram && kb * 64 / S::kTri < row / S::kTri; };
+
+  if (S::kHandOver && warp < S::kEpilogue) tc::registers_down<40>();
+  if (warp == 0 && lane_id() == 0) {
+    const Matrix &MA = KIND == kGram ? A.x : KIND == kSquare ? A.sq : A.poly;
+    const Matrix &MB = KIND == kSquare ? A.sq : A.x;
+    int kb = 0;
+    for (; kb < k_blocks; ++kb) {
+      const int s = kb % A.stages, round = kb / A.stages;
+      if (round > 0 && !mbar_wait(&empty[s], (round - 1) & 1)) {
+        failed = 1;
+        break;
+      }
+      char *a = smem + (size_t)s * S::kStage, *b = a + S::kPlanesA * 128 * 128;
+      mbar_expect_tx(&full[s], S::kStage);
+      for (int q = 0; q < S::kPlanesA; ++q)
+        fetch_rows(q ? MA.lo : MA.hi, MA, batch, i * 128, 128, kb, below(i * 128, kb),
+                   a + q * 128 * 128, &full[s]);
+      for (int q = 0; q < S::kPlanesB; ++q)
+        fetch_rows(q ? MB.lo : MB.hi, MB, batch, j * BN, BN, kb,
+                   KIND == kApply || (KIND == kSquare && below(j * BN, kb)), b + q * BN * 128, &full[s]);
+    }
+    if (kb < k_blocks)  // given up: the copies in flight still land here
+      for (int q = kb > A.stages ? kb - A.stages : 0; q < kb; ++q)
+        mbar_wait(&full[q % A.stages], (q / A.stages) & 1);
+  } else if (warp == 1 && lane_id() == 0) {
+    for (int kb = 0; kb < k_blocks; ++kb) {
+      const int s = kb % A.stages, chunk = kb / S::kChunk, acc = chunk & 1;
+      const bool fresh = kb % S::kChunk == 0;
+      if (!mbar_wait(&full[s], (kb / A.stages) & 1) ||
+          (fresh && chunk >= 2 && !mbar_wait(&drained[acc], (chunk / 2 - 1) & 1))) {
+        failed = 1;
+        break;
+      }
+      tc::fence_after();
+      const uint32_t a = smem_addr(smem + (size_t)s * S::kStage), b = a + S::kPlanesA * 128 * 128;
+      const bool a_mn = below(i * 128, kb), b_mn = KIND == kApply || (KIND == kSquare && below(j * BN, kb));
+      const uint32_t instr = tc::instruction_f16(128, BN, a_mn, b_mn);
+#pragma unroll
+      for (int q = 0; q < (FULL ? 3 : S::kPlanesB); ++q) {  // hi hi, hi lo, lo hi
+        const uint32_t aq = a + (q == 2 ? 128 * 128 : 0), bq = b + (q == 1 ? BN * 128 : 0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          tc::mma_f16(tmem + acc * S::kWidth + (S::kCross && q > 0 ? BN : 0), operand(aq, a_mn, k),
+                      operand(bq, b_mn, k), instr, !(fresh && k == 0 && (q == 0 || (S::kCross && q == 1))));
+      }
+      tc::commit(&empty[s]);
+      if (kb % S::kChunk == S::kChunk - 1 || kb == k_blocks - 1) tc::commit(&ready[acc]);
+    }
+  } else if (warp >= S::kEpilogue) {
+    if (S::kHandOver) tc::registers_up<232>();
+    const int quarter = warp & 3;  // the lanes of tensor memory that the warp may read
+    const int r = quarter * 32 + (int)lane_id(), row = i * 128 + r;
+    const int c0 = (warp - S::kEpilogue) / 4 * (BN / 2);
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + c0;
+    float v[BN / 2];
+    const int chunks = (k_blocks + S::kChunk - 1) / S::kChunk;
+    bool good = true;
+    for (int chunk = 0; chunk < chunks && good; ++chunk) {
+      const int acc = chunk & 1;
+      good = mbar_wait(&ready[acc], (chunk / 2) & 1);
+      if (!good) break;
+      tc::fence_after();
+#pragma unroll
+      for (int c = 0; c < BN / 2; c += 32) {
+        float part[32];
+        tc::load_columns(lanes + acc * S::kWidth + c, part);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[c + e] = chunk == 0 ? part[e] : v[c + e] + part[e];
+        if (S::kCross) {
+          tc::load_columns(lanes + acc * S::kWidth + BN + c, part);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[c + e] += part[e];
+        }
+      }
+      if (chunk + 2 < chunks) {
+        tc::fence_before();
+        __syncwarp();
+        if (lane_id() == 0) tc::arrive(&drained[acc]);
+      }
+    }
+    if (!good) {
+      failed = 1;
+    } else if (!A.out.update || ld_volatile_u32(A.status) == 0u) {  // the optimizers' gate
+      const Matrix &dst = KIND == kGram ? A.sq : KIND == kSquare ? A.poly : A.y;
+      const Matrix &old = KIND == kSquare ? A.sq : A.x;
+#pragma unroll
+      for (int g = 0; g < BN / 2; g += 8) {
+        const int col = j * BN + c0 + g, at = chunk_at(r, col);
+        float w[8];
+        if (KIND == kGram) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = v[g + e] * kUnscale;
+        } else {
+          float o[8] = {};
+          add8(*reinterpret_cast<const uint4 *>(block_at(old.hi, old, batch, i, col / 64) + at), o);
+          if (FULL || KIND == kApply)
+            add8(*reinterpret_cast<const uint4 *>(block_at(old.lo, old, batch, i, col / 64) + at), o);
+          const float p = KIND == kSquare ? A.b : A.a, q = KIND == kSquare ? A.c * kUnscale : kUnscale;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = fmaf(p, o[e], q * v[g + e]);
+        }
+        if (KIND == kApply && A.out.p != nullptr) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) store_result(A.out, batch, row, col + e, w[e] * kUnscale);
+        } else {
+          uint4 hi, lo;
+          split8(w, hi, lo);
+          *reinterpret_cast<uint4 *>(block_at(dst.hi, dst, batch, i, col / 64) + at) = hi;
+          if (FULL || KIND == kApply)
+            *reinterpret_cast<uint4 *>(block_at(dst.lo, dst, batch, i, col / 64) + at) = lo;
+        }
+      }
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && failed) atomicCAS(A.status, 0u, (uint32_t)GS_ERR_DEVICE_TIMEOUT);
+  if (warp == 1) {
+    tc::fence_after();
+    tc::tmem_free(tmem, S::kColumns);
+  }
+}
+
+// ---- the update: what is orthogonalised -------------------------------------------
+
+struct Source {
+  const void *u;          // the update, or the gradient that feeds the momentum
+  int type;
+  int64_t batch_stride, row_stride, col_stride;  // of X's rows and columns
+  float *momentum;        // contiguous like the gradient; null: u is the update
+  float beta, fresh;      // fresh = 1 - beta, from 64 bits
+  int nesterov;
+  int rows, cols;         // of X
+};
+
+__device__ __forceinline__ float read_f32(const void *p, int type, int64_t at) {
+  return type == GS_TYPE_F32 ? reinterpret_cast<const float *>(p)[at]
+         : type == GS_TYPE_BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[at])
+                                : __half2float(reinterpret_cast<const __half *>(p)[at]);
+}
+
+// M = beta M + (1 - beta) G and what of it is orthogonalised, rounded alike in
+// both kernels that need it.
+__device__ __forceinline__ float next_momentum(const Source &s, float m, float g) {
+  return fmaf(s.beta, m, s.fresh * g);
+}
+__device__ __forceinline__ float update_of(const Source &s, float m_new, float g) {
+  return s.nesterov ? fmaf(s.beta, m_new, s.fresh * g) : m_new;
+}
+
+constexpr int kNormThreads = 256, kMaxParts = 256;
+
+// Sums of squares, in 64 bits so that neither tiny nor huge gradients leave
+// the range; the momentum is updated on the way. Parts are added in order by
+// the reader.
+__global__ void __launch_bounds__(kNormThreads) norm_kernel(const Source s, double *parts,
+                                                            const uint32_t *status) {
+  if (s.momentum != nullptr && ld_volatile_u32(status) != 0u) return;
+  const int64_t size = (int64_t)s.rows * s.cols, base = (int64_t)blockIdx.y * s.batch_stride;
+  // elements in the order of memory: the smaller stride runs fastest
+  const bool cols_fast = s.col_stride <= s.row_stride;
+  const int64_t fast = cols_fast ? s.cols : s.rows;
+  const int64_t fs = cols_fast ? s.col_stride : s.row_stride, ss = cols_fast ? s.row_stride : s.col_stride;
+  double sum = 0.0;
+  for (int64_t k = (int64_t)blockIdx.x * kNormThreads + threadIdx.x; k < size;
+       k += (int64_t)gridDim.x * kNormThreads) {
+    const int64_t at = base + (k / fast) * ss + (k % fast) * fs;
+    float v = read_f32(s.u, s.type, at);
+    if (s.momentum != nullptr) {
+      const float m = next_momentum(s, s.momentum[at], v);
+      s.momentum[at] = m;
+      v = update_of(s, m, v);
+    }
+    sum = fma((double)v, (double)v, sum);
+  }
+  __shared__ double warps[kNormThreads / 32];
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_down_sync(0xffffffffu, sum, d);
+  if (lane_id() == 0) warps[threadIdx.x / 32] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kNormThreads / 32; ++w) sum += warps[w];
+    parts[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = sum;
+  }
+}
+
+// X0, 64 x 64 elements a block, scaled and split into the workspace's layout.
+__global__ void __launch_bounds__(256) split_kernel(const Source s, const double *parts, int num_parts,
+                                                    double eps, Matrix x, int column_blocks) {
+  __shared__ float tile[64][65];
+  __shared__ double total;
+  const int batch = blockIdx.y, r0 = blockIdx.x / column_blocks * 64, c0 = blockIdx.x % column_blocks * 64;
+  if (threadIdx.x < 32) {
+    double sum = 0.0;
+    for (int k = threadIdx.x; k < num_parts; k += 32) sum += parts[(int64_t)batch * num_parts + k];
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_down_sync(0xffffffffu, sum, d);
+    if (threadIdx.x == 0) {
+      const double norm = sqrt(sum);
+      total = (double)kScale / (norm < eps ? eps : norm);
+    }
+  }
+  __syncthreads();
+  const double scale = total;
+  const bool cols_fast = s.col_stride <= s.row_stride;
+  for (int k = threadIdx.x; k < 64 * 64; k += 256) {
+    const int r = cols_fast ? k / 64 : k % 64, c = cols_fast ? k % 64 : k / 64;
+    float v = 0.f;
+    if (r0 + r < s.rows && c0 + c < s.cols) {
+      const int64_t at = (int64_t)batch * s.batch_stride + (r0 + r) * s.row_stride + (c0 + c) * s.col_stride;
+      v = read_f32(s.u, s.type, at);
+      if (s.momentum != nullptr) v = update_of(s, s.momentum[at], v);
+      v = (float)((double)v * scale);
+    }
+    tile[r][c] = v;
+  }
+  __syncthreads();
+  for (int k = threadIdx.x; k < 64 * 8; k += 256) {
+    const int r = k / 8, c = k % 8 * 8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = tile[r][c + e];
+    uint4 hi, lo;
+    split8(v, hi, lo);
+    const int at = chunk_at((r0 + r) % 128, c);
+    *reinterpret_cast<uint4 *>(block_at(x.hi, x, batch, (r0 + r) / 128, c0 / 64) + at) = hi;
+    *reinterpret_cast<uint4 *>(block_at(x.lo, x, batch, (r0 + r) / 128, c0 / 64) + at) = lo;
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------
+
+struct Plan {
+  int m, n, bn;             // X is m x n, tiles are 128 x bn
+  int row_blocks, column_blocks, sq_column_blocks;
+  bool full;
+  int parts;
+  size_t x_bytes, sq_bytes, total;  // of a plane and of everything, all batches
+};
+
+static Plan make_plan(int batch, int rows, int cols, int type) {
+  Plan p;
+  p.m = rows < cols ? rows : cols;
+  p.n = rows < cols ? cols : rows;
+  p.full = type != GS_TYPE_BF16;
+  const auto tiles = [&](int bn) { return (int64_t)batch * ((p.m + 127) / 128) * ((p.n + bn - 1) / bn); };
+  p.bn = tiles(256) >= 148 ? 256 : tiles(128) >= 148 ? 128 : 64;
+  const int tri = p.bn > 128 ? p.bn : 128;
+  const int mp = (p.m + tri - 1) / tri * tri, np = (p.n + p.bn - 1) / p.bn * p.bn;
+  p.row_blocks = mp / 128;
+  p.column_blocks = np / 64;
+  p.sq_column_blocks = mp / 64;
+  const int64_t size = (int64_t)rows * cols;
+  const int64_t parts = (size + 8191) / 8192;
+  p.parts = (int)(parts < kMaxParts ? parts : kMaxParts);
+  p.x_bytes = (size_t)batch * p.row_blocks * p.column_blocks * kBlockBytes;
+  p.sq_bytes = (size_t)batch * p.row_blocks * p.sq_column_blocks * kBlockBytes;
+  p.total = 4 * p.x_bytes + (p.full ? 4 : 2) * p.sq_bytes + (size_t)batch * p.parts * 8;
+  return p;
+}
+
+template <int BN, int KIND, bool FULL>
+static int launch_product(Args A, int tiles, int batch, cudaStream_t st) {
+  using S = Shape<BN, KIND, FULL>;
+  A.stages = (220 * 1024) / S::kStage;
+  if (A.stages > kMaxStages) A.stages = kMaxStages;
+  const int bytes = A.stages * S::kStage + 1024;
+  thread_local unsigned long long ready = 0;  // the context whose kernel has its shared memory set
+  const unsigned long long ctx = current_context_id();
+  if (ctx == 0 || ctx != ready) {
+    const int rc = cuda_status(cudaFuncSetAttribute(product_kernel<BN, KIND, FULL>,
+                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (rc) return rc;
+    ready = ctx != 0 ? ctx : current_context_id();
+  }
+  product_kernel<BN, KIND, FULL><<<dim3(tiles, batch), S::kThreads, bytes, st>>>(A);
+  count_launch();
+  return launch_status();
+}
+
+template <int BN, bool FULL>
+static int run_steps(Args A, const Plan &p, int batch, int steps, const Out &out, cudaStream_t st) {
+  int tri_tiles = 0;
+  constexpr int kTri = BN > 128 ? BN : 128;
+  for (int j = 0; j < p.sq_column_blocks * 64 / BN; ++j) tri_tiles += (j * BN / kTri + 1) * (kTri / 128);
+  for (int k = 0; k < steps; ++k) {
+    A.out = out;
+    if (k + 1 < steps) A.out.p = nullptr;
+    int rc = launch_product<BN, kGram, FULL>(A, tri_tiles, batch, st);
+    if (!rc) rc = launch_product<BN, kSquare, FULL>(A, tri_tiles, batch, st);
+    if (!rc) rc = launch_product<BN, kApply, FULL>(A, p.row_blocks * p.column_blocks * 64 / BN, batch, st);
+    if (rc) return rc;
+    const Matrix x = A.x;
+    A.x = A.y;
+    A.y = x;
+  }
+  return GS_OK;
+}
+
+// The largest |X|_2 and |b A + c A A|_2 that the steps can reach from
+// |X|_2 <= 1, from the extremes of the two polynomials on [0, r]. Both have to
+// stay below 8 for the fp16 range.
+static bool in_range(int steps, double a, double b, double c) {
+  double r = 1.0;
+  for (int k = 0; k < steps; ++k) {
+    const auto p = [&](double s) { return fabs(s * (a + s * s * (b + s * s * c))); };
+    const auto q = [&](double y) { return fabs(y * (b + y * c)); };
+    double most = p(r), poly = q(r * r);
+    // p'(s) = a + 3 b s^2 + 5 c s^4
+    const double disc = 9 * b * b - 20 * a * c;
+    if (c != 0 && disc >= 0)
+      for (int sign = -1; sign <= 1; sign += 2) {
+        const double y = (-3 * b + sign * sqrt(disc)) / (10 * c);
+        if (y > 0 && y < r * r) most = fmax(most, p(sqrt(y)));
+      }
+    else if (c == 0 && b != 0 && -a / (3 * b) > 0 && -a / (3 * b) < r * r)
+      most = fmax(most, p(sqrt(-a / (3 * b))));
+    if (c != 0 && -b / (2 * c) > 0 && -b / (2 * c) < r * r) poly = fmax(poly, q(-b / (2 * c)));
+    if (!(most < 8.0) || !(poly < 8.0)) return false;
+    r = fmax(most, 1.0);
+  }
+  return true;
+}
+
+static int run(int batch, const Plan &p, const Source &src, const Out &out, int steps, float a, float b,
+               float c, float eps, void *scratch, size_t scratch_bytes, cudaStream_t st) {
+  if (scratch == nullptr || ((uintptr_t)scratch & 15)) return GS_ERR_INVALID_ARGUMENT;
+  if (scratch_bytes < p.total) return GS_ERR_CAPACITY;
+  Args A{};
+  A.status = device_status_word();
+  if (A.status == nullptr) return GS_ERR_CUDA;
+  char *at = static_cast<char *>(scratch);
+  const auto take = [&](size_t n) {
+    char *q = at;
+    at += n;
+    return q;
+  };
+  const int64_t xb = (int64_t)(p.x_bytes / batch), sb = (int64_t)(p.sq_bytes / batch);
+  A.x = {take(p.x_bytes), take(p.x_bytes), xb, p.column_blocks};
+  A.y = {take(p.x_bytes), take(p.x_bytes), xb, p.column_blocks};
+  A.sq = {take(p.sq_bytes), p.full ? take(p.sq_bytes) : nullptr, sb, p.sq_column_blocks};
+  A.poly = {take(p.sq_bytes), p.full ? take(p.sq_bytes) : nullptr, sb, p.sq_column_blocks};
+  double *parts = reinterpret_cast<double *>(at);
+  A.row_blocks = p.row_blocks;
+  A.column_blocks = p.column_blocks;
+  A.k_blocks_n = (p.n + 63) / 64;
+  A.k_blocks_m = (p.m + 63) / 64;
+  A.a = a;
+  A.b = b;
+  A.c = c;
+  norm_kernel<<<dim3(p.parts, batch), kNormThreads, 0, st>>>(src, parts, A.status);
+  split_kernel<<<dim3(p.row_blocks * 2 * p.column_blocks, batch), 256, 0, st>>>(
+      src, parts, p.parts, (double)eps, A.x, p.column_blocks);
+  count_launch(2);
+  int rc = launch_status();
+  if (rc) return rc;
+  if (p.full)
+    return p.bn == 256   ? run_steps<256, true>(A, p, batch, steps, out, st)
+           : p.bn == 128 ? run_steps<128, true>(A, p, batch, steps, out, st)
+                         : run_steps<64, true>(A, p, batch, steps, out, st);
+  return p.bn == 256   ? run_steps<256, false>(A, p, batch, steps, out, st)
+         : p.bn == 128 ? run_steps<128, false>(A, p, batch, steps, out, st)
+                       : run_steps<64, false>(A, p, batch, steps, out, st);
+}
+
+static bool known_type(int type) {
+  return type == GS_TYPE_F32 || type == GS_TYPE_BF16 || type == GS_TYPE_F16;
+}
+
+static int check(int batch, int rows, int cols, int type, int steps, float a, float b, float c, float eps) {
+  if (batch < 1 || batch > 65535 || rows < 1 || cols < 1 || rows > (1 << 24) || cols > (1 << 24) ||
+      (rows < cols ? rows : cols) > (1 << 15) || !known_type(type) || steps < 1 || steps > 100 ||
+      !(eps > 0.f) || !in_range(steps, a, b, c))
+    return GS_ERR_INVALID_ARGUMENT;
+  return GS_OK;
+}
+
+}  // namespace ns
+}  // namespace gs
+
+using namespace gs;
+using namespace gs::ns;
+
+extern "C" size_t gs_orthogonalize_scratch_bytes(int batch, int rows, int cols, int type) {
+  if (check(batch, rows, cols, type, 1, 1.f, 0.f, 0.f, 1.f)) return 0;
+  return make_plan(batch, rows, cols, type).total;
+}
+
+extern "C" int gs_orthogonalize(int batch, int rows, int cols, int type, const void *update,
+                                int64_t batch_stride, int64_t row_stride, int64_t col_stride, void *out,
+                                int steps, float a, float b, float c, float eps, void *scratch,
+                                size_t scratch_bytes, void *stream) {
+  const int rc = check(batch, rows, cols, type, steps, a, b, c, eps);
+  if (rc) return rc;
+  const int mask = type == GS_TYPE_F32 ? 3 : 1;
+  if (update == nullptr || out == nullptr || (((uintptr_t)update | (uintptr_t)out) & mask) ||
+      batch_stride < 0 || row_stride < 0 || col_stride < 0)
+    return GS_ERR_INVALID_ARGUMENT;
+  const Plan p = make_plan(batch, rows, cols, type);
+  const bool tall = rows > cols;
+  Source s{};
+  s.u = update;
+  s.type = type;
+  s.batch_stride = batch_stride;
+  s.row_stride = tall ? col_stride : row_stride;
+  s.col_stride = tall ? row_stride : col_stride;
+  s.rows = p.m;
+  s.cols = p.n;
+  Out o{};
+  o.p = out;
+  o.type = type;
+  o.tall = tall;
+  o.rows = p.m;
+  o.cols = p.n;
+  o.batch_stride = (int64_t)rows * cols;
+  return run(batch, p, s, o, steps, a, b, c, eps, scratch, scratch_bytes,
+             reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int gs_muon_step(int batch, int rows, int cols, int grad_type, float *params, const void *grads,
+                            float *momentum, double lr, double beta, int nesterov, double weight_decay,
+                            double scale, int steps, float a, float b, float c, float eps, void *scratch,
+                            size_t scratch_bytes, void *stream) {
+  const int rc = check(batch, rows, cols, grad_type, steps, a, b, c, eps);
+  if (rc) return rc;
+  const int mask = grad_type == GS_TYPE_F32 ? 3 : 1;
+  if (params == nullptr || grads == nullptr || momentum == nullptr ||
+      (((uintptr_t)params | (uintptr_t)momentum) & 3) || ((uintptr_t)grads & mask) || !(beta >= 0.0) ||
+      !(beta < 1.0))
+    return GS_ERR_INVALID_ARGUMENT;
+  // fp32 weights: the full products, whatever the gradient's type
+  const Plan p = make_plan(batch, rows, cols, GS_TYPE_F32);
+  const bool tall = rows > cols;
+  Source s{};
+  s.u = grads;
+  s.type = grad_type;
+  s.batch_stride = (int64_t)rows * cols;
+  s.row_stride = tall ? 1 : cols;
+  s.col_stride = tall ? cols : 1;
+  s.momentum = momentum;
+  s.beta = (float)beta;
+  s.fresh = (float)(1.0 - beta);
+  s.nesterov = nesterov != 0;
+  s.rows = p.m;
+  s.cols = p.n;
+  Out o{};
+  o.p = params;
+  o.type = GS_TYPE_F32;
+  o.update = 1;
+  o.tall = tall;
+  o.rows = p.m;
+  o.cols = p.n;
+  o.batch_stride = s.batch_stride;
+  o.decay = (float)(1.0 - lr * weight_decay);
+  o.step = (float)(lr * scale);
+  return run(batch, p, s, o, steps, a, b, c, eps, scratch, scratch_bytes,
+             reinterpret_cast<cudaStream_t>(stream));
+}

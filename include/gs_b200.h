@@ -622,6 +622,38 @@ GS_API int gs_gated_scan_backward(int64_t rows, int sequences, int channels, int
                                   float *grad_initial, void *scratch, size_t scratch_bytes,
                                   void *stream);
 
+/* ---- orthogonalised updates -------------------------------------------------
+ * No counterpart in the reference (whose optimizer is Adam). For each of
+ * `batch` matrices U of rows x cols, X = U / max(|U|_F, eps) (transposed while
+ * rows > cols) and `steps` times
+ *   A = X X^T;  B = b A + c A A;  X = a X + B X,
+ * which brings X near the orthogonal factor of U: every singular value s
+ * follows p(s) = a s + b s^3 + c s^5. Products run on the tensor cores with
+ * fp32 accumulation; results of type fp32 and fp16 carry fp32's accuracy, bf16
+ * results that of their type.
+ *
+ * 1 <= batch <= 65535, rows and cols <= 2^24, the smaller <= 2^15;
+ * 1 <= steps <= 100; eps > 0. The coefficients have to keep |X|_2 and |B|_2
+ * below 8 through all steps (GS_ERR_INVALID_ARGUMENT otherwise). Strides of U
+ * in elements, any that are not negative; out is contiguous (batch, rows,
+ * cols) of U's type and does not overlap U. Scratch: 16-byte aligned. A
+ * non-finite U gives non-finite results. */
+GS_API size_t gs_orthogonalize_scratch_bytes(int batch, int rows, int cols, int type);
+GS_API int gs_orthogonalize(int batch, int rows, int cols, int type, const void *update,
+                            int64_t batch_stride, int64_t row_stride, int64_t col_stride, void *out,
+                            int steps, float a, float b, float c, float eps, void *scratch,
+                            size_t scratch_bytes, void *stream);
+
+/* One optimizer step of `batch` contiguous fp32 matrices:
+ *   M = beta M + (1 - beta) G;  U = nesterov ? beta M + (1 - beta) G : M;
+ *   W = (1 - lr weight_decay) W - lr scale orthogonalize(U),
+ * G of grad_type, contiguous. Scratch: gs_orthogonalize_scratch_bytes with
+ * GS_TYPE_F32. Gated on the device status word like gs_adam_step. */
+GS_API int gs_muon_step(int batch, int rows, int cols, int grad_type, float *params,
+                        const void *grads, float *momentum, double lr, double beta, int nesterov,
+                        double weight_decay, double scale, int steps, float a, float b, float c,
+                        float eps, void *scratch, size_t scratch_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

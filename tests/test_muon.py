@@ -1,0 +1,261 @@
+"""Orthogonalised updates and the optimizer step built on them, against the
+formulas in 64 bits.
+
+Tolerances. One step is bounded entry by entry. A product's operands are two
+fp16 numbers (each value to 2^-22), the product of the two low parts (2^-22) is
+left out, and at most 48 partial sums are cut off at 2^-23 of them before they
+are added in fp32 (at most 2^9 parts at 2^-24): 1e-5 of the same product of
+absolute values covers it. bf16 runs hold A and B, and X inside A, to fp16's
+2^-11. The chain b A + c A A, then times X, holds at most 8 such errors.
+
+After several steps the yardstick is the same formula in fp32 (torch on the
+CPU): its own distance from 64 bits, times 4, plus the rounding to the result's
+type (half a step: 2^-9 of a bf16 value, twice, since such a run may add as
+much of its own).
+"""
+import importlib
+import math
+
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+DEV = "cuda:0"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+ABC = (3.4445, -4.7750, 2.0315)
+
+
+def plain(u, steps=5, abc=ABC, eps=1e-7, dtype=torch.float64):
+    a, b, c = abc
+    x = u.detach().cpu().double()
+    x = (x / torch.linalg.matrix_norm(x, keepdim=True).clamp(min=eps)).to(dtype)
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT if tall else x
+    for _ in range(steps):
+        g = x @ x.mT
+        x = a * x + (b * g + c * g @ g) @ x
+    return x.mT if tall else x
+
+
+def rel(got, ref):
+    return float((got.detach().double().cpu() - ref).norm() / ref.norm())
+
+
+def strong(m, n, rank, dtype=F32, batch=None, seed=0, scale=1e-3):
+    gen = torch.Generator().manual_seed(seed)
+    lead = () if batch is None else (batch,)
+    u = torch.randn(*lead, m, rank, generator=gen) @ torch.randn(*lead, rank, n, generator=gen)
+    return (scale * (u + 0.05 * torch.randn(*lead, m, n, generator=gen))).to(dtype)
+
+
+SIZES = [(1, 1), (1, 70), (70, 1), (16, 16), (63, 65), (64, 64), (128, 128), (129, 127), (45, 3000), (200, 130),
+         (257, 255), (384, 640), (1000, 300)]
+
+
+@gpu
+@pytest.mark.parametrize("m,n", SIZES)
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_one_step_entry_by_entry(gs, m, n, dtype):
+    u = strong(m, n, 2, dtype)     # few directions: singular values near 1, all terms count
+    for abc in (ABC, (0.0, 1.0, 0.0), (0.0, 0.0, 1.0)):
+        got = gs.orthogonalize(u.to(DEV), steps=1, coefficients=abc)
+        assert got.dtype == dtype and got.shape == u.shape and got.is_contiguous()
+        ref = plain(u, 1, abc)
+        size = plain(u.abs(), 1, tuple(abs(v) for v in abc))
+        unit = 1e-5 if dtype != BF16 else 2.0 ** -11
+        half = torch.finfo(dtype).eps / 2
+        tol = 8 * unit * size + half * ref.abs() + torch.finfo(dtype).tiny
+        err = (got.double().cpu() - ref).abs()
+        assert bool((err <= tol).all()), (abc, float((err / tol).max()))
+
+
+@gpu
+@pytest.mark.parametrize("m,n", SIZES + [(1024, 1024), (700, 2100)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_five_steps(gs, m, n, dtype):
+    u = strong(m, n, max(1, min(m, n) // 16), dtype, seed=m)
+    got = gs.orthogonalize(u.to(DEV))
+    ref = plain(u)
+    yard = rel(plain(u, dtype=F32), ref)
+    round_off = {F32: 0.0, F16: 2.0 ** -12, BF16: 2 * 2.0 ** -9}[dtype]
+    assert rel(got, ref) <= 4 * yard + 2 ** -22 + round_off
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_stacks_and_strides(gs, dtype):
+    u = strong(60, 100, 4, dtype, batch=5, seed=1).to(DEV)
+    whole = gs.orthogonalize(u)
+    assert whole.shape == u.shape
+    for k in range(5):
+        # a matrix alone may be cut into other tiles: the same but for the order of sums
+        assert rel(gs.orthogonalize(u[k]), whole[k].double().cpu()) <= (1e-5 if dtype == F32 else 2 * 2.0 ** -9)
+    same = u.mT.contiguous().mT
+    assert torch.equal(gs.orthogonalize(same), whole)
+    wide = torch.randn(5, 61, 240, device=DEV).to(dtype)
+    wide[:, 1:, 3:203:2] = u
+    assert torch.equal(gs.orthogonalize(wide[:, 1:, 3:203:2]), whole)
+    assert torch.equal(gs.orthogonalize(u[:1].expand(3, -1, -1))[2], gs.orthogonalize(u[:1].repeat(3, 1, 1))[2])
+    flipped = gs.orthogonalize(u.mT)
+    assert torch.equal(flipped, whole.mT)
+    assert gs.orthogonalize(u[:0]).shape == (0, 60, 100)
+
+
+@gpu
+def test_scales_zero_and_nan(gs):
+    u = strong(90, 40, 3)
+    ref = gs.orthogonalize(u.to(DEV))
+    for power in (-60, 60):          # squares leave fp32's range, the norm does not
+        got = gs.orthogonalize((u * 2.0 ** power).to(DEV), eps=1e-30)
+        assert torch.equal(got, ref)
+    assert torch.equal(gs.orthogonalize(torch.zeros(90, 40, device=DEV)), torch.zeros(90, 40, device=DEV))
+    small = gs.orthogonalize(torch.full((4, 4), 1e-12, device=DEV), steps=1)   # eps takes over
+    assert rel(small, plain(torch.full((4, 4), 1e-12), 1)) <= 1e-5
+    u[3, 4] = float("nan")
+    stack = torch.stack([u, strong(90, 40, 3)]).to(DEV)
+    got = gs.orthogonalize(stack)
+    assert not bool(torch.isfinite(got[0]).any()) and torch.equal(got[1], ref)
+    u[3, 4] = float("inf")
+    assert not bool(torch.isfinite(gs.orthogonalize(u.to(DEV))).all())
+
+
+@gpu
+def test_singular_values_come_near_one(gs):
+    u = torch.randn(96, 160, generator=torch.Generator().manual_seed(2))
+    s = torch.linalg.svdvals(gs.orthogonalize(u.to(DEV)).double().cpu())
+    assert float(s.max()) < 1.21 and float(s.min()) > 0.6   # the quintic's band around 1
+    spikes = torch.zeros(70, 90)
+    spikes[5, 7] = 3.0                                       # an entry of 1 after the norm
+    got = gs.orthogonalize(spikes.to(DEV))
+    assert rel(got, plain(spikes)) <= 1e-5
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(40, 72), (72, 40), (3, 64, 128), (300, 200), (1, 1)])
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("grad_dtype", [F32, BF16])
+def test_steps_of_the_optimizer(gs, shape, nesterov, grad_dtype):
+    gen = torch.Generator().manual_seed(7)
+    w = torch.randn(*shape, generator=gen) * 0.05
+    m = torch.zeros(*shape)
+    param, momentum = w.to(DEV), m.to(DEV)
+    W, M = w.double(), m.double()
+    lr, beta, decay = 0.02, 0.9, 0.1
+    scale = math.sqrt(max(1.0, shape[-2] / shape[-1]))
+    for k in range(3):
+        g = strong(*shape[-2:], 3, grad_dtype, batch=shape[0] if len(shape) == 3 else None, seed=k)
+        gs.muon_step(param, g.to(DEV), momentum, lr, beta=beta, nesterov=nesterov, weight_decay=decay)
+        M = beta * M + (1 - beta) * g.double()
+        U = beta * M + (1 - beta) * g.double() if nesterov else M
+        O = plain(U)
+        W = (1 - lr * decay) * W - lr * scale * O
+        # fp32 momentum: half a step each of its product, its sum and its factors
+        assert float((momentum.double().cpu() - M).abs().max()) <= 4 * (k + 1) * 2.0 ** -24 * float(M.abs().max())
+        yard = rel(plain(U.float(), dtype=F32), plain(U.float())) + 2.0 ** -20
+        err = float((param.double().cpu() - W).norm())
+        assert err <= (k + 1) * (lr * scale * 8 * yard * float(O.norm()) + 4 * 2.0 ** -24 * float(W.norm()))
+    again = param.clone()
+    gs.muon_step(param, g.to(DEV), momentum, lr, scale=0.0)
+    assert torch.equal(param, again)
+
+
+@gpu
+def test_the_optimizer_is_gated_on_the_status_word(gs):
+    nat = importlib.import_module("3dgs_from_scratch_b200._native")
+    w, g, m = (torch.randn(80, 130, device=DEV) for _ in range(3))
+    kept = w.clone(), m.clone()
+    flag = torch.zeros(1, dtype=torch.int32, device=DEV)
+    assert nat.query("gs_check_status", nat.stream_ptr()) == 0
+    nat.call("gs_selftest_set_timeout", flag.data_ptr(), nat.stream_ptr())
+    gs.muon_step(w, g, m, 0.1)
+    assert nat.query("gs_check_status", nat.stream_ptr()) == nat.GS_ERR_DEVICE_TIMEOUT
+    assert torch.equal(w, kept[0]) and torch.equal(m, kept[1])
+    gs.muon_step(w, g, m, 0.1)
+    assert nat.query("gs_check_status", nat.stream_ptr()) == 0
+    assert not torch.equal(w, kept[0]) and not torch.equal(m, kept[1])
+
+
+@gpu
+def test_the_same_bits_every_time_from_graphs_and_streams(gs):
+    u = strong(300, 500, 9).to(DEV)
+    w, g, m = (strong(200, 90, 5, seed=k).to(DEV) for k in range(3))
+    ref = gs.orthogonalize(u)
+    assert all(torch.equal(gs.orthogonalize(u), ref) for _ in range(3))
+    w1, m1 = w.clone(), m.clone()
+    for _ in range(2):
+        gs.muon_step(w1, g, m1, 0.1)
+    w2, m2 = w.clone(), m.clone()
+    graphs = []
+    for _ in range(2):                # two graphs, each with its own scratch
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = gs.orthogonalize(u)
+            gs.muon_step(w2, g, m2, 0.1)
+        graphs.append((graph, out))
+    assert torch.equal(w2, w)         # captured, not run
+    for graph, out in graphs:
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref)
+    assert torch.equal(w2, w1) and torch.equal(m2, m1)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(3)], []
+    for s in streams:                 # calls side by side
+        with torch.cuda.stream(s):
+            outs.append(gs.orthogonalize(u))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, ref) for o in outs)
+
+
+def test_refuses_what_it_cannot_run(gs):
+    x = torch.zeros(4, 6)
+    for bad in (lambda: gs.orthogonalize(x), lambda: gs.orthogonalize(x[0]), lambda: gs.orthogonalize(x[:0]),
+                lambda: gs.orthogonalize(x.double()), lambda: gs.orthogonalize(x[None, None]),
+                lambda: gs.muon_step(x, x, x, 0.1)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@gpu
+def test_refuses_wrong_steps_and_parameters(gs):
+    x = torch.ones(4, 6, device=DEV)
+    for kw in (dict(steps=0), dict(steps=101), dict(steps=1.5), dict(coefficients=(1.0, 2.0)), dict(eps=0.0),
+               dict(coefficients=(float("nan"), 0.0, 0.0))):
+        with pytest.raises(ValueError):
+            gs.orthogonalize(x, **kw)
+    nat = importlib.import_module("3dgs_from_scratch_b200._native")
+    with pytest.raises(nat.NativeError):
+        gs.orthogonalize(x, coefficients=(9.0, 0.0, 0.0))      # would leave the range
+    for args in ((x, x, x[:, :3], 0.1), (x, x[:2], x, 0.1), (x.bfloat16(), x, x, 0.1), (x, x, x.half(), 0.1),
+                 (x.t(), x.t(), x.t(), 0.1), (x, x.cpu(), x, 0.1), (x, x, x.cpu(), 0.1)):
+        with pytest.raises(ValueError):
+            gs.muon_step(*args)
+    with pytest.raises(ValueError):
+        gs.muon_step(x, x, x, 0.1, beta=1.0)
+
+
+def test_entry_points_refuse_bad_arguments(gs):
+    lib = gs.load_native()
+    nat = importlib.import_module("3dgs_from_scratch_b200._native")
+    bad, at = nat.GS_ERR_INVALID_ARGUMENT, 0x10000
+
+    def run(batch=1, rows=8, cols=8, kind=0, u=at, strides=(64, 8, 1), out=at, steps=5, abc=ABC, eps=1e-7,
+            scratch=at, nbytes=0):
+        return lib.gs_orthogonalize(batch, rows, cols, kind, u, *strides, out, steps, *abc, eps, scratch, nbytes,
+                                    None)
+
+    for kw in (dict(batch=0), dict(batch=65536), dict(rows=0), dict(cols=0), dict(rows=(1 << 24) + 1),
+               dict(rows=(1 << 15) + 1, cols=(1 << 15) + 1), dict(kind=3), dict(u=None), dict(out=None),
+               dict(u=at + 2), dict(strides=(64, -8, 1)), dict(steps=0), dict(steps=101), dict(eps=0.0),
+               dict(eps=float("nan")), dict(abc=(8.5, 0.0, 0.0)), dict(abc=(3.0, 3.0, 3.0)),
+               dict(abc=(float("nan"), 0.0, 0.0)), dict(scratch=None), dict(scratch=at + 8)):
+        assert run(**kw) == bad, kw
+    assert run() == nat.GS_ERR_CAPACITY
+    assert run(steps=2, abc=(3.0, 0.0, 0.0)) == bad       # 3, then 9
+    assert run(steps=1, abc=(3.0, 0.0, 0.0)) == nat.GS_ERR_CAPACITY
+    assert lib.gs_muon_step(1, 8, 8, 0, at, at, at, 0.1, 1.0, 1, 0.0, 1.0, 5, *ABC, 1e-7, at, 0, None) == bad
+    assert lib.gs_muon_step(1, 8, 8, 0, at, at, None, 0.1, 0.9, 1, 0.0, 1.0, 5, *ABC, 1e-7, at, 0, None) == bad
+    assert lib.gs_orthogonalize_scratch_bytes(0, 8, 8, 0) == 0
+    one = lib.gs_orthogonalize_scratch_bytes(1, 300, 500, 0)
+    assert 0 < one < lib.gs_orthogonalize_scratch_bytes(2, 300, 500, 0)
