@@ -67,7 +67,7 @@ struct Out {
 
 struct Args {
   Matrix x, y, sq, poly;  // X, the next X, A, B
-  int row_blocks, column_blocks;  // of 128 rows and of 64 columns, X
+  int tiles, row_tiles, batches;  // of a product: tiles of a matrix, rows of them, matrices
   int k_blocks_n, k_blocks_m;     // 64-wide K blocks that hold data
   int stages;
   float a, b, c;
@@ -107,11 +107,12 @@ __device__ __forceinline__ uint32_t fetch_rows(char *plane, const Matrix &M, int
   return rows * 128;
 }
 
-__device__ __forceinline__ uint64_t operand(uint32_t addr, bool mn, int k) {
-  // 16 elements of K further: 32 bytes along a row, or 16 rows of 128 bytes
-  return mn ? tc::descriptor(addr + k * 2048, kBlockBytes / 2, 1024)
-            : tc::descriptor(addr + k * 32, 16, 1024);
+// An operand's descriptor, and what 16 elements of K further add to it: 32
+// bytes along a row, or 16 rows of 128 bytes (in units of 16 bytes).
+__device__ __forceinline__ uint64_t operand(uint32_t addr, bool mn) {
+  return mn ? tc::descriptor(addr, kBlockBytes / 2, 1024) : tc::descriptor(addr, 16, 1024);
 }
+__device__ __forceinline__ uint32_t k_step(bool mn) { return mn ? 128 : 2; }
 
 __device__ __forceinline__ void split8(const float *v, uint4 &hi, uint4 &lo) {
   __half h[8], l[8];
@@ -130,204 +131,332 @@ __device__ __forceinline__ void add8(const uint4 &q, float (&v)[8]) {
   for (int i = 0; i < 8; ++i) v[i] += __half2float(h[i]);
 }
 
-__device__ __forceinline__ void store_result(const Out &o, int batch, int row, int col, float v) {
-  if (row >= o.rows || col >= o.cols) return;
-  const int64_t at = (int64_t)batch * o.batch_stride +
-                     (o.tall ? (int64_t)col * o.rows + row : (int64_t)row * o.cols + col);
-  if (o.update) {
-    float *w = reinterpret_cast<float *>(o.p);
-    w[at] = fmaf(o.decay, w[at], -o.step * v);
-  } else if (o.type == GS_TYPE_F32) {
-    reinterpret_cast<float *>(o.p)[at] = v;
-  } else if (o.type == GS_TYPE_BF16) {
-    reinterpret_cast<__nv_bfloat16 *>(o.p)[at] = __float2bfloat16_rn(v);
-  } else {
-    reinterpret_cast<__half *>(o.p)[at] = __float2half_rn(v);
+__device__ __forceinline__ void store_as(void *p, int type, int64_t at, float v) {
+  if (type == GS_TYPE_F32) reinterpret_cast<float *>(p)[at] = v;
+  else if (type == GS_TYPE_BF16) reinterpret_cast<__nv_bfloat16 *>(p)[at] = __float2bfloat16_rn(v);
+  else reinterpret_cast<__half *>(p)[at] = __float2half_rn(v);
+}
+
+// 32 rows x 32 columns of the result, thread l holding row `row` (+ l) from
+// column `col` on. A tall result is X's transpose: the warp's rows are adjacent
+// there. Otherwise the warp turns them in shared memory, so that its threads
+// write adjacent columns.
+__device__ __forceinline__ void store_result(const Out &o, int batch, int row, int col,
+                                             const float (&w)[32], float (*turn)[33]) {
+  const int lane = (int)lane_id();
+  const int64_t base = (int64_t)batch * o.batch_stride;
+  if (!o.tall) {
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < 32; ++e) turn[lane][e] = w[e];
+    __syncwarp();
+  }
+  // entry e of this thread: (row + lane, col + e), or turned (row + e, col + lane)
+  const int limit = o.tall ? o.cols - col : o.rows - row;
+  const bool on = o.tall ? row + lane < o.rows : col + lane < o.cols;
+  const int64_t first = base + (o.tall ? (int64_t)col * o.rows + row + lane
+                                       : (int64_t)row * o.cols + col + lane);
+  const int64_t step = o.tall ? o.rows : o.cols;
+  if (!on) return;
+#pragma unroll
+  for (int e0 = 0; e0 < 32; e0 += 8) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = o.tall ? w[e0 + e] : turn[e0 + e][lane];
+    if (o.update) {
+      float *p = reinterpret_cast<float *>(o.p);
+      float old[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) old[e] = e0 + e < limit ? p[first + (e0 + e) * step] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e0 + e < limit) p[first + (e0 + e) * step] = fmaf(o.decay, old[e], -o.step * v[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e0 + e < limit) store_as(o.p, o.type, first + (e0 + e) * step, v[e]);
+    }
   }
 }
 
-template <int BN, int KIND, bool FULL>
+template <int BN, int KIND, bool FULL, int CTAS>
 struct Shape {
   static constexpr int kPlanesA = FULL ? 2 : 1;
   static constexpr int kPlanesB = FULL || KIND == kApply ? 2 : 1;
-  static constexpr int kStage = (kPlanesA * 128 + kPlanesB * BN) * 128;
-  static constexpr int kTri = BN > 128 ? BN : 128;
+  static constexpr int kRowsB = BN / CTAS;                 // of B's rows in each block
+  static constexpr int kPlaneA = 128 * 128, kPlaneB = kRowsB * 128;  // bytes
+  static constexpr int kStage = kPlanesA * kPlaneA + kPlanesB * kPlaneB;
+  static constexpr int kTri = BN > 128 * CTAS ? BN : 128 * CTAS;
   static constexpr int kChunk = FULL ? 4 : 1 << 30;        // K blocks of an accumulator
   // Where there is room, hi lo + lo hi have an accumulator of their own: far
   // fewer cut-off additions to the large one (128 x 64 in fp32: the result's
   // error 2.3e-6 -> 1.2e-6, as fp32 products have).
   static constexpr bool kCross = FULL && BN <= 128;
-  static constexpr int kWidth = kCross ? 2 * BN : BN;        // columns of tensor memory
-  static constexpr int kColumns = FULL ? 2 * kWidth : kWidth;  // two take turns
+  static constexpr int kWidth = kCross ? 2 * BN : BN;      // columns of tensor memory
+  static constexpr int kColumns = 2 * kWidth;              // two accumulators take turns
   // A copy warp, an MMA warp and the epilogue. Where an epilogue thread holds
-  // 128 sums, a whole warpgroup goes to the first two, so that it can hand its
+  // 64 or 128 sums, a whole warpgroup goes to the first two, so that it can hand its
   // registers over: 384 threads x 168 = 128 x 40 + 256 x 232.
-  static constexpr bool kHandOver = FULL && BN == 256;
+  static constexpr bool kHandOver = BN >= 128;
   static constexpr int kEpilogue = kHandOver ? 4 : 2;      // its first warp
   static constexpr int kThreads = 32 * (kEpilogue + kEpilogueWarps);
+  static constexpr int kTurn = kEpilogueWarps * 32 * 33 * 4;
 };
 
-template <int BN, int KIND, bool FULL>
-__global__ void __launch_bounds__(Shape<BN, KIND, FULL>::kThreads, 1) product_kernel(const Args A) {
-  using S = Shape<BN, KIND, FULL>;
+// Tiles of 128 CTAS x BN, one after another in a persistent block (or pair of
+// blocks): while the epilogue works on a tile, the next one's products run
+// into the other accumulator.
+template <int BN, int KIND, bool FULL, int CTAS>
+__global__ void __launch_bounds__(Shape<BN, KIND, FULL, CTAS>::kThreads, 1)
+    product_kernel(const __grid_constant__ Args A) {
+  using S = Shape<BN, KIND, FULL, CTAS>;
   extern __shared__ char raw[];
   char *smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], ready[2], drained[2];
+  __shared__ uint64_t full[kMaxStages], peer[kMaxStages], empty[kMaxStages], ready[2], drained[2];
   __shared__ uint32_t tmem_base, failed;
-  const int warp = threadIdx.x / 32, batch = blockIdx.y;
-  int i, j;  // the tile: rows 128 i.., columns BN j..
-  if (KIND == kApply) {
-    i = blockIdx.x % A.row_blocks;
-    j = blockIdx.x / A.row_blocks;
-  } else {  // column j of tiles holds the rows down to its diagonal block
-    int left = blockIdx.x, rows;
-    for (j = 0;; ++j) {
-      rows = (j * BN / S::kTri + 1) * (S::kTri / 128);
-      if (left < rows) break;
-      left -= rows;
-    }
-    i = left;
-  }
+  const int warp = threadIdx.x / 32;
+  const int rank = CTAS == 2 ? (int)tc::cluster_rank() : 0;
   const int k_blocks = KIND == kGram ? A.k_blocks_n : A.k_blocks_m;
+  const int chunks = (k_blocks + S::kChunk - 1) / S::kChunk;
+  const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS, total = A.tiles * A.batches;
   if (threadIdx.x == 0) {
     for (int s = 0; s < A.stages; ++s) {
       mbar_init(&full[s], 1);
+      mbar_init(&peer[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&ready[s], 1);
-      mbar_init(&drained[s], kEpilogueWarps);
+      mbar_init(&drained[s], kEpilogueWarps * CTAS);
     }
     failed = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tc::tmem_alloc(&tmem_base, S::kColumns);
+  if (warp == 1) tc::tmem_alloc<CTAS>(&tmem_base, S::kColumns);
   tc::fence_before();
   __syncthreads();
+  if (CTAS == 2) tc::cluster_sync();
   tc::fence_after();
   const uint32_t tmem = tmem_base;
+  // Tile t: its matrix, row of tiles and column of tiles.
+  struct Spot {
+    int batch, i, j;
+  };
+  const auto spot = [&](int t) {
+    Spot p;
+    p.batch = t / A.tiles;
+    int left = t % A.tiles;
+    if (KIND == kApply) {
+      p.i = left % A.row_tiles;
+      p.j = left / A.row_tiles;
+    } else {  // column j of tiles holds the rows down to its diagonal block
+      int rows;
+      for (p.j = 0;; ++p.j) {
+        rows = (p.j * BN / S::kTri + 1) * (S::kTri / (128 * CTAS));
+        if (left < rows) break;
+        left -= rows;
+      }
+      p.i = left;
+    }
+    return p;
+  };
   // Whether a K block of a symmetric matrix lies below the diagonal of rows.
   const auto below = [&](int row, int kb) { return KIND != kGram && kb * 64 / S::kTri < row / S::kTri; };
 
   if (S::kHandOver && warp < S::kEpilogue) tc::registers_down<40>();
-  if (warp == 0 && lane_id() == 0) {
+  if (warp == 0) {
     const Matrix &MA = KIND == kGram ? A.x : KIND == kSquare ? A.sq : A.poly;
     const Matrix &MB = KIND == kSquare ? A.sq : A.x;
-    int kb = 0;
-    for (; kb < k_blocks; ++kb) {
-      const int s = kb % A.stages, round = kb / A.stages;
-      if (round > 0 && !mbar_wait(&empty[s], (round - 1) & 1)) {
-        failed = 1;
-        break;
+    int it = 0, done = 0;
+    bool good = true;
+    for (int t = first; t < total && good; t += step) {
+      const Spot p = spot(t);
+      const int row_a = (p.i * CTAS + rank) * 128, row_b = p.j * BN + rank * S::kRowsB;
+      for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+        const int s = it % A.stages, round = it / A.stages;
+        good = __all_sync(0xffffffffu, round == 0 || mbar_wait(&empty[s], (round - 1) & 1));
+        if (!good) break;
+        done = it + 1;
+        if (!tc::elect_one()) continue;
+        char *a = smem + (size_t)s * S::kStage, *b = a + S::kPlanesA * S::kPlaneA;
+        mbar_expect_tx(&full[s], S::kStage);
+        for (int q = 0; q < S::kPlanesA; ++q)
+          fetch_rows(q ? MA.lo : MA.hi, MA, p.batch, row_a, 128, kb, below(row_a, kb),
+                     a + q * S::kPlaneA, &full[s]);
+        for (int q = 0; q < S::kPlanesB; ++q)
+          fetch_rows(q ? MB.lo : MB.hi, MB, p.batch, row_b, S::kRowsB, kb,
+                     KIND == kApply || (KIND == kSquare && below(p.j * BN, kb)),
+                     b + q * S::kPlaneB, &full[s]);
       }
-      char *a = smem + (size_t)s * S::kStage, *b = a + S::kPlanesA * 128 * 128;
-      mbar_expect_tx(&full[s], S::kStage);
-      for (int q = 0; q < S::kPlanesA; ++q)
-        fetch_rows(q ? MA.lo : MA.hi, MA, batch, i * 128, 128, kb, below(i * 128, kb),
-                   a + q * 128 * 128, &full[s]);
-      for (int q = 0; q < S::kPlanesB; ++q)
-        fetch_rows(q ? MB.lo : MB.hi, MB, batch, j * BN, BN, kb,
-                   KIND == kApply || (KIND == kSquare && below(j * BN, kb)), b + q * BN * 128, &full[s]);
     }
-    if (kb < k_blocks)  // given up: the copies in flight still land here
-      for (int q = kb > A.stages ? kb - A.stages : 0; q < kb; ++q)
+    if (!good) {  // given up: the copies in flight still land here
+      failed = 1;
+      for (int q = done > A.stages ? done - A.stages : 0; q < done; ++q)
         mbar_wait(&full[q % A.stages], (q / A.stages) & 1);
-  } else if (warp == 1 && lane_id() == 0) {
-    for (int kb = 0; kb < k_blocks; ++kb) {
-      const int s = kb % A.stages, chunk = kb / S::kChunk, acc = chunk & 1;
-      const bool fresh = kb % S::kChunk == 0;
-      if (!mbar_wait(&full[s], (kb / A.stages) & 1) ||
-          (fresh && chunk >= 2 && !mbar_wait(&drained[acc], (chunk / 2 - 1) & 1))) {
-        failed = 1;
-        break;
-      }
-      tc::fence_after();
-      const uint32_t a = smem_addr(smem + (size_t)s * S::kStage), b = a + S::kPlanesA * 128 * 128;
-      const bool a_mn = below(i * 128, kb), b_mn = KIND == kApply || (KIND == kSquare && below(j * BN, kb));
-      const uint32_t instr = tc::instruction_f16(128, BN, a_mn, b_mn);
-#pragma unroll
-      for (int q = 0; q < (FULL ? 3 : S::kPlanesB); ++q) {  // hi hi, hi lo, lo hi
-        const uint32_t aq = a + (q == 2 ? 128 * 128 : 0), bq = b + (q == 1 ? BN * 128 : 0);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          tc::mma_f16(tmem + acc * S::kWidth + (S::kCross && q > 0 ? BN : 0), operand(aq, a_mn, k),
-                      operand(bq, b_mn, k), instr, !(fresh && k == 0 && (q == 0 || (S::kCross && q == 1))));
-      }
-      tc::commit(&empty[s]);
-      if (kb % S::kChunk == S::kChunk - 1 || kb == k_blocks - 1) tc::commit(&ready[acc]);
     }
+  } else if (warp == 1 && rank == 1) {  // tells block 0 what has arrived here
+    int it = 0;
+    bool good = true;
+    for (int t = first; t < total && good; t += step)
+      for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+        good = __all_sync(0xffffffffu, mbar_wait(&full[it % A.stages], (it / A.stages) & 1));
+        if (!good) break;
+        if (tc::elect_one()) tc::arrive_at(&peer[it % A.stages], 0);
+      }
+    if (!good) failed = 1;
+  } else if (warp == 1) {
+    int it = 0, chunk = 0;
+    bool good = true;
+    for (int t = first; t < total && good; t += step) {
+      const Spot p = spot(t);
+      for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+        const int s = it % A.stages, acc = chunk & 1;
+        const bool fresh = kb % S::kChunk == 0, last = kb % S::kChunk == S::kChunk - 1 || kb == k_blocks - 1;
+        bool ok = mbar_wait(&full[s], (it / A.stages) & 1);
+        if (CTAS == 2) ok = ok && tc::wait_cluster(&peer[s], (it / A.stages) & 1);
+        if (fresh && chunk >= 2) ok = ok && tc::wait_cluster(&drained[acc], (chunk / 2 - 1) & 1);
+        good = __all_sync(0xffffffffu, ok);
+        if (!good) break;
+        tc::fence_after();
+        const uint32_t at = smem_addr(smem) + s * S::kStage;
+        const bool a_mn = below(p.i * CTAS * 128, kb);
+        const bool b_mn = KIND == kApply || (KIND == kSquare && below(p.j * BN, kb));
+        // One lane issues, so the loop holds an addition or two for each MMA.
+        const uint64_t a = operand(at, a_mn), b = operand(at + S::kPlanesA * S::kPlaneA, b_mn);
+        const uint32_t instr = tc::instruction_f16(128 * CTAS, BN, a_mn, b_mn);
+        const uint32_t a_step = k_step(a_mn), b_step = k_step(b_mn);
+        const uint32_t main = tmem + acc * S::kWidth, cross = S::kCross ? main + BN : main;
+        if (tc::elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc::mma_f16<CTAS>(main, a + k * a_step, b + k * b_step, instr, k > 0 || !fresh);
+          if (S::kPlanesB == 2) {  // hi lo
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              tc::mma_f16<CTAS>(cross, a + k * a_step, b + (S::kPlaneB / 16) + k * b_step, instr,
+                                k > 0 || !S::kCross || !fresh);
+          }
+          if (S::kPlanesA == 2) {  // lo hi
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              tc::mma_f16<CTAS>(cross, a + (S::kPlaneA / 16) + k * a_step, b + k * b_step, instr, true);
+          }
+          tc::commit<CTAS>(&empty[s]);
+          if (last) tc::commit<CTAS>(&ready[acc]);
+        }
+        __syncwarp();
+        chunk += last;
+      }
+    }
+    if (!good) failed = 1;
   } else if (warp >= S::kEpilogue) {
     if (S::kHandOver) tc::registers_up<232>();
     const int quarter = warp & 3;  // the lanes of tensor memory that the warp may read
-    const int r = quarter * 32 + (int)lane_id(), row = i * 128 + r;
+    const int r = quarter * 32 + (int)lane_id();
     const int c0 = (warp - S::kEpilogue) / 4 * (BN / 2);
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + c0;
-    float v[BN / 2];
-    const int chunks = (k_blocks + S::kChunk - 1) / S::kChunk;
+    float(*turn)[33] = reinterpret_cast<float(*)[33]>(smem + (size_t)A.stages * S::kStage) +
+                       (warp - S::kEpilogue) * 32;
+    const Matrix &dst = KIND == kGram ? A.sq : KIND == kSquare ? A.poly : A.y;
+    const Matrix &old = KIND == kSquare ? A.sq : A.x;
+    constexpr bool kOldLo = FULL || KIND == kApply;
+    // The old values of a small tile are on their way before its products are done.
+    constexpr bool kAhead = KIND != kGram && BN <= 128;
+    constexpr int kOld = KIND == kGram ? 1 : kAhead ? BN / 16 : 4;
+    int chunk = 0;
     bool good = true;
-    for (int chunk = 0; chunk < chunks && good; ++chunk) {
-      const int acc = chunk & 1;
-      good = mbar_wait(&ready[acc], (chunk / 2) & 1);
-      if (!good) break;
-      tc::fence_after();
+    for (int t = first; t < total && good; t += step) {
+      const Spot p = spot(t);
+      const int i = p.i * CTAS + rank;  // the block's rows: 128 i..
+      uint4 oh[kOld], ol[kOld];
+      const auto load_old = [&](int from, int count) {
 #pragma unroll
-      for (int c = 0; c < BN / 2; c += 32) {
-        float part[32];
-        tc::load_columns(lanes + acc * S::kWidth + c, part);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) v[c + e] = chunk == 0 ? part[e] : v[c + e] + part[e];
-        if (S::kCross) {
-          tc::load_columns(lanes + acc * S::kWidth + BN + c, part);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[c + e] += part[e];
+        for (int q = 0; q < count; ++q) {
+          const int col = p.j * BN + c0 + from + 8 * q, at = chunk_at(r, col);
+          oh[q] = *reinterpret_cast<const uint4 *>(block_at(old.hi, old, p.batch, i, col / 64) + at);
+          if (kOldLo)
+            ol[q] = *reinterpret_cast<const uint4 *>(block_at(old.lo, old, p.batch, i, col / 64) + at);
         }
-      }
-      if (chunk + 2 < chunks) {
+      };
+      if (kAhead) load_old(0, kOld);
+      float v[BN / 2];
+#pragma unroll
+      for (int e = 0; e < BN / 2; ++e) v[e] = 0.f;
+#pragma unroll 1
+      for (int part = 0; part < chunks; ++part, ++chunk) {
+        const int acc = chunk & 1;
+        good = __all_sync(0xffffffffu, mbar_wait(&ready[acc], (chunk / 2) & 1));
+        if (!good) break;
+        tc::fence_after();
+#pragma unroll
+        for (int c = 0; c < BN / 2; c += 32) {
+          float f[32];
+          tc::load_columns(lanes + acc * S::kWidth + c, f);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[c + e] += f[e];
+          if (S::kCross) {
+            tc::load_columns(lanes + acc * S::kWidth + BN + c, f);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[c + e] += f[e];
+          }
+        }
         tc::fence_before();
         __syncwarp();
-        if (lane_id() == 0) tc::arrive(&drained[acc]);
-      }
-    }
-    if (!good) {
-      failed = 1;
-    } else if (!A.out.update || ld_volatile_u32(A.status) == 0u) {  // the optimizers' gate
-      const Matrix &dst = KIND == kGram ? A.sq : KIND == kSquare ? A.poly : A.y;
-      const Matrix &old = KIND == kSquare ? A.sq : A.x;
-#pragma unroll
-      for (int g = 0; g < BN / 2; g += 8) {
-        const int col = j * BN + c0 + g, at = chunk_at(r, col);
-        float w[8];
-        if (KIND == kGram) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = v[g + e] * kUnscale;
-        } else {
-          float o[8] = {};
-          add8(*reinterpret_cast<const uint4 *>(block_at(old.hi, old, batch, i, col / 64) + at), o);
-          if (FULL || KIND == kApply)
-            add8(*reinterpret_cast<const uint4 *>(block_at(old.lo, old, batch, i, col / 64) + at), o);
-          const float p = KIND == kSquare ? A.b : A.a, q = KIND == kSquare ? A.c * kUnscale : kUnscale;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = fmaf(p, o[e], q * v[g + e]);
+        if (lane_id() == 0) {
+          if (CTAS == 2) tc::arrive_at(&drained[acc], 0);
+          else tc::arrive(&drained[acc]);
         }
+      }
+      if (!good) break;
+      if (A.out.update && ld_volatile_u32(A.status) != 0u) continue;  // the optimizers' gate
+#pragma unroll
+      for (int c = 0; c < BN / 2; c += 32) {
+        asm volatile("" ::: "memory");  // one group's loads at a time: registers
+        if (KIND != kGram && !kAhead) load_old(c, 4);
+        float w[32];
+#pragma unroll
+        for (int g = 0; g < 32; g += 8) {
+          if (KIND == kGram) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[g + e] = v[c + g + e] * kUnscale;
+          } else {
+            float o[8] = {};
+            const int q = kAhead ? (c + g) / 8 : g / 8;
+            add8(oh[q], o);
+            if (kOldLo) add8(ol[q], o);
+            const float f = KIND == kSquare ? A.b : A.a, h = KIND == kSquare ? A.c * kUnscale : kUnscale;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[g + e] = fmaf(f, o[e], h * v[c + g + e]);
+          }
+        }
+        const int col0 = p.j * BN + c0 + c;
+        asm volatile("" ::: "memory");
         if (KIND == kApply && A.out.p != nullptr) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) store_result(A.out, batch, row, col + e, w[e] * kUnscale);
+          for (int e = 0; e < 32; ++e) w[e] *= kUnscale;
+          store_result(A.out, p.batch, i * 128 + quarter * 32, col0, w, turn);
         } else {
-          uint4 hi, lo;
-          split8(w, hi, lo);
-          *reinterpret_cast<uint4 *>(block_at(dst.hi, dst, batch, i, col / 64) + at) = hi;
-          if (FULL || KIND == kApply)
-            *reinterpret_cast<uint4 *>(block_at(dst.lo, dst, batch, i, col / 64) + at) = lo;
+#pragma unroll
+          for (int g = 0; g < 32; g += 8) {
+            const int col = col0 + g, at = chunk_at(r, col);
+            uint4 hi, lo;
+            split8(w + g, hi, lo);
+            *reinterpret_cast<uint4 *>(block_at(dst.hi, dst, p.batch, i, col / 64) + at) = hi;
+            if (FULL || KIND == kApply)
+              *reinterpret_cast<uint4 *>(block_at(dst.lo, dst, p.batch, i, col / 64) + at) = lo;
+          }
         }
       }
     }
+    if (!good) failed = 1;
   }
   tc::fence_before();
   __syncthreads();
+  if (CTAS == 2) tc::cluster_sync();  // neither block leaves while the other may reach into it
   if (threadIdx.x == 0 && failed) atomicCAS(A.status, 0u, (uint32_t)GS_ERR_DEVICE_TIMEOUT);
   if (warp == 1) {
     tc::fence_after();
-    tc::tmem_free(tmem, S::kColumns);
+    tc::tmem_free<CTAS>(tmem, S::kColumns);
   }
 }
 
@@ -358,30 +487,52 @@ __device__ __forceinline__ float update_of(const Source &s, float m_new, float g
   return s.nesterov ? fmaf(s.beta, m_new, s.fresh * g) : m_new;
 }
 
-constexpr int kNormThreads = 256, kMaxParts = 256;
+constexpr int kNormThreads = 256, kMaxParts = 296;
 
 // Sums of squares, in 64 bits so that neither tiny nor huge gradients leave
-// the range; the momentum is updated on the way. Parts are added in order by
-// the reader.
+// the range; the momentum is updated on the way. A warp takes a line of
+// elements that are adjacent (or the smaller stride apart) at a time. Parts
+// are added in order by the reader.
 __global__ void __launch_bounds__(kNormThreads) norm_kernel(const Source s, double *parts,
                                                             const uint32_t *status) {
   if (s.momentum != nullptr && ld_volatile_u32(status) != 0u) return;
-  const int64_t size = (int64_t)s.rows * s.cols, base = (int64_t)blockIdx.y * s.batch_stride;
-  // elements in the order of memory: the smaller stride runs fastest
+  const int64_t base = (int64_t)blockIdx.y * s.batch_stride;
   const bool cols_fast = s.col_stride <= s.row_stride;
-  const int64_t fast = cols_fast ? s.cols : s.rows;
-  const int64_t fs = cols_fast ? s.col_stride : s.row_stride, ss = cols_fast ? s.row_stride : s.col_stride;
+  int64_t lines = cols_fast ? s.rows : s.cols, len = cols_fast ? s.cols : s.rows;
+  int64_t fs = cols_fast ? s.col_stride : s.row_stride, ss = cols_fast ? s.row_stride : s.col_stride;
+  const int64_t size = (int64_t)s.rows * s.cols;
+  if (fs == 1 && ss == len) {  // one piece of memory, in lines of 1024
+    len = 1024;
+    ss = 1024;
+    lines = (size + 1023) / 1024;
+  } else {
+    len = len < size ? len : size;
+  }
+  const bool flat = fs == 1 && ss == 1024 && len == 1024;
   double sum = 0.0;
-  for (int64_t k = (int64_t)blockIdx.x * kNormThreads + threadIdx.x; k < size;
-       k += (int64_t)gridDim.x * kNormThreads) {
-    const int64_t at = base + (k / fast) * ss + (k % fast) * fs;
-    float v = read_f32(s.u, s.type, at);
-    if (s.momentum != nullptr) {
-      const float m = next_momentum(s, s.momentum[at], v);
-      s.momentum[at] = m;
-      v = update_of(s, m, v);
+  for (int64_t k = (int64_t)blockIdx.x * (kNormThreads / 32) + threadIdx.x / 32; k < lines;
+       k += (int64_t)gridDim.x * (kNormThreads / 32)) {
+    const int64_t here = flat && size - k * 1024 < len ? size - k * 1024 : len;
+    for (int64_t f0 = lane_id(); f0 < here; f0 += 32 * 8) {
+      float v[8], m[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int64_t f = f0 + 32 * e, at = base + k * ss + f * fs;
+        v[e] = f < here ? read_f32(s.u, s.type, at) : 0.f;
+        if (s.momentum != nullptr) m[e] = f < here ? s.momentum[at] : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int64_t f = f0 + 32 * e, at = base + k * ss + f * fs;
+        if (f >= here) continue;
+        if (s.momentum != nullptr) {
+          m[e] = next_momentum(s, m[e], v[e]);
+          s.momentum[at] = m[e];
+          v[e] = update_of(s, m[e], v[e]);
+        }
+        sum = fma((double)v[e], (double)v[e], sum);
+      }
     }
-    sum = fma((double)v, (double)v, sum);
   }
   __shared__ double warps[kNormThreads / 32];
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_down_sync(0xffffffffu, sum, d);
@@ -394,11 +545,13 @@ __global__ void __launch_bounds__(kNormThreads) norm_kernel(const Source s, doub
 }
 
 // X0, 64 x 64 elements a block, scaled and split into the workspace's layout.
+// Rows of adjacent elements go straight into their chunks, others are turned
+// in shared memory.
 __global__ void __launch_bounds__(256) split_kernel(const Source s, const double *parts, int num_parts,
-                                                    double eps, Matrix x, int column_blocks) {
+                                                    double eps, Matrix x) {
   __shared__ float tile[64][65];
   __shared__ double total;
-  const int batch = blockIdx.y, r0 = blockIdx.x / column_blocks * 64, c0 = blockIdx.x % column_blocks * 64;
+  const int batch = blockIdx.y, r0 = blockIdx.x / x.column_blocks * 64, c0 = blockIdx.x % x.column_blocks * 64;
   if (threadIdx.x < 32) {
     double sum = 0.0;
     for (int k = threadIdx.x; k < num_parts; k += 32) sum += parts[(int64_t)batch * num_parts + k];
@@ -410,24 +563,26 @@ __global__ void __launch_bounds__(256) split_kernel(const Source s, const double
   }
   __syncthreads();
   const double scale = total;
+  const int64_t base = (int64_t)batch * s.batch_stride;
+  const auto read = [&](int r, int c) {
+    if (r0 + r >= s.rows || c0 + c >= s.cols) return 0.f;
+    const int64_t at = base + (r0 + r) * s.row_stride + (c0 + c) * s.col_stride;
+    float v = read_f32(s.u, s.type, at);
+    if (s.momentum != nullptr) v = update_of(s, s.momentum[at], v);
+    return (float)((double)v * scale);
+  };
   const bool cols_fast = s.col_stride <= s.row_stride;
-  for (int k = threadIdx.x; k < 64 * 64; k += 256) {
-    const int r = cols_fast ? k / 64 : k % 64, c = cols_fast ? k % 64 : k / 64;
-    float v = 0.f;
-    if (r0 + r < s.rows && c0 + c < s.cols) {
-      const int64_t at = (int64_t)batch * s.batch_stride + (r0 + r) * s.row_stride + (c0 + c) * s.col_stride;
-      v = read_f32(s.u, s.type, at);
-      if (s.momentum != nullptr) v = update_of(s, s.momentum[at], v);
-      v = (float)((double)v * scale);
-    }
-    tile[r][c] = v;
+  if (!cols_fast) {
+#pragma unroll 4
+    for (int k = threadIdx.x; k < 64 * 64; k += 256) tile[k % 64][k / 64] = read(k % 64, k / 64);
+    __syncthreads();
   }
-  __syncthreads();
+#pragma unroll
   for (int k = threadIdx.x; k < 64 * 8; k += 256) {
     const int r = k / 8, c = k % 8 * 8;
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = tile[r][c + e];
+    for (int e = 0; e < 8; ++e) v[e] = cols_fast ? read(r, c + e) : tile[r][c + e];
     uint4 hi, lo;
     split8(v, hi, lo);
     const int at = chunk_at((r0 + r) % 128, c);
@@ -439,7 +594,7 @@ __global__ void __launch_bounds__(256) split_kernel(const Source s, const double
 // ---- host -----------------------------------------------------------------------------
 
 struct Plan {
-  int m, n, bn;             // X is m x n, tiles are 128 x bn
+  int m, n, bn, ctas;       // X is m x n, tiles are 128 ctas x bn
   int row_blocks, column_blocks, sq_column_blocks;
   bool full;
   int parts;
@@ -453,7 +608,8 @@ static Plan make_plan(int batch, int rows, int cols, int type) {
   p.full = type != GS_TYPE_BF16;
   const auto tiles = [&](int bn) { return (int64_t)batch * ((p.m + 127) / 128) * ((p.n + bn - 1) / bn); };
   p.bn = tiles(256) >= 148 ? 256 : tiles(128) >= 148 ? 128 : 64;
-  const int tri = p.bn > 128 ? p.bn : 128;
+  p.ctas = p.bn == 256 ? 2 : 1;
+  const int tri = p.bn > 128 * p.ctas ? p.bn : 128 * p.ctas;
   const int mp = (p.m + tri - 1) / tri * tri, np = (p.n + p.bn - 1) / p.bn * p.bn;
   p.row_blocks = mp / 128;
   p.column_blocks = np / 64;
@@ -467,36 +623,61 @@ static Plan make_plan(int batch, int rows, int cols, int type) {
   return p;
 }
 
-template <int BN, int KIND, bool FULL>
-static int launch_product(Args A, int tiles, int batch, cudaStream_t st) {
-  using S = Shape<BN, KIND, FULL>;
-  A.stages = (220 * 1024) / S::kStage;
+template <int BN, int KIND, bool FULL, int CTAS>
+static int launch_product(Args A, int tiles, int row_tiles, int batch, cudaStream_t st) {
+  using S = Shape<BN, KIND, FULL, CTAS>;
+  const auto kernel = product_kernel<BN, KIND, FULL, CTAS>;
+  A.stages = (227 * 1024 - 2048 - S::kTurn) / S::kStage;
   if (A.stages > kMaxStages) A.stages = kMaxStages;
-  const int bytes = A.stages * S::kStage + 1024;
-  thread_local unsigned long long ready = 0;  // the context whose kernel has its shared memory set
+  A.tiles = tiles;
+  A.row_tiles = row_tiles;
+  A.batches = batch;
+  const int bytes = A.stages * S::kStage + S::kTurn + 1024;
+  // Per context: the kernel's shared memory and how many blocks run at a time.
+  thread_local unsigned long long ready = 0;
+  thread_local int resident = 0;
   const unsigned long long ctx = current_context_id();
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CTAS;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.blockDim = dim3(S::kThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
   if (ctx == 0 || ctx != ready) {
-    const int rc = cuda_status(cudaFuncSetAttribute(product_kernel<BN, KIND, FULL>,
-                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    int rc = cuda_status(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
     if (rc) return rc;
+    cfg.gridDim = dim3(CTAS);
+    rc = cuda_status(cudaOccupancyMaxActiveClusters(&resident, kernel, &cfg));
+    if (rc) return rc;
+    if (resident < 1) return GS_ERR_CUDA;
     ready = ctx != 0 ? ctx : current_context_id();
   }
-  product_kernel<BN, KIND, FULL><<<dim3(tiles, batch), S::kThreads, bytes, st>>>(A);
+  const int64_t all = (int64_t)tiles * batch;
+  cfg.gridDim = dim3((unsigned)(all < resident ? all : resident) * CTAS);
+  const int rc = cuda_status(cudaLaunchKernelEx(&cfg, kernel, A));
+  if (rc) return rc;
   count_launch();
-  return launch_status();
+  return GS_OK;
 }
 
-template <int BN, bool FULL>
+template <int BN, bool FULL, int CTAS>
 static int run_steps(Args A, const Plan &p, int batch, int steps, const Out &out, cudaStream_t st) {
   int tri_tiles = 0;
-  constexpr int kTri = BN > 128 ? BN : 128;
-  for (int j = 0; j < p.sq_column_blocks * 64 / BN; ++j) tri_tiles += (j * BN / kTri + 1) * (kTri / 128);
+  constexpr int kTri = BN > 128 * CTAS ? BN : 128 * CTAS;
+  for (int j = 0; j < p.sq_column_blocks * 64 / BN; ++j)
+    tri_tiles += (j * BN / kTri + 1) * (kTri / (128 * CTAS));
+  const int row_tiles = p.row_blocks / CTAS;
   for (int k = 0; k < steps; ++k) {
     A.out = out;
-    if (k + 1 < steps) A.out.p = nullptr;
-    int rc = launch_product<BN, kGram, FULL>(A, tri_tiles, batch, st);
-    if (!rc) rc = launch_product<BN, kSquare, FULL>(A, tri_tiles, batch, st);
-    if (!rc) rc = launch_product<BN, kApply, FULL>(A, p.row_blocks * p.column_blocks * 64 / BN, batch, st);
+    if (k + 1 < steps) A.out.p = nullptr, A.out.update = 0;
+    int rc = launch_product<BN, kGram, FULL, CTAS>(A, tri_tiles, row_tiles, batch, st);
+    if (!rc) rc = launch_product<BN, kSquare, FULL, CTAS>(A, tri_tiles, row_tiles, batch, st);
+    if (!rc)
+      rc = launch_product<BN, kApply, FULL, CTAS>(A, row_tiles * (p.column_blocks * 64 / BN), row_tiles, batch, st);
     if (rc) return rc;
     const Matrix x = A.x;
     A.x = A.y;
@@ -549,8 +730,6 @@ static int run(int batch, const Plan &p, const Source &src, const Out &out, int 
   A.sq = {take(p.sq_bytes), p.full ? take(p.sq_bytes) : nullptr, sb, p.sq_column_blocks};
   A.poly = {take(p.sq_bytes), p.full ? take(p.sq_bytes) : nullptr, sb, p.sq_column_blocks};
   double *parts = reinterpret_cast<double *>(at);
-  A.row_blocks = p.row_blocks;
-  A.column_blocks = p.column_blocks;
   A.k_blocks_n = (p.n + 63) / 64;
   A.k_blocks_m = (p.m + 63) / 64;
   A.a = a;
@@ -558,17 +737,17 @@ static int run(int batch, const Plan &p, const Source &src, const Out &out, int 
   A.c = c;
   norm_kernel<<<dim3(p.parts, batch), kNormThreads, 0, st>>>(src, parts, A.status);
   split_kernel<<<dim3(p.row_blocks * 2 * p.column_blocks, batch), 256, 0, st>>>(
-      src, parts, p.parts, (double)eps, A.x, p.column_blocks);
+      src, parts, p.parts, (double)eps, A.x);
   count_launch(2);
   int rc = launch_status();
   if (rc) return rc;
   if (p.full)
-    return p.bn == 256   ? run_steps<256, true>(A, p, batch, steps, out, st)
-           : p.bn == 128 ? run_steps<128, true>(A, p, batch, steps, out, st)
-                         : run_steps<64, true>(A, p, batch, steps, out, st);
-  return p.bn == 256   ? run_steps<256, false>(A, p, batch, steps, out, st)
-         : p.bn == 128 ? run_steps<128, false>(A, p, batch, steps, out, st)
-                       : run_steps<64, false>(A, p, batch, steps, out, st);
+    return p.bn == 256   ? run_steps<256, true, 2>(A, p, batch, steps, out, st)
+           : p.bn == 128 ? run_steps<128, true, 1>(A, p, batch, steps, out, st)
+                         : run_steps<64, true, 1>(A, p, batch, steps, out, st);
+  return p.bn == 256   ? run_steps<256, false, 2>(A, p, batch, steps, out, st)
+         : p.bn == 128 ? run_steps<128, false, 1>(A, p, batch, steps, out, st)
+                       : run_steps<64, false, 1>(A, p, batch, steps, out, st);
 }
 
 static bool known_type(int type) {

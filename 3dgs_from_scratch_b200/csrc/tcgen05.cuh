@@ -8,16 +8,54 @@
 namespace gs {
 namespace tc {
 
-// Tensor memory: `columns` (a power of two from 32) of 128 lanes x 32 bits,
-// address written to shared memory; one whole warp allocates and frees.
-__device__ __forceinline__ void tmem_alloc(uint32_t *dst, uint32_t columns) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)),
-               "r"(columns)
-               : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+// CTAS = 1: a block by itself. CTAS = 2: the two blocks of a cluster work on
+// one tile (cta_group::2): each holds its half of A's rows and of B's in its
+// own shared memory and its half of the accumulator's rows in its own tensor
+// memory; block 0 issues for both.
+
+// One lane of a converged warp, the same one every time: the compiler then
+// keeps what the lane hands to the tensor core in uniform registers (an MMA
+// issued under a lane comparison took 77 cycles).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
 }
+
+// Tensor memory: `columns` (a power of two from 32) of 128 lanes x 32 bits,
+// address written to shared memory; one whole warp (of each block) allocates
+// and frees.
+template <int CTAS>
+__device__ __forceinline__ void tmem_alloc(uint32_t *dst, uint32_t columns) {
+  if (CTAS == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)),
+                 "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst)),
+                 "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+  }
+}
+template <int CTAS>
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t columns) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns));
+  if (CTAS == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns));
+  else
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns));
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Every thread of both blocks.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 __device__ __forceinline__ void fence_before() {
@@ -44,14 +82,22 @@ __host__ __device__ constexpr uint32_t instruction_f16(int m, int n, bool a_mn, 
          ((uint32_t)(m >> 4) << 24);
 }
 
-// D (+)= A B over 16 elements of K; one thread issues it for the block.
+// D (+)= A B over 16 elements of K; one thread issues it for the block or pair.
+template <int CTAS>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction,
                                         bool accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(instruction), "r"(accumulate ? 1u : 0u)
-      : "memory");
+  if (CTAS == 1)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(instruction), "r"(accumulate ? 1u : 0u)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(instruction), "r"(accumulate ? 1u : 0u)
+        : "memory");
 }
 
 __device__ __forceinline__ void arrive(uint64_t *bar) {
@@ -69,27 +115,62 @@ __device__ __forceinline__ void registers_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// Arrives on the barrier when the thread's MMAs so far are done.
-__device__ __forceinline__ void commit(uint64_t *bar) {
+// The same on the barrier at `bar`'s place in block `rank` of the cluster.
+__device__ __forceinline__ void arrive_at(uint64_t *bar, uint32_t rank) {
   asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+      "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n"
+      " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n}\n" ::"r"(smem_addr(bar)),
+      "r"(rank)
       : "memory");
 }
 
-// 32 columns of the warp's 32 lanes: thread l gets row l, columns addr...
+// Bounded wait that also orders what the other block did before it arrived.
+__device__ __forceinline__ bool wait_cluster(uint64_t *bar, uint32_t parity) {
+  for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+
+// Arrives on the barrier (of both blocks of a pair) when the thread's MMAs so
+// far are done.
+template <int CTAS>
+__device__ __forceinline__ void commit(uint64_t *bar) {
+  if (CTAS == 1)
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+        : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_addr(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+
+// 32 columns of the warp's 32 lanes: thread l gets row l, columns addr... The
+// wait belongs to the same statement, so that nothing is read before it.
 __device__ __forceinline__ void load_columns(uint32_t addr, float (&v)[32]) {
   uint32_t r[32];
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
         "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
         "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
         "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(addr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      : "r"(addr)
+      : "memory");
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
