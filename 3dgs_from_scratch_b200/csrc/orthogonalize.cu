@@ -35,6 +35,8 @@
 // Padding to whole blocks is zero from the start and stays zero.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cstdlib>
+#include <type_traits>
 
 #include "tcgen05.cuh"
 
@@ -42,7 +44,6 @@ namespace gs {
 namespace ns {
 
 constexpr int kBlockBytes = 128 * 64 * 2;
-constexpr int kEpilogueWarps = 8;  // two for each quarter of tensor memory's lanes
 constexpr int kMaxStages = 8;
 constexpr float kScale = 4096.f, kUnscale = 1.f / 4096.f;
 
@@ -74,6 +75,14 @@ struct Args {
   Out out;
   uint32_t *status;
 };
+
+// Launches of one call overlap: each may start its set-up while the one before
+// it still runs, and touches global memory only after that one is complete.
+__device__ __forceinline__ void start_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("fence.proxy.async.global;" ::: "memory");  // the bulk copies read what it wrote
+}
 
 __device__ __forceinline__ char *block_at(char *plane, const Matrix &M, int batch, int rb, int cb) {
   return plane + (int64_t)batch * M.batch_bytes + ((int64_t)rb * M.column_blocks + cb) * kBlockBytes;
@@ -109,10 +118,36 @@ __device__ __forceinline__ uint32_t fetch_rows(char *plane, const Matrix &M, int
 
 // An operand's descriptor, and what 16 elements of K further add to it: 32
 // bytes along a row, or 16 rows of 128 bytes (in units of 16 bytes).
-__device__ __forceinline__ uint64_t operand(uint32_t addr, bool mn) {
-  return mn ? tc::descriptor(addr, kBlockBytes / 2, 1024) : tc::descriptor(addr, 16, 1024);
+template <bool MN>
+__device__ __forceinline__ uint64_t operand(uint32_t addr) {
+  return MN ? tc::descriptor(addr, kBlockBytes / 2, 1024) : tc::descriptor(addr, 16, 1024);
 }
-__device__ __forceinline__ uint32_t k_step(bool mn) { return mn ? 128 : 2; }
+
+// The MMAs of one K block. `main` takes hi hi, `cross` hi lo and lo hi (it may
+// be the same accumulator).
+template <class S, bool A_MN, bool B_MN, bool FRESH>
+__device__ __forceinline__ void issue_block(uint32_t at, uint32_t main, uint32_t cross) {
+  constexpr uint32_t kInstr = tc::instruction_f16(128 * S::kCtas, S::kBN, A_MN, B_MN);
+  constexpr int kA = A_MN ? 128 : 2, kB = B_MN ? 128 : 2;
+  const uint64_t a = operand<A_MN>(at), b = operand<B_MN>(at + S::kPlanesA * S::kPlaneA);
+  constexpr int kLoA = S::kPlaneA / 16, kLoB = S::kPlaneB / 16;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (FRESH && k == 0) tc::mma_f16<S::kCtas, false, kInstr>(main, a, b);
+    else tc::mma_f16<S::kCtas, true, kInstr>(main, a + k * kA, b + k * kB);
+  }
+  if (S::kPlanesB == 2) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (FRESH && S::kCross && k == 0) tc::mma_f16<S::kCtas, false, kInstr>(cross, a, b + kLoB);
+      else tc::mma_f16<S::kCtas, true, kInstr>(cross, a + k * kA, b + kLoB + k * kB);
+    }
+  }
+  if (S::kPlanesA == 2) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) tc::mma_f16<S::kCtas, true, kInstr>(cross, a + kLoA + k * kA, b + k * kB);
+  }
+}
 
 __device__ __forceinline__ void split8(const float *v, uint4 &hi, uint4 &lo) {
   __half h[8], l[8];
@@ -129,6 +164,34 @@ __device__ __forceinline__ void add8(const uint4 &q, float (&v)[8]) {
   const __half *h = reinterpret_cast<const __half *>(&q);
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] += __half2float(h[i]);
+}
+
+// 32 rows x 64 columns of a block, 4 KB of its image: between global memory,
+// where the warp moves 512 adjacent bytes at a time, and registers, where
+// thread l holds row l's 16-byte chunks in the order of its columns. `turn` is
+// the warp's 4 KB of shared memory; both of its access patterns are free of bank
+// conflicts (the swizzle). Accesses by row straight to global memory touch 32
+// lines each: they took 9 us of a 256 x 256 tile per direction.
+__device__ __forceinline__ void load_image(const char *at, char *turn, uint4 (&q)[8]) {
+  const int lane = (int)lane_id();
+#pragma unroll
+  for (int e = 0; e < 8; ++e) q[e] = *reinterpret_cast<const uint4 *>(at + e * 512 + lane * 16);
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4 *>(turn + e * 512 + lane * 16) = q[e];
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 8; ++e) q[e] = *reinterpret_cast<const uint4 *>(turn + chunk_at(lane, 8 * e));
+}
+__device__ __forceinline__ void store_image(char *at, char *turn, const uint4 (&q)[8]) {
+  const int lane = (int)lane_id();
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4 *>(turn + chunk_at(lane, 8 * e)) = q[e];
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    *reinterpret_cast<uint4 *>(at + e * 512 + lane * 16) = *reinterpret_cast<const uint4 *>(turn + e * 512 + lane * 16);
 }
 
 __device__ __forceinline__ void store_as(void *p, int type, int64_t at, float v) {
@@ -181,6 +244,7 @@ __device__ __forceinline__ void store_result(const Out &o, int batch, int row, i
 
 template <int BN, int KIND, bool FULL, int CTAS>
 struct Shape {
+  static constexpr int kBN = BN, kCtas = CTAS;
   static constexpr int kPlanesA = FULL ? 2 : 1;
   static constexpr int kPlanesB = FULL || KIND == kApply ? 2 : 1;
   static constexpr int kRowsB = BN / CTAS;                 // of B's rows in each block
@@ -194,9 +258,12 @@ struct Shape {
   static constexpr bool kCross = FULL && BN <= 128;
   static constexpr int kWidth = kCross ? 2 * BN : BN;      // columns of tensor memory
   static constexpr int kColumns = 2 * kWidth;              // two accumulators take turns
-  // A copy warp, an MMA warp and the epilogue. Where an epilogue thread holds
-  // 64 or 128 sums, a whole warpgroup goes to the first two, so that it can hand its
-  // registers over: 384 threads x 168 = 128 x 40 + 256 x 232.
+  // A copy warp, an MMA warp and the epilogue, whose warps hold 32 rows x 64
+  // (128) columns each. Where the registers of 64 such sums and more would not
+  // go round, a whole warpgroup goes to the first two, so that it can hand its
+  // own over: 384 threads x 168 = 128 x 40 + 256 x 232.
+  static constexpr int kEpilogueWarps = BN == 64 ? 4 : 8;
+  static constexpr int kHeld = BN * 4 / kEpilogueWarps;    // columns of an epilogue warp
   static constexpr bool kHandOver = BN >= 128;
   static constexpr int kEpilogue = kHandOver ? 4 : 2;      // its first warp
   static constexpr int kThreads = 32 * (kEpilogue + kEpilogueWarps);
@@ -227,7 +294,7 @@ __global__ void __launch_bounds__(Shape<BN, KIND, FULL, CTAS>::kThreads, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&ready[s], 1);
-      mbar_init(&drained[s], kEpilogueWarps * CTAS);
+      mbar_init(&drained[s], S::kEpilogueWarps * CTAS);
     }
     failed = 0;
     fence_mbar_init();
@@ -238,6 +305,8 @@ __global__ void __launch_bounds__(Shape<BN, KIND, FULL, CTAS>::kThreads, 1)
   if (CTAS == 2) tc::cluster_sync();
   tc::fence_after();
   const uint32_t tmem = tmem_base;
+  start_next();
+  wait_for_previous();
   // Tile t: its matrix, row of tiles and column of tiles.
   struct Spot {
     int batch, i, j;
@@ -265,123 +334,122 @@ __global__ void __launch_bounds__(Shape<BN, KIND, FULL, CTAS>::kThreads, 1)
 
   if (S::kHandOver && warp < S::kEpilogue) tc::registers_down<40>();
   if (warp == 0) {
-    const Matrix &MA = KIND == kGram ? A.x : KIND == kSquare ? A.sq : A.poly;
-    const Matrix &MB = KIND == kSquare ? A.sq : A.x;
-    int it = 0, done = 0;
-    bool good = true;
-    for (int t = first; t < total && good; t += step) {
-      const Spot p = spot(t);
-      const int row_a = (p.i * CTAS + rank) * 128, row_b = p.j * BN + rank * S::kRowsB;
-      for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-        const int s = it % A.stages, round = it / A.stages;
-        good = __all_sync(0xffffffffu, round == 0 || mbar_wait(&empty[s], (round - 1) & 1));
-        if (!good) break;
-        done = it + 1;
-        if (!tc::elect_one()) continue;
-        char *a = smem + (size_t)s * S::kStage, *b = a + S::kPlanesA * S::kPlaneA;
-        mbar_expect_tx(&full[s], S::kStage);
-        for (int q = 0; q < S::kPlanesA; ++q)
-          fetch_rows(q ? MA.lo : MA.hi, MA, p.batch, row_a, 128, kb, below(row_a, kb),
-                     a + q * S::kPlaneA, &full[s]);
-        for (int q = 0; q < S::kPlanesB; ++q)
-          fetch_rows(q ? MB.lo : MB.hi, MB, p.batch, row_b, S::kRowsB, kb,
-                     KIND == kApply || (KIND == kSquare && below(p.j * BN, kb)),
-                     b + q * S::kPlaneB, &full[s]);
-      }
-    }
-    if (!good) {  // given up: the copies in flight still land here
-      failed = 1;
-      for (int q = done > A.stages ? done - A.stages : 0; q < done; ++q)
-        mbar_wait(&full[q % A.stages], (q / A.stages) & 1);
-    }
-  } else if (warp == 1 && rank == 1) {  // tells block 0 what has arrived here
-    int it = 0;
-    bool good = true;
-    for (int t = first; t < total && good; t += step)
-      for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-        good = __all_sync(0xffffffffu, mbar_wait(&full[it % A.stages], (it / A.stages) & 1));
-        if (!good) break;
-        if (tc::elect_one()) tc::arrive_at(&peer[it % A.stages], 0);
-      }
-    if (!good) failed = 1;
-  } else if (warp == 1) {
-    int it = 0, chunk = 0;
-    bool good = true;
-    for (int t = first; t < total && good; t += step) {
-      const Spot p = spot(t);
-      for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-        const int s = it % A.stages, acc = chunk & 1;
-        const bool fresh = kb % S::kChunk == 0, last = kb % S::kChunk == S::kChunk - 1 || kb == k_blocks - 1;
-        bool ok = mbar_wait(&full[s], (it / A.stages) & 1);
-        if (CTAS == 2) ok = ok && tc::wait_cluster(&peer[s], (it / A.stages) & 1);
-        if (fresh && chunk >= 2) ok = ok && tc::wait_cluster(&drained[acc], (chunk / 2 - 1) & 1);
-        good = __all_sync(0xffffffffu, ok);
-        if (!good) break;
-        tc::fence_after();
-        const uint32_t at = smem_addr(smem) + s * S::kStage;
-        const bool a_mn = below(p.i * CTAS * 128, kb);
-        const bool b_mn = KIND == kApply || (KIND == kSquare && below(p.j * BN, kb));
-        // One lane issues, so the loop holds an addition or two for each MMA.
-        const uint64_t a = operand(at, a_mn), b = operand(at + S::kPlanesA * S::kPlaneA, b_mn);
-        const uint32_t instr = tc::instruction_f16(128 * CTAS, BN, a_mn, b_mn);
-        const uint32_t a_step = k_step(a_mn), b_step = k_step(b_mn);
-        const uint32_t main = tmem + acc * S::kWidth, cross = S::kCross ? main + BN : main;
-        if (tc::elect_one()) {
+    if (tc::elect_one()) {
+      const Matrix &MA = KIND == kGram ? A.x : KIND == kSquare ? A.sq : A.poly;
+      const Matrix &MB = KIND == kSquare ? A.sq : A.x;
+      int s = 0, used = 0;
+      uint32_t phase = 1;  // of the slot's last reader; the first round has none
+      bool good = true;
+      for (int t = first; t < total && good; t += step) {
+        const Spot p = spot(t);
+        const int row_a = (p.i * CTAS + rank) * 128, row_b = p.j * BN + rank * S::kRowsB;
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          good = used < A.stages || mbar_wait(&empty[s], phase);
+          if (!good) break;
+          char *a = smem + (size_t)s * S::kStage, *b = a + S::kPlanesA * S::kPlaneA;
+          mbar_expect_tx(&full[s], S::kStage);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc::mma_f16<CTAS>(main, a + k * a_step, b + k * b_step, instr, k > 0 || !fresh);
-          if (S::kPlanesB == 2) {  // hi lo
+          for (int q = 0; q < S::kPlanesA; ++q)
+            fetch_rows(q ? MA.lo : MA.hi, MA, p.batch, row_a, 128, kb, below(row_a, kb),
+                       a + q * S::kPlaneA, &full[s]);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              tc::mma_f16<CTAS>(cross, a + k * a_step, b + (S::kPlaneB / 16) + k * b_step, instr,
-                                k > 0 || !S::kCross || !fresh);
-          }
-          if (S::kPlanesA == 2) {  // lo hi
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              tc::mma_f16<CTAS>(cross, a + (S::kPlaneA / 16) + k * a_step, b + k * b_step, instr, true);
-          }
-          tc::commit<CTAS>(&empty[s]);
-          if (last) tc::commit<CTAS>(&ready[acc]);
+          for (int q = 0; q < S::kPlanesB; ++q)
+            fetch_rows(q ? MB.lo : MB.hi, MB, p.batch, row_b, S::kRowsB, kb,
+                       KIND == kApply || (KIND == kSquare && below(p.j * BN, kb)),
+                       b + q * S::kPlaneB, &full[s]);
+          ++used;
+          if (++s == A.stages) s = 0, phase ^= 1;
         }
-        __syncwarp();
-        chunk += last;
+      }
+      if (!good) {  // given up: the copies in flight still land here
+        failed = 1;
+        for (int q = used > A.stages ? used - A.stages : 0; q < used; ++q)
+          mbar_wait(&full[q % A.stages], (q / A.stages) & 1);
       }
     }
-    if (!good) failed = 1;
+  } else if (warp == 1 && rank == 1) {
+    if (tc::elect_one()) {  // tells block 0 what has arrived here
+      int s = 0;
+      uint32_t phase = 0;
+      bool good = true;
+      for (int t = first; t < total && good; t += step)
+        for (int kb = 0; kb < k_blocks && good; ++kb) {
+          good = mbar_wait(&full[s], phase);
+          if (good) tc::arrive_at(&peer[s], 0);
+          if (++s == A.stages) s = 0, phase ^= 1;
+        }
+      if (!good) failed = 1;
+    }
+  } else if (warp == 1) {
+    if (tc::elect_one()) {
+      int s = 0, chunk = 0;
+      uint32_t phase = 0;
+      bool good = true;
+      for (int t = first; t < total && good; t += step) {
+        const Spot p = spot(t);
+        int left = 0;  // K blocks to go in this accumulator
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          const int acc = chunk & 1;
+          const bool fresh = left == 0;
+          if (fresh) left = k_blocks - kb < S::kChunk ? k_blocks - kb : S::kChunk;
+          good = (!fresh || chunk < 2 || tc::wait_cluster(&drained[acc], (chunk / 2 - 1) & 1)) &&
+                 mbar_wait(&full[s], phase) && (CTAS == 1 || tc::wait_cluster(&peer[s], phase));
+          if (!good) break;
+          tc::fence_after();
+          const uint32_t at = smem_addr(smem) + s * S::kStage;
+          const bool a_mn = below(p.i * CTAS * 128, kb);
+          const bool b_mn = KIND == kApply || (KIND == kSquare && below(p.j * BN, kb));
+          const uint32_t main = tmem + acc * S::kWidth, cross = S::kCross ? main + BN : main;
+          const auto issue = [&](auto a_is_mn, auto b_is_mn) {
+            if (fresh) issue_block<S, decltype(a_is_mn)::value, decltype(b_is_mn)::value, true>(at, main, cross);
+            else issue_block<S, decltype(a_is_mn)::value, decltype(b_is_mn)::value, false>(at, main, cross);
+          };
+          using Yes = std::true_type;
+          using No = std::false_type;
+          if (KIND == kGram) issue(No(), No());
+          else if (KIND == kApply && a_mn) issue(Yes(), Yes());
+          else if (KIND == kApply) issue(No(), Yes());
+          else if (a_mn && b_mn) issue(Yes(), Yes());
+          else if (a_mn) issue(Yes(), No());
+          else if (b_mn) issue(No(), Yes());
+          else issue(No(), No());
+          tc::commit<CTAS>(&empty[s]);
+          if (--left == 0) {
+            tc::commit<CTAS>(&ready[acc]);
+            ++chunk;
+          }
+          if (++s == A.stages) s = 0, phase ^= 1;
+        }
+      }
+      if (!good) failed = 1;
+    }
   } else if (warp >= S::kEpilogue) {
     if (S::kHandOver) tc::registers_up<232>();
     const int quarter = warp & 3;  // the lanes of tensor memory that the warp may read
-    const int r = quarter * 32 + (int)lane_id();
-    const int c0 = (warp - S::kEpilogue) / 4 * (BN / 2);
+    const int c0 = (warp - S::kEpilogue) / 4 * S::kHeld;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + c0;
-    float(*turn)[33] = reinterpret_cast<float(*)[33]>(smem + (size_t)A.stages * S::kStage) +
-                       (warp - S::kEpilogue) * 32;
+    char *turn = smem + (size_t)A.stages * S::kStage + (warp - S::kEpilogue) * (32 * 33 * 4);
     const Matrix &dst = KIND == kGram ? A.sq : KIND == kSquare ? A.poly : A.y;
     const Matrix &old = KIND == kSquare ? A.sq : A.x;
-    constexpr bool kOldLo = FULL || KIND == kApply;
-    // The old values of a small tile are on their way before its products are done.
-    constexpr bool kAhead = KIND != kGram && BN <= 128;
-    constexpr int kOld = KIND == kGram ? 1 : kAhead ? BN / 16 : 4;
+    constexpr bool kLo = FULL || KIND == kApply;  // of the old and the new values
+    // The old values of one block are on their way before the products are done.
+    constexpr bool kAhead = KIND != kGram && S::kHeld == 64;
     int chunk = 0;
     bool good = true;
     for (int t = first; t < total && good; t += step) {
       const Spot p = spot(t);
       const int i = p.i * CTAS + rank;  // the block's rows: 128 i..
-      uint4 oh[kOld], ol[kOld];
-      const auto load_old = [&](int from, int count) {
-#pragma unroll
-        for (int q = 0; q < count; ++q) {
-          const int col = p.j * BN + c0 + from + 8 * q, at = chunk_at(r, col);
-          oh[q] = *reinterpret_cast<const uint4 *>(block_at(old.hi, old, p.batch, i, col / 64) + at);
-          if (kOldLo)
-            ol[q] = *reinterpret_cast<const uint4 *>(block_at(old.lo, old, p.batch, i, col / 64) + at);
-        }
+      const auto image = [&](char *plane, const Matrix &M, int c) {
+        return block_at(plane, M, p.batch, i, (p.j * BN + c0 + c) / 64) + quarter * 4096;
       };
-      if (kAhead) load_old(0, kOld);
-      float v[BN / 2];
+      uint4 hi[8], lo[8];
+      if (kAhead) {
+        load_image(image(old.hi, old, 0), turn, hi);
+        if (kLo) load_image(image(old.lo, old, 0), turn, lo);
+      }
+      float v[S::kHeld];
 #pragma unroll
-      for (int e = 0; e < BN / 2; ++e) v[e] = 0.f;
+      for (int e = 0; e < S::kHeld; ++e) v[e] = 0.f;
 #pragma unroll 1
       for (int part = 0; part < chunks; ++part, ++chunk) {
         const int acc = chunk & 1;
@@ -389,7 +457,7 @@ __global__ void __launch_bounds__(Shape<BN, KIND, FULL, CTAS>::kThreads, 1)
         if (!good) break;
         tc::fence_after();
 #pragma unroll
-        for (int c = 0; c < BN / 2; c += 32) {
+        for (int c = 0; c < S::kHeld; c += 32) {
           float f[32];
           tc::load_columns(lanes + acc * S::kWidth + c, f);
 #pragma unroll
@@ -410,46 +478,45 @@ __global__ void __launch_bounds__(Shape<BN, KIND, FULL, CTAS>::kThreads, 1)
       if (!good) break;
       if (A.out.update && ld_volatile_u32(A.status) != 0u) continue;  // the optimizers' gate
 #pragma unroll
-      for (int c = 0; c < BN / 2; c += 32) {
-        asm volatile("" ::: "memory");  // one group's loads at a time: registers
-        if (KIND != kGram && !kAhead) load_old(c, 4);
-        float w[32];
+      for (int c = 0; c < S::kHeld; c += 64) {
+        if (KIND != kGram && !kAhead) {
+          load_image(image(old.hi, old, c), turn, hi);
+          if (kLo) load_image(image(old.lo, old, c), turn, lo);
+        }
+        const float f = KIND == kSquare ? A.b : A.a, h = KIND == kSquare ? A.c * kUnscale : kUnscale;
 #pragma unroll
-        for (int g = 0; g < 32; g += 8) {
-          if (KIND == kGram) {
+        for (int g = 0; g < 8; ++g) {
+          float o[8] = {};
+          if (KIND != kGram) {
+            add8(hi[g], o);
+            if (kLo) add8(lo[g], o);
+          }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[g + e] = v[c + g + e] * kUnscale;
-          } else {
-            float o[8] = {};
-            const int q = kAhead ? (c + g) / 8 : g / 8;
-            add8(oh[q], o);
-            if (kOldLo) add8(ol[q], o);
-            const float f = KIND == kSquare ? A.b : A.a, h = KIND == kSquare ? A.c * kUnscale : kUnscale;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[g + e] = fmaf(f, o[e], h * v[c + g + e]);
+          for (int e = 0; e < 8; ++e) {
+            float &x = v[c + 8 * g + e];
+            x = KIND == kGram ? x * kUnscale : fmaf(f, o[e], h * x);
           }
         }
-        const int col0 = p.j * BN + c0 + c;
-        asm volatile("" ::: "memory");
         if (KIND == kApply && A.out.p != nullptr) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) w[e] *= kUnscale;
-          store_result(A.out, p.batch, i * 128 + quarter * 32, col0, w, turn);
+          for (int g = 0; g < 64; g += 32) {
+            float w[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) w[e] = v[c + g + e] * kUnscale;
+            store_result(A.out, p.batch, i * 128 + quarter * 32, p.j * BN + c0 + c + g, w,
+                         reinterpret_cast<float(*)[33]>(turn));
+          }
         } else {
 #pragma unroll
-          for (int g = 0; g < 32; g += 8) {
-            const int col = col0 + g, at = chunk_at(r, col);
-            uint4 hi, lo;
-            split8(w + g, hi, lo);
-            *reinterpret_cast<uint4 *>(block_at(dst.hi, dst, p.batch, i, col / 64) + at) = hi;
-            if (FULL || KIND == kApply)
-              *reinterpret_cast<uint4 *>(block_at(dst.lo, dst, p.batch, i, col / 64) + at) = lo;
-          }
+          for (int g = 0; g < 8; ++g) split8(v + c + 8 * g, hi[g], lo[g]);
+          store_image(image(dst.hi, dst, c), turn, hi);
+          if (kLo) store_image(image(dst.lo, dst, c), turn, lo);
         }
       }
     }
     if (!good) failed = 1;
   }
+  __syncwarp();
   tc::fence_before();
   __syncthreads();
   if (CTAS == 2) tc::cluster_sync();  // neither block leaves while the other may reach into it
@@ -487,52 +554,85 @@ __device__ __forceinline__ float update_of(const Source &s, float m_new, float g
   return s.nesterov ? fmaf(s.beta, m_new, s.fresh * g) : m_new;
 }
 
+// Eight adjacent elements, in 16-byte loads (the caller knows that they fit).
+__device__ __forceinline__ void read8(const void *p, int type, int64_t at, float (&v)[8]) {
+  if (type == GS_TYPE_F32) {
+    const float4 *q = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + at);
+    const float4 a = q[0], b = q[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+    const uint4 q = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(p) + at);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint16_t h = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+      v[e] = type == GS_TYPE_BF16 ? __bfloat162float(__ushort_as_bfloat16(h)) : __half2float(__ushort_as_half(h));
+    }
+  }
+}
+// Whether rows of 8 adjacent elements can be read so everywhere.
+__device__ __forceinline__ bool vector_rows(const Source &s, int64_t stride) {
+  const int each = s.type == GS_TYPE_F32 ? 4 : 8;
+  return (((uintptr_t)s.u | (uintptr_t)s.momentum) & 15) == 0 && stride % each == 0 &&
+         s.batch_stride % each == 0 && (s.momentum == nullptr || (stride % 4 == 0 && s.batch_stride % 4 == 0));
+}
+
 constexpr int kNormThreads = 256, kMaxParts = 296;
 
 // Sums of squares, in 64 bits so that neither tiny nor huge gradients leave
-// the range; the momentum is updated on the way. A warp takes a line of
-// elements that are adjacent (or the smaller stride apart) at a time. Parts
-// are added in order by the reader.
+// the range; the momentum is updated on the way. A matrix in one
+// piece is read in 16-byte loads, others a line at a time along the smaller
+// stride. Parts are added in order by the reader.
 __global__ void __launch_bounds__(kNormThreads) norm_kernel(const Source s, double *parts,
                                                             const uint32_t *status) {
+  start_next();
   if (s.momentum != nullptr && ld_volatile_u32(status) != 0u) return;
   const int64_t base = (int64_t)blockIdx.y * s.batch_stride;
   const bool cols_fast = s.col_stride <= s.row_stride;
-  int64_t lines = cols_fast ? s.rows : s.cols, len = cols_fast ? s.cols : s.rows;
-  int64_t fs = cols_fast ? s.col_stride : s.row_stride, ss = cols_fast ? s.row_stride : s.col_stride;
+  const int64_t lines = cols_fast ? s.rows : s.cols, len = cols_fast ? s.cols : s.rows;
+  const int64_t fs = cols_fast ? s.col_stride : s.row_stride, ss = cols_fast ? s.row_stride : s.col_stride;
   const int64_t size = (int64_t)s.rows * s.cols;
-  if (fs == 1 && ss == len) {  // one piece of memory, in lines of 1024
-    len = 1024;
-    ss = 1024;
-    lines = (size + 1023) / 1024;
-  } else {
-    len = len < size ? len : size;
-  }
-  const bool flat = fs == 1 && ss == 1024 && len == 1024;
+  const int64_t warp = (int64_t)blockIdx.x * (kNormThreads / 32) + threadIdx.x / 32;
+  const int64_t warps_all = (int64_t)gridDim.x * (kNormThreads / 32);
   double sum = 0.0;
-  for (int64_t k = (int64_t)blockIdx.x * (kNormThreads / 32) + threadIdx.x / 32; k < lines;
-       k += (int64_t)gridDim.x * (kNormThreads / 32)) {
-    const int64_t here = flat && size - k * 1024 < len ? size - k * 1024 : len;
-    for (int64_t f0 = lane_id(); f0 < here; f0 += 32 * 8) {
-      float v[8], m[8];
+  const auto take = [&](int64_t at, float v, float m) {
+    if (s.momentum != nullptr) {
+      m = next_momentum(s, m, v);
+      s.momentum[at] = m;
+      v = update_of(s, m, v);
+    }
+    sum = fma((double)v, (double)v, sum);
+  };
+  if (fs == 1 && ss == len && vector_rows(s, 8)) {  // one piece of memory
+    for (int64_t k = warp * 1024; k < size; k += warps_all * 1024) {
+      float v[4][8], m[4][8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int64_t f = f0 + 32 * e, at = base + k * ss + f * fs;
-        v[e] = f < here ? read_f32(s.u, s.type, at) : 0.f;
-        if (s.momentum != nullptr) m[e] = f < here ? s.momentum[at] : 0.f;
+      for (int q = 0; q < 4; ++q) {
+        const int64_t at = k + q * 256 + lane_id() * 8;
+        if (at + 8 <= size) {
+          read8(s.u, s.type, base + at, v[q]);
+          if (s.momentum != nullptr) read8(s.momentum, GS_TYPE_F32, base + at, m[q]);
+        }
       }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int64_t f = f0 + 32 * e, at = base + k * ss + f * fs;
-        if (f >= here) continue;
-        if (s.momentum != nullptr) {
-          m[e] = next_momentum(s, m[e], v[e]);
-          s.momentum[at] = m[e];
-          v[e] = update_of(s, m[e], v[e]);
+      for (int q = 0; q < 4; ++q) {
+        const int64_t at = k + q * 256 + lane_id() * 8;
+        if (at + 8 <= size) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) take(base + at + e, v[q][e], m[q][e]);
+        } else {
+          for (int64_t f = at; f < size; ++f)
+            take(base + f, read_f32(s.u, s.type, base + f), s.momentum != nullptr ? s.momentum[base + f] : 0.f);
         }
-        sum = fma((double)v[e], (double)v[e], sum);
       }
     }
+  } else {
+    for (int64_t k = warp; k < lines; k += warps_all)
+#pragma unroll 4
+      for (int64_t f = lane_id(); f < len; f += 32) {
+        const int64_t at = base + k * ss + f * fs;
+        take(at, read_f32(s.u, s.type, at), s.momentum != nullptr ? s.momentum[at] : 0.f);
+      }
   }
   __shared__ double warps[kNormThreads / 32];
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_down_sync(0xffffffffu, sum, d);
@@ -551,6 +651,8 @@ __global__ void __launch_bounds__(256) split_kernel(const Source s, const double
                                                     double eps, Matrix x) {
   __shared__ float tile[64][65];
   __shared__ double total;
+  start_next();
+  wait_for_previous();
   const int batch = blockIdx.y, r0 = blockIdx.x / x.column_blocks * 64, c0 = blockIdx.x % x.column_blocks * 64;
   if (threadIdx.x < 32) {
     double sum = 0.0;
@@ -572,6 +674,7 @@ __global__ void __launch_bounds__(256) split_kernel(const Source s, const double
     return (float)((double)v * scale);
   };
   const bool cols_fast = s.col_stride <= s.row_stride;
+  const bool wide = s.col_stride == 1 && vector_rows(s, s.row_stride);
   if (!cols_fast) {
 #pragma unroll 4
     for (int k = threadIdx.x; k < 64 * 64; k += 256) tile[k % 64][k / 64] = read(k % 64, k / 64);
@@ -582,7 +685,24 @@ __global__ void __launch_bounds__(256) split_kernel(const Source s, const double
     const int r = k / 8, c = k % 8 * 8;
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = cols_fast ? read(r, c + e) : tile[r][c + e];
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    if (!cols_fast) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = tile[r][c + e];
+    } else if (wide && r0 + r < s.rows && c0 + c + 8 <= s.cols) {
+      const int64_t at = base + (r0 + r) * s.row_stride + c0 + c;
+      read8(s.u, s.type, at, v);
+      float m[8];
+      if (s.momentum != nullptr) read8(s.momentum, GS_TYPE_F32, at, m);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (s.momentum != nullptr) v[e] = update_of(s, m[e], v[e]);
+        v[e] = (float)((double)v[e] * scale);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = read(r, c + e);
+    }
     uint4 hi, lo;
     split8(v, hi, lo);
     const int at = chunk_at((r0 + r) % 128, c);
@@ -601,14 +721,40 @@ struct Plan {
   size_t x_bytes, sq_bytes, total;  // of a plane and of everything, all batches
 };
 
+// What a step costs in tiles of 128 ctas x bn, in microseconds: rounds of
+// tiles, each its K blocks at the slower of the copies (the L2 hands an SM
+// about 60 bytes a nanosecond) and the MMAs, and a constant for filling and
+// draining.
+static double cost_of(int batch, int m, int n, bool full, int bn, int ctas) {
+  const int tri = bn > 128 * ctas ? bn : 128 * ctas, rows = 128 * ctas;
+  const int sq = (m + tri - 1) / tri, per = tri / rows;  // superblocks, rows of tiles in one
+  const int64_t half = (int64_t)(sq * (sq + 1) / 2) * per * (tri / bn);
+  const int64_t whole = (int64_t)sq * per * ((n + bn - 1) / bn);
+  const int at_once = 148 / ctas, kn = (n + 63) / 64, km = (m + 63) / 64;
+  const auto block = [&](int planes_a, int planes_b, int products) {
+    const double copy = (planes_a * 128 + planes_b * (bn / ctas)) * 128 / 60e3;
+    const double mma = products * 4 * (bn == 64 ? 48 : bn / 2) / 1.7e3;
+    return copy > mma ? copy : mma;
+  };
+  const auto rounds = [&](int64_t tiles) { return (double)((tiles * batch + at_once - 1) / at_once); };
+  const double syrk = block(full ? 2 : 1, full ? 2 : 1, full ? 3 : 1), apply = block(full ? 2 : 1, 2, full ? 3 : 2);
+  return rounds(half) * (2.0 + kn * syrk) + rounds(half) * (2.0 + km * syrk) + rounds(whole) * (2.0 + km * apply);
+}
+
 static Plan make_plan(int batch, int rows, int cols, int type) {
   Plan p;
   p.m = rows < cols ? rows : cols;
   p.n = rows < cols ? cols : rows;
   p.full = type != GS_TYPE_BF16;
-  const auto tiles = [&](int bn) { return (int64_t)batch * ((p.m + 127) / 128) * ((p.n + bn - 1) / bn); };
-  p.bn = tiles(256) >= 148 ? 256 : tiles(128) >= 148 ? 128 : 64;
-  p.ctas = p.bn == 256 ? 2 : 1;
+  const char *force = getenv("NS_FORCE");
+  double best = 0.0;
+  p.bn = 0;
+  const int shapes[4][2] = {{64, 1}, {128, 1}, {128, 2}, {256, 2}};
+  for (const auto &q : shapes) {
+    const double cost = cost_of(batch, p.m, p.n, p.full, q[0], q[1]);
+    if (p.bn == 0 || cost < best) best = cost, p.bn = q[0], p.ctas = q[1];
+  }
+  if (force) { p.bn = atoi(force) / 10; p.ctas = atoi(force) % 10; }
   const int tri = p.bn > 128 * p.ctas ? p.bn : 128 * p.ctas;
   const int mp = (p.m + tri - 1) / tri * tri, np = (p.n + p.bn - 1) / p.bn * p.bn;
   p.row_blocks = mp / 128;
@@ -621,6 +767,13 @@ static Plan make_plan(int batch, int rows, int cols, int type) {
   p.sq_bytes = (size_t)batch * p.row_blocks * p.sq_column_blocks * kBlockBytes;
   p.total = 4 * p.x_bytes + (p.full ? 4 : 2) * p.sq_bytes + (size_t)batch * p.parts * 8;
   return p;
+}
+
+static cudaLaunchAttribute overlapping() {
+  cudaLaunchAttribute a{};
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  return a;
 }
 
 template <int BN, int KIND, bool FULL, int CTAS>
@@ -638,12 +791,13 @@ static int launch_product(Args A, int tiles, int row_tiles, int batch, cudaStrea
   thread_local int resident = 0;
   const unsigned long long ctx = current_context_id();
   cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = CTAS;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1] = overlapping();
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
@@ -736,16 +890,25 @@ static int run(int batch, const Plan &p, const Source &src, const Out &out, int 
   A.b = b;
   A.c = c;
   norm_kernel<<<dim3(p.parts, batch), kNormThreads, 0, st>>>(src, parts, A.status);
-  split_kernel<<<dim3(p.row_blocks * 2 * p.column_blocks, batch), 256, 0, st>>>(
-      src, parts, p.parts, (double)eps, A.x);
-  count_launch(2);
   int rc = launch_status();
   if (rc) return rc;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr = overlapping();
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3(p.row_blocks * 2 * p.column_blocks, batch);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  rc = cuda_status(cudaLaunchKernelEx(&cfg, split_kernel, src, (const double *)parts, p.parts, (double)eps, A.x));
+  if (rc) return rc;
+  count_launch(2);
   if (p.full)
     return p.bn == 256   ? run_steps<256, true, 2>(A, p, batch, steps, out, st)
+           : p.bn == 128 && p.ctas == 2 ? run_steps<128, true, 2>(A, p, batch, steps, out, st)
            : p.bn == 128 ? run_steps<128, true, 1>(A, p, batch, steps, out, st)
                          : run_steps<64, true, 1>(A, p, batch, steps, out, st);
   return p.bn == 256   ? run_steps<256, false, 2>(A, p, batch, steps, out, st)
+         : p.bn == 128 && p.ctas == 2 ? run_steps<128, false, 2>(A, p, batch, steps, out, st)
          : p.bn == 128 ? run_steps<128, false, 1>(A, p, batch, steps, out, st)
                        : run_steps<64, false, 1>(A, p, batch, steps, out, st);
 }

@@ -13,9 +13,7 @@ namespace tc {
 // own shared memory and its half of the accumulator's rows in its own tensor
 // memory; block 0 issues for both.
 
-// One lane of a converged warp, the same one every time: the compiler then
-// keeps what the lane hands to the tensor core in uniform registers (an MMA
-// issued under a lane comparison took 77 cycles).
+// One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
@@ -82,21 +80,23 @@ __host__ __device__ constexpr uint32_t instruction_f16(int m, int n, bool a_mn, 
          ((uint32_t)(m >> 4) << 24);
 }
 
-// D (+)= A B over 16 elements of K; one thread issues it for the block or pair.
-template <int CTAS>
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction,
-                                        bool accumulate) {
+// D = A B (ADD: D += A B) over 16 elements of K; one lane issues it for the
+// block or pair. What kind of instruction it is is known at compile time: with
+// the instruction descriptor or the predicate in registers each issue took
+// about 100 cycles, 48 (64, 128) otherwise for N = 64 (128, 256).
+template <int CTAS, bool ADD, uint32_t INSTRUCTION>
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b) {
   if (CTAS == 1)
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
         " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(instruction), "r"(accumulate ? 1u : 0u)
+        "l"(a), "l"(b), "n"(INSTRUCTION), "n"(ADD ? 1 : 0)
         : "memory");
   else
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
         " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(instruction), "r"(accumulate ? 1u : 0u)
+        "l"(a), "l"(b), "n"(INSTRUCTION), "n"(ADD ? 1 : 0)
         : "memory");
 }
 
@@ -115,11 +115,14 @@ __device__ __forceinline__ void registers_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-// The same on the barrier at `bar`'s place in block `rank` of the cluster.
+// The same on the barrier at `bar`'s place in block `rank` of the cluster. With
+// an explicit release at cluster scope every arrival took about 1 us; nothing
+// that this orders is written by the arriving thread (bulk copies and MMAs
+// complete on barriers of their own before it).
 __device__ __forceinline__ void arrive_at(uint64_t *bar, uint32_t rank) {
   asm volatile(
       "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n"
-      " mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n}\n" ::"r"(smem_addr(bar)),
+      " mbarrier.arrive.shared::cluster.b64 _, [a];\n}\n" ::"r"(smem_addr(bar)),
       "r"(rank)
       : "memory");
 }
