@@ -149,21 +149,28 @@ __device__ __forceinline__ void issue_block(uint32_t at, uint32_t main, uint32_t
   }
 }
 
+// Eight values as hi + lo, two at a time (the packed conversions run at several
+// times the rate of single ones).
 __device__ __forceinline__ void split8(const float *v, uint4 &hi, uint4 &lo) {
-  __half h[8], l[8];
+  uint32_t *h = &hi.x, *l = &lo.x;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    h[i] = __float2half_rn(v[i]);
-    l[i] = __float2half_rn(v[i] - __half2float(h[i]));
+  for (int i = 0; i < 4; ++i) {
+    const __half2 a = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    const float2 f = __half22float2(a);
+    const __half2 b = __floats2half2_rn(v[2 * i] - f.x, v[2 * i + 1] - f.y);
+    h[i] = *reinterpret_cast<const uint32_t *>(&a);
+    l[i] = *reinterpret_cast<const uint32_t *>(&b);
   }
-  hi = *reinterpret_cast<uint4 *>(h);
-  lo = *reinterpret_cast<uint4 *>(l);
 }
 
 __device__ __forceinline__ void add8(const uint4 &q, float (&v)[8]) {
-  const __half *h = reinterpret_cast<const __half *>(&q);
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] += __half2float(h[i]);
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+    v[2 * i] += f.x;
+    v[2 * i + 1] += f.y;
+  }
 }
 
 // 32 rows x 64 columns of a block, 4 KB of its image: between global memory,
@@ -577,6 +584,38 @@ __device__ __forceinline__ bool vector_rows(const Source &s, int64_t stride) {
          s.batch_stride % each == 0 && (s.momentum == nullptr || (stride % 4 == 0 && s.batch_stride % 4 == 0));
 }
 
+// The sum of 8 squares: in fp32 where neither the largest nor what matters next
+// to it can leave the range, else in 64 bits.
+__device__ __forceinline__ double squares(const float (&v)[8]) {
+  float most = 0.f, sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    most = fmaxf(most, fabsf(v[e]));
+    sum = fmaf(v[e], v[e], sum);
+  }
+  if (most > 1e-14f && most < 1e14f) return (double)sum;
+  double wide = 0.0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) wide = fma((double)v[e], (double)v[e], wide);
+  return wide;
+}
+
+// 2^12 / max(norm, eps), applied in fp32 where it is a normal number.
+struct Scale {
+  double wide;
+  float narrow;
+  bool fits;
+  __device__ __forceinline__ Scale(double sum_of_squares, double eps) {
+    const double norm = sqrt(sum_of_squares);
+    wide = (double)kScale / (norm < eps ? eps : norm);
+    narrow = (float)wide;
+    fits = wide > 1e-30 && wide < 1e30;
+  }
+  __device__ __forceinline__ float operator()(float v) const {
+    return fits ? v * narrow : (float)((double)v * wide);
+  }
+};
+
 constexpr int kNormThreads = 256, kMaxParts = 296;
 
 // Sums of squares, in 64 bits so that neither tiny nor huge gradients leave
@@ -618,8 +657,17 @@ __global__ void __launch_bounds__(kNormThreads) norm_kernel(const Source s, doub
       for (int q = 0; q < 4; ++q) {
         const int64_t at = k + q * 256 + lane_id() * 8;
         if (at + 8 <= size) {
+          if (s.momentum != nullptr) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) take(base + at + e, v[q][e], m[q][e]);
+            for (int e = 0; e < 8; ++e) {
+              m[q][e] = next_momentum(s, m[q][e], v[q][e]);
+              v[q][e] = update_of(s, m[q][e], v[q][e]);
+            }
+            float4 *to = reinterpret_cast<float4 *>(s.momentum + base + at);
+            to[0] = make_float4(m[q][0], m[q][1], m[q][2], m[q][3]);
+            to[1] = make_float4(m[q][4], m[q][5], m[q][6], m[q][7]);
+          }
+          sum += squares(v[q]);
         } else {
           for (int64_t f = at; f < size; ++f)
             take(base + f, read_f32(s.u, s.type, base + f), s.momentum != nullptr ? s.momentum[base + f] : 0.f);
@@ -650,7 +698,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_kernel(const Source s, doub
 __global__ void __launch_bounds__(256) split_kernel(const Source s, const double *parts, int num_parts,
                                                     double eps, Matrix x) {
   __shared__ float tile[64][65];
-  __shared__ double total;
+  __shared__ double total;  // sum of squares
   start_next();
   wait_for_previous();
   const int batch = blockIdx.y, r0 = blockIdx.x / x.column_blocks * 64, c0 = blockIdx.x % x.column_blocks * 64;
@@ -658,20 +706,17 @@ __global__ void __launch_bounds__(256) split_kernel(const Source s, const double
     double sum = 0.0;
     for (int k = threadIdx.x; k < num_parts; k += 32) sum += parts[(int64_t)batch * num_parts + k];
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_down_sync(0xffffffffu, sum, d);
-    if (threadIdx.x == 0) {
-      const double norm = sqrt(sum);
-      total = (double)kScale / (norm < eps ? eps : norm);
-    }
+    if (threadIdx.x == 0) total = sum;
   }
   __syncthreads();
-  const double scale = total;
+  const Scale scale(total, eps);
   const int64_t base = (int64_t)batch * s.batch_stride;
   const auto read = [&](int r, int c) {
     if (r0 + r >= s.rows || c0 + c >= s.cols) return 0.f;
     const int64_t at = base + (r0 + r) * s.row_stride + (c0 + c) * s.col_stride;
     float v = read_f32(s.u, s.type, at);
     if (s.momentum != nullptr) v = update_of(s, s.momentum[at], v);
-    return (float)((double)v * scale);
+    return scale(v);
   };
   const bool cols_fast = s.col_stride <= s.row_stride;
   const bool wide = s.col_stride == 1 && vector_rows(s, s.row_stride);
@@ -697,7 +742,7 @@ __global__ void __launch_bounds__(256) split_kernel(const Source s, const double
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if (s.momentum != nullptr) v[e] = update_of(s, m[e], v[e]);
-        v[e] = (float)((double)v[e] * scale);
+        v[e] = scale(v[e]);
       }
     } else {
 #pragma unroll
@@ -711,6 +756,321 @@ __global__ void __launch_bounds__(256) split_kernel(const Source s, const double
   }
 }
 
+// ---- small matrices -----------------------------------------------------------------
+//
+// Up to 128 rows, a matrix stays on chip for the whole call: a block (or a
+// cluster of C blocks, NC columns each) keeps its columns of X and the whole of
+// A in shared memory, in the same block images, and runs norm, steps and result
+// in one launch. A launch for each product took 5 to 6 us each, 17 of them.
+// In a cluster every block forms the part of A = X X^T that its columns give;
+// block k adds the parts of its 128 / C rows in the blocks' order and hands the
+// result to all. B = b A + c A A is cheap enough to be formed by each block.
+constexpr int kSmallThreads = 512;  // four warps for each quarter of tensor memory's lanes
+
+struct SmallArgs {
+  Source src;
+  Out out;
+  int cluster, steps;
+  float a, b, c;
+  double eps;
+  uint32_t *status;
+};
+
+// X has up to MC rows. The MMAs' M is 128: what their rows beyond MC hold is
+// neither set nor looked at.
+template <int MC, int NC>
+struct SmallShape {
+  static constexpr int kBlocks = NC / 64;
+  static constexpr int kX = kBlocks * kBlockBytes;          // a plane of X
+  static constexpr int kSq = MC / 64 * kBlockBytes;         // a plane of A or B
+  static constexpr int kPart = NC == 128 ? MC * MC * 4 : 0;  // a block's part of A (clusters)
+  static constexpr int kTurn = kSmallThreads / 32 * 32 * 33 * 4;  // in place of A and the part, or behind
+  static constexpr int kRest = 2 * kSq + kPart > kTurn ? 2 * kSq + kPart : kTurn;
+  static constexpr int kBytes = 2 * kX + kRest;
+  static constexpr int kTop = NC > MC ? NC : MC;            // columns of an accumulator
+};
+
+// All MMAs of D = P Q^T (or P Q, Q's rows along K) over `blocks` K blocks:
+// hi hi into main, hi lo + lo hi into cross.
+template <int N, bool Q_MN>
+__device__ __forceinline__ void small_product(uint32_t main, uint32_t cross, uint32_t p, uint32_t p_lo,
+                                              uint32_t q, uint32_t q_lo, int blocks) {
+  constexpr uint32_t kInstr = tc::instruction_f16(128, N, false, Q_MN);
+  // K-major: a block of 64 K per image, 16 of them 32 bytes further. MN-major:
+  // 16 rows of 128 bytes, images 64 columns apart.
+  const auto q_at = [&](uint32_t base, int kb, int k) {
+    return Q_MN ? tc::descriptor(base + (kb * 4 + k) * 2048, kBlockBytes, 1024)
+                : tc::descriptor(base + kb * kBlockBytes + k * 32, 16, 1024);
+  };
+  for (int kb = 0; kb < blocks; ++kb) {
+    const bool fresh = kb == 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint64_t a = tc::descriptor(p + kb * kBlockBytes + k * 32, 16, 1024);
+      if (fresh && k == 0) tc::mma_f16<1, false, kInstr>(main, a, q_at(q, kb, k));
+      else tc::mma_f16<1, true, kInstr>(main, a, q_at(q, kb, k));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint64_t a = tc::descriptor(p + kb * kBlockBytes + k * 32, 16, 1024);
+      if (fresh && k == 0) tc::mma_f16<1, false, kInstr>(cross, a, q_at(q_lo, kb, k));
+      else tc::mma_f16<1, true, kInstr>(cross, a, q_at(q_lo, kb, k));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      tc::mma_f16<1, true, kInstr>(cross, tc::descriptor(p_lo + kb * kBlockBytes + k * 32, 16, 1024),
+                                   q_at(q, kb, k));
+  }
+}
+
+template <int MC, int NC>
+__global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_constant__ SmallArgs A) {
+  using S = SmallShape<MC, NC>;
+  extern __shared__ char raw[];
+  char *x_hi = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023), *x_lo = x_hi + S::kX;
+  char *sq_hi = x_lo + S::kX, *sq_lo = sq_hi + S::kSq, *part = sq_lo + S::kSq;
+  __shared__ uint64_t done;
+  __shared__ uint32_t tmem_base, failed;
+  __shared__ double warp_sums[kSmallThreads / 32], block_sum;
+  const int warp = threadIdx.x / 32, lane = (int)lane_id();
+  const int C = A.cluster, rank = C > 1 ? (int)tc::cluster_rank() : 0, batch = blockIdx.x / C;
+  const int col_base = rank * NC;  // of X
+  const Source &s = A.src;
+  if (threadIdx.x == 0) {
+    mbar_init(&done, 1);
+    failed = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) tc::tmem_alloc<1>(&tmem_base, 2 * S::kTop);
+  // Skipped optimizer steps run through, so that the blocks of a cluster stay
+  // together, and write nothing.
+  const bool skip = A.out.update && ld_volatile_u32(A.status) != 0u;
+
+  // The update, 8 columns of a row at a time, and its sum of squares.
+  constexpr int kEach = MC * NC / 8 / kSmallThreads;
+  const bool cols_fast = s.col_stride <= s.row_stride;
+  const bool wide = s.col_stride == 1 && vector_rows(s, s.row_stride);
+  const int64_t base = (int64_t)batch * s.batch_stride;
+  float u[kEach][8];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int at = k * kSmallThreads + threadIdx.x;
+    const int r = cols_fast ? at / (NC / 8) : at % MC, c = (cols_fast ? at % (NC / 8) : at / MC) * 8;
+    const int col = col_base + c;
+    const int64_t from = base + r * s.row_stride + col * s.col_stride;
+    if (wide && r < s.rows && col + 8 <= s.cols) {
+      read8(s.u, s.type, from, u[k]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        u[k][e] = r < s.rows && col + e < s.cols ? read_f32(s.u, s.type, from + e * s.col_stride) : 0.f;
+    }
+  }
+  if (s.momentum != nullptr) {
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int at = k * kSmallThreads + threadIdx.x;
+      const int r = cols_fast ? at / (NC / 8) : at % MC, c = (cols_fast ? at % (NC / 8) : at / MC) * 8;
+      const int col = col_base + c;
+      const int64_t from = base + r * s.row_stride + col * s.col_stride;
+      float m[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        m[e] = r < s.rows && col + e < s.cols ? s.momentum[from + e * s.col_stride] : 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        m[e] = next_momentum(s, m[e], u[k][e]);
+        if (!skip && r < s.rows && col + e < s.cols) s.momentum[from + e * s.col_stride] = m[e];
+        u[k][e] = update_of(s, m[e], u[k][e]);
+      }
+    }
+  }
+  double sum = 0.0;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) sum += squares(u[k]);
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_down_sync(0xffffffffu, sum, d);
+  if (lane == 0) warp_sums[warp] = sum;
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kSmallThreads / 32; ++w) sum += warp_sums[w];
+    block_sum = sum;
+  }
+  double total = 0.0;
+  if (C > 1) {
+    tc::cluster_sync();
+    for (int k = 0; k < C; ++k) total += tc::cluster_load_f64(tc::cluster_addr(&block_sum, k));
+  } else {
+    __syncthreads();
+    total = block_sum;
+  }
+  const Scale scale(total, A.eps);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int at = k * kSmallThreads + threadIdx.x;
+    const int r = cols_fast ? at / (NC / 8) : at % MC, c = (cols_fast ? at % (NC / 8) : at / MC) * 8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = scale(u[k][e]);
+    uint4 hi, lo;
+    split8(v, hi, lo);
+    const int to = c / 64 * kBlockBytes + chunk_at(r, c);
+    *reinterpret_cast<uint4 *>(x_hi + to) = hi;
+    *reinterpret_cast<uint4 *>(x_lo + to) = lo;
+  }
+  const uint32_t tmem = tmem_base, cross = tmem + S::kTop;
+  const int quarter = warp & 3, group = warp / 4, r = quarter * 32 + lane;
+  const bool on = quarter * 32 < MC;  // the warp's rows are X's
+  const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+  uint32_t phase = 0;
+  const auto run = [&](auto issue) {  // what was written is read by the tensor core
+    fence_proxy_async_smem();
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 0 && tc::elect_one()) {
+      tc::fence_after();
+      issue();
+      tc::commit<1>(&done);
+    }
+    __syncwarp();
+    if (!mbar_wait(&done, phase)) failed = 1;
+    phase ^= 1;
+    __syncwarp();
+    tc::fence_after();
+  };
+  // 32 columns of the product for this thread's row.
+  const auto columns = [&](int c, float (&v)[32]) {
+    tc::load_sum(tmem + lanes + c, cross + lanes + c, v);
+  };
+  // w = f old + g w for 8 columns, old from the image that the result replaces.
+  const auto blend = [&](char *hi_at, char *lo_at, float f, float g, const float *v, float (&w)[8]) {
+    float o[8] = {};
+    add8(*reinterpret_cast<const uint4 *>(hi_at), o);
+    add8(*reinterpret_cast<const uint4 *>(lo_at), o);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = fmaf(f, o[e], g * v[e]);
+  };
+  const auto put = [&](char *hi_at, char *lo_at, const float *w) {
+    uint4 hi, lo;
+    split8(w, hi, lo);
+    *reinterpret_cast<uint4 *>(hi_at) = hi;
+    *reinterpret_cast<uint4 *>(lo_at) = lo;
+  };
+
+  for (int step = 0; step < A.steps; ++step) {
+    run([&] {
+      small_product<MC, false>(tmem, cross, smem_addr(x_hi), smem_addr(x_lo), smem_addr(x_hi),
+                               smem_addr(x_lo), S::kBlocks);
+    });
+    if (on && group * 32 < MC) {
+      const int c = group * 32;
+      float v[32];
+      columns(c, v);
+      if (C == 1) {
+#pragma unroll
+        for (int g = 0; g < 32; g += 8) {
+          float w[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w[e] = v[g + e] * kUnscale;
+          const int to = (c + g) / 64 * kBlockBytes + chunk_at(r, c + g);
+          put(sq_hi + to, sq_lo + to, w);
+        }
+      } else if (S::kPart > 0) {  // rows of MC floats, their 16-byte chunks swizzled
+#pragma unroll
+        for (int g = 0; g < 32; g += 4)
+          *reinterpret_cast<float4 *>(part + r * (MC * 4) + ((((c + g) / 4) ^ (r & (MC / 4 - 1))) << 4)) =
+              make_float4(v[g], v[g + 1], v[g + 2], v[g + 3]);
+      }
+    }
+    if (S::kPart > 0 && C > 1) {
+      tc::cluster_sync();
+      const int rows = MC / C;
+      for (int k = threadIdx.x; k < rows * (MC / 8); k += kSmallThreads) {
+        const int row = rank * rows + k / (MC / 8), c = k % (MC / 8) * 8;
+        float4 f[8], g[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (q < C) {
+            const uint32_t from = tc::cluster_addr(part, q) + row * (MC * 4);
+            f[q] = tc::cluster_load(from + (((c / 4) ^ (row & (MC / 4 - 1))) << 4));
+            g[q] = tc::cluster_load(from + (((c / 4 + 1) ^ (row & (MC / 4 - 1))) << 4));
+          }
+        float w[8] = {};
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (q < C) {
+            w[0] += f[q].x, w[1] += f[q].y, w[2] += f[q].z, w[3] += f[q].w;
+            w[4] += g[q].x, w[5] += g[q].y, w[6] += g[q].z, w[7] += g[q].w;
+          }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] *= kUnscale;
+        uint4 hi, lo;
+        split8(w, hi, lo);
+        const int to = c / 64 * kBlockBytes + chunk_at(row, c);
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          if (q < C) {
+            tc::cluster_store(tc::cluster_addr(sq_hi + to, q), hi);
+            tc::cluster_store(tc::cluster_addr(sq_lo + to, q), lo);
+          }
+      }
+      asm volatile("fence.proxy.async;" ::: "memory");
+      __syncwarp();
+      tc::cluster_sync();
+    }
+    run([&] {
+      small_product<MC, false>(tmem, cross, smem_addr(sq_hi), smem_addr(sq_lo), smem_addr(sq_hi),
+                               smem_addr(sq_lo), MC / 64);
+    });
+    if (on && group * 32 < MC) {
+      const int c = group * 32;
+      float v[32];
+      columns(c, v);
+#pragma unroll
+      for (int g = 0; g < 32; g += 8) {
+        const int to = (c + g) / 64 * kBlockBytes + chunk_at(r, c + g);
+        float w[8];
+        blend(sq_hi + to, sq_lo + to, A.b, A.c * kUnscale, v + g, w);
+        put(sq_hi + to, sq_lo + to, w);
+      }
+    }
+    run([&] {
+      small_product<NC, true>(tmem, cross, smem_addr(sq_hi), smem_addr(sq_lo), smem_addr(x_hi),
+                              smem_addr(x_lo), MC / 64);
+    });
+    const bool last = step + 1 == A.steps;
+    if (on) {
+#pragma unroll 1
+      for (int c = group * 32; c < NC; c += 128) {
+        float v[32];
+        columns(c, v);
+#pragma unroll
+        for (int g = 0; g < 32; g += 8) {
+          const int to = (c + g) / 64 * kBlockBytes + chunk_at(r, c + g);
+          float w[8];
+          blend(x_hi + to, x_lo + to, A.a, kUnscale, v + g, w);
+          if (!last) put(x_hi + to, x_lo + to, w);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[g + e] = w[e] * kUnscale;
+        }
+        if (last && !skip)  // B is done with: its place serves to turn the result
+          store_result(A.out, batch, quarter * 32, col_base + c, v,
+                       reinterpret_cast<float(*)[33]>(sq_hi + warp * (32 * 33 * 4)));
+      }
+    }
+    __syncwarp();
+  }
+  tc::fence_before();
+  __syncthreads();
+  if (C > 1) tc::cluster_sync();  // no block leaves while another may reach into it
+  if (threadIdx.x == 0 && failed) atomicCAS(A.status, 0u, (uint32_t)GS_ERR_DEVICE_TIMEOUT);
+  if (warp == 0) {
+    tc::fence_after();
+    tc::tmem_free<1>(tmem, 2 * S::kTop);
+  }
+}
+
 // ---- host -----------------------------------------------------------------------------
 
 struct Plan {
@@ -720,6 +1080,19 @@ struct Plan {
   int parts;
   size_t x_bytes, sq_bytes, total;  // of a plane and of everything, all batches
 };
+
+// How a matrix of m <= 128 rows is cut for small_kernel: columns of a block (0:
+// too wide for it) and blocks.
+struct SmallPlan {
+  int columns, cluster;
+};
+static SmallPlan small_plan(int m, int n) {
+  if (m > 128 || n > 1024) return {0, 0};
+  if (n <= 64) return {64, 1};
+  if (n <= 128) return {128, 1};
+  if (n <= 256) return {256, 1};
+  return {128, n <= 512 ? 4 : 8};
+}
 
 // What a step costs in tiles of 128 ctas x bn, in microseconds: rounds of
 // tiles, each its K blocks at the slower of the copies (the L2 hands an SM
@@ -766,6 +1139,7 @@ static Plan make_plan(int batch, int rows, int cols, int type) {
   p.x_bytes = (size_t)batch * p.row_blocks * p.column_blocks * kBlockBytes;
   p.sq_bytes = (size_t)batch * p.row_blocks * p.sq_column_blocks * kBlockBytes;
   p.total = 4 * p.x_bytes + (p.full ? 4 : 2) * p.sq_bytes + (size_t)batch * p.parts * 8;
+  if (small_plan(p.m, p.n).columns) p.total = 16;  // all on chip
   return p;
 }
 
@@ -840,6 +1214,33 @@ static int run_steps(Args A, const Plan &p, int batch, int steps, const Out &out
   return GS_OK;
 }
 
+template <int MC, int NC>
+static int launch_small(const SmallArgs &A, int batch, cudaStream_t st) {
+  constexpr int kBytes = SmallShape<MC, NC>::kBytes + 1024;
+  thread_local unsigned long long ready = 0;
+  const unsigned long long ctx = current_context_id();
+  if (ctx == 0 || ctx != ready) {
+    const int rc = cuda_status(cudaFuncSetAttribute(small_kernel<MC, NC>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+    if (rc) return rc;
+    ready = ctx != 0 ? ctx : current_context_id();
+  }
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = A.cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3(batch * A.cluster);
+  cfg.blockDim = dim3(kSmallThreads);
+  cfg.dynamicSmemBytes = kBytes;
+  cfg.stream = st;
+  const int rc = cuda_status(cudaLaunchKernelEx(&cfg, small_kernel<MC, NC>, A));
+  if (rc) return rc;
+  count_launch();
+  return GS_OK;
+}
+
 // The largest |X|_2 and |b A + c A A|_2 that the steps can reach from
 // |X|_2 <= 1, from the extremes of the two polynomials on [0, r]. Both have to
 // stay below 8 for the fp16 range.
@@ -872,6 +1273,15 @@ static int run(int batch, const Plan &p, const Source &src, const Out &out, int 
   Args A{};
   A.status = device_status_word();
   if (A.status == nullptr) return GS_ERR_CUDA;
+  const SmallPlan small = small_plan(p.m, p.n);
+  if (small.columns) {
+    const SmallArgs B{src, out, small.cluster, steps, a, b, c, (double)eps, A.status};
+    if (p.m <= 64)
+      return small.columns == 64    ? launch_small<64, 64>(B, batch, st)
+             : small.columns == 128 ? launch_small<64, 128>(B, batch, st)
+                                    : launch_small<64, 256>(B, batch, st);
+    return small.columns == 128 ? launch_small<128, 128>(B, batch, st) : launch_small<128, 256>(B, batch, st);
+  }
   char *at = static_cast<char *>(scratch);
   const auto take = [&](size_t n) {
     char *q = at;

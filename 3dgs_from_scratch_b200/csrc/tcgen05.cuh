@@ -20,6 +20,31 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+// Shared memory of block `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_addr(const void *p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float4 cluster_load(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(at)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ double cluster_load_f64(uint32_t at) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_store(uint32_t at, const uint4 &v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z),
+               "r"(v.w)
+               : "memory");
+}
+
 // Tensor memory: `columns` (a power of two from 32) of 128 lanes x 32 bits,
 // address written to shared memory; one whole warp (of each block) allocates
 // and frees.
@@ -176,6 +201,43 @@ __device__ __forceinline__ void load_columns(uint32_t addr, float (&v)[32]) {
       : "memory");
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// The sum of 32 columns of two accumulators, both on their way at once.
+__device__ __forceinline__ void load_sum(uint32_t addr, uint32_t other, float (&v)[32]) {
+  uint32_t r[32], q[32];
+#define GS_TC_LD(R, ADDR)                                                                                  \
+  asm volatile(                                                                                            \
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "                                                            \
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "                            \
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"            \
+      : "=r"(R[0]), "=r"(R[1]), "=r"(R[2]), "=r"(R[3]), "=r"(R[4]), "=r"(R[5]), "=r"(R[6]), "=r"(R[7]),    \
+        "=r"(R[8]), "=r"(R[9]), "=r"(R[10]), "=r"(R[11]), "=r"(R[12]), "=r"(R[13]), "=r"(R[14]),           \
+        "=r"(R[15]), "=r"(R[16]), "=r"(R[17]), "=r"(R[18]), "=r"(R[19]), "=r"(R[20]), "=r"(R[21]),         \
+        "=r"(R[22]), "=r"(R[23]), "=r"(R[24]), "=r"(R[25]), "=r"(R[26]), "=r"(R[27]), "=r"(R[28]),         \
+        "=r"(R[29]), "=r"(R[30]), "=r"(R[31])                                                              \
+      : "r"(ADDR)                                                                                          \
+      : "memory")
+  GS_TC_LD(r, addr);
+  GS_TC_LD(q, other);
+#undef GS_TC_LD
+  // The wait takes the registers along, so that nothing reads them before it.
+#define GS_TC_PASS(R)                                                                                      \
+  asm volatile(""                                                                                          \
+               : "+r"(R[0]), "+r"(R[1]), "+r"(R[2]), "+r"(R[3]), "+r"(R[4]), "+r"(R[5]), "+r"(R[6]),       \
+                 "+r"(R[7]), "+r"(R[8]), "+r"(R[9]), "+r"(R[10]), "+r"(R[11]), "+r"(R[12]), "+r"(R[13]),   \
+                 "+r"(R[14]), "+r"(R[15]), "+r"(R[16]), "+r"(R[17]), "+r"(R[18]), "+r"(R[19]),             \
+                 "+r"(R[20]), "+r"(R[21]), "+r"(R[22]), "+r"(R[23]), "+r"(R[24]), "+r"(R[25]),             \
+                 "+r"(R[26]), "+r"(R[27]), "+r"(R[28]), "+r"(R[29])                                        \
+               :                                                                                           \
+               : "memory");                                                                                \
+  asm volatile("" : "+r"(R[30]), "+r"(R[31])::"memory")
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  GS_TC_PASS(r);
+  GS_TC_PASS(q);
+#undef GS_TC_PASS
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) + __uint_as_float(q[i]);
 }
 
 }  // namespace tc
