@@ -46,9 +46,10 @@ struct Args {
   void *h, *dx, *dgate;
   float *final_state, *dinitial;
   float *saved;      // (tiles, channels): the state before each tile
-  float2 *chains;    // (tiles, channels): each tile's (P, L)
-  uint32_t *cuts;    // (tiles): whether the chain is cut in the tile
-  float *carry;      // (tiles, channels): the state that enters each tile
+  uint32_t *ticket;  // hands out the tiles in the chain's order; null: one tile
+  uint32_t *flags;   // (tiles, channel blocks): the tile's map is in place
+  uint2 *groups;     // (groups, channels): the state after a group of tiles, and whether it is there
+  float2 *maps;      // (tiles, channels): each tile's (P, L)
   float *partial;    // (slots, rows, gates): gate gradients of channel blocks, or nullptr
   int slots;
   uint32_t *status;
@@ -70,21 +71,27 @@ int check_shape(int64_t rows, int sequences, int channels, int gates, int x_type
                 const int32_t *offsets);
 bool suits(const void *p, int64_t stride, int bytes, int vec);
 void fill_plan(Args &A, const Plan &p);
-void launch_carry(const Args &A, bool back, cudaStream_t st);
 
-// The scratch of the tiles' chains: maps, entering states, cuts.
+// Tiles of a group, whose last one passes the state on to the next group.
+constexpr int kGroup = 64;
+
+// The scratch of the tiles' chain: ticket, flags and group states (zeroed
+// before every launch), then the maps.
 inline size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
-inline size_t chain_bytes(const Plan &p, int channels) {
-  if (p.tiles == 1) return 0;
-  const size_t n = (size_t)p.tiles * channels;
-  return round16(n * 8) + round16(n * 4) + round16((size_t)p.tiles * 4);
+inline int64_t groups_of(const Plan &p) { return (p.tiles + kGroup - 1) / kGroup; }
+inline size_t zeroed_bytes(const Plan &p, int channels) {
+  return 16 + round16((size_t)p.tiles * p.channel_blocks * 4) + round16((size_t)groups_of(p) * channels * 8);
 }
-inline void place_chains(Args &A, const Plan &p, void *scratch) {
-  const size_t n = (size_t)p.tiles * A.channels;
+inline size_t chain_bytes(const Plan &p, int channels) {
+  return p.tiles == 1 ? 0 : zeroed_bytes(p, channels) + round16((size_t)p.tiles * channels * 8);
+}
+inline int place_chain(Args &A, const Plan &p, void *scratch, cudaStream_t st) {
   char *b = static_cast<char *>(scratch);
-  A.chains = reinterpret_cast<float2 *>(b);
-  A.carry = reinterpret_cast<float *>(b + round16(n * 8));
-  A.cuts = reinterpret_cast<uint32_t *>(b + round16(n * 8) + round16(n * 4));
+  A.ticket = reinterpret_cast<uint32_t *>(b);
+  A.flags = reinterpret_cast<uint32_t *>(b + 16);
+  A.groups = reinterpret_cast<uint2 *>(b + 16 + round16((size_t)p.tiles * p.channel_blocks * 4));
+  A.maps = reinterpret_cast<float2 *>(b + zeroed_bytes(p, A.channels));
+  return zero_async(scratch, zeroed_bytes(p, A.channels), st);
 }
 
 // ---- loads and stores of V consecutive elements ---------------------------------
@@ -391,16 +398,157 @@ __device__ __forceinline__ void put_segment(const Args &A, const Place &p, Tile<
   if (p.tx == 0) S.cut[p.sg] = cut;
 }
 
-// A segment's state before it, from the state that enters the tile.
+// A segment's state before it, from the state that enters the tile
+// (carry[channel of the block]).
 template <int V, int R>
 __device__ __forceinline__ void enter_segment(const Args &A, const Place &p, const Tile<V, R> &S,
-                                              const float *__restrict__ carry, float (&h)[V]) {
+                                              const float *carry, float (&h)[V]) {
   const bool cut = S.cut_before[p.sg];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const float2 m = S.map[(p.sg * A.tx + p.tx) * V + v];
-    h[v] = pass(cut, m.x, m.y, carry != nullptr ? carry[p.tile * A.channels + p.c + v] : 0.f);
+    h[v] = pass(cut, m.x, m.y, carry[p.tx * V + v]);
   }
+}
+
+// ---- the chain from tile to tile ---------------------------------------------------
+//
+// Blocks take their tiles by ticket, in the chain's order (position k counts
+// along it), so every tile that a block waits for is held by a block that runs
+// already. A tile puts its own map in place as soon as it has it. The state
+// that enters tile k is then: the state after the group of kGroup tiles before
+// k's own group, and the maps of the tiles between, folded in order; of the
+// tiles only those count that hold rows of the sequence that reaches into k. A
+// group's last tile passes the state on. What is added to what depends on
+// positions alone, so every run rounds alike. Waits are bounded; one that gives
+// up records GS_ERR_DEVICE_TIMEOUT.
+
+__device__ __forceinline__ uint32_t load_acquire(const uint32_t *p) {
+  uint32_t v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_release(uint32_t *p, uint32_t v) {
+  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+// A state and its flag in one 8-byte word, which arrives whole.
+__device__ __forceinline__ uint2 load_word(const uint2 *p) {
+  uint64_t v;
+  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+  return make_uint2((uint32_t)v, (uint32_t)(v >> 32));
+}
+__device__ __forceinline__ void store_word(uint2 *p, float state) {
+  const uint64_t v = (uint64_t)__float_as_uint(state) | (1ull << 32);
+  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
+}
+
+// The tile that this block takes: (position in the chain, channel block).
+__device__ __forceinline__ void take_tile(const Args &A, int64_t &position, int &cblk) {
+  __shared__ uint32_t mine;
+  uint32_t t = blockIdx.x;
+  if (A.ticket != nullptr) {
+    if (threadIdx.x == 0) mine = atomicAdd(A.ticket, 1u);
+    __syncthreads();
+    t = mine;
+  }
+  position = t / A.channel_blocks;
+  cblk = t % A.channel_blocks;
+}
+
+// First position of the chain of `in`, the info of the row at which the chain
+// enters position k (BACK: its last row): that of its sequence's first row, k
+// where nothing enters.
+template <bool BACK>
+__device__ __forceinline__ int64_t chain_start(const Args &A, int64_t k, int in) {
+  if (in < 0 || (in & (BACK ? 2 : 1))) return k;
+  const int s = in >> 2;
+  const int64_t a = A.offsets != nullptr ? A.offsets[s] : s * A.period;      // rows a..b-1
+  const int64_t b = A.offsets != nullptr ? A.offsets[s + 1] : (s + 1) * A.period;
+  const int64_t t = (A.reverse != 0) != BACK ? A.rows - b : a;                // along the chain
+  // Against the direction tiles are counted from the end of whole tiles.
+  const int64_t shift = BACK ? A.tiles * A.tile_rows - A.rows : 0;
+  const int64_t at = (t + shift) / A.tile_rows;
+  return at < 0 ? 0 : at < k ? at : k;
+}
+
+// Publishes the tile's map (P, L; thread c for channel c of the block) and
+// finds the state that enters it, into carry[c]. All threads call it; it
+// synchronises.
+template <bool BACK>
+__device__ __forceinline__ void join_chain(const Args &A, int64_t k, int cblk, int width, int in,
+                                           bool cut, float P, float L, float *carry,
+                                           float2 *parts) {
+  const int c = threadIdx.x, at = cblk * width + c;
+  const bool mine = c < width && at < A.channels;
+  if (A.ticket == nullptr) {
+    if (c < width) carry[c] = 0.f;
+    __syncthreads();
+    return;
+  }
+  if (mine) A.maps[k * A.channels + at] = make_float2(P, L);
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) store_release(&A.flags[k * A.channel_blocks + cblk], 1u);
+  const int64_t group = k / kGroup, start = chain_start<BACK>(A, k, in);
+  const bool from_group = start < group * kGroup;
+  const int64_t base = from_group ? group * kGroup : start;
+  const int count = (int)(k - base);
+  bool late = false;
+  if (threadIdx.x < count) {  // count < kGroup <= threads
+    uint32_t spins = 0;
+    while (load_acquire(&A.flags[(base + threadIdx.x) * A.channel_blocks + cblk]) == 0u)
+      if (++spins == kSpinLimit) {
+        late = true;
+        break;
+      }
+  }
+  __syncthreads();
+  // The maps between, folded in up to threads / width runs of tiles.
+  const int runs = kThreads / width, run = c / width, cc = c % width;
+  if (run < runs) {
+    const int j0 = count * run / runs, j1 = count * (run + 1) / runs;
+    float p = 1.f, l = 0.f;
+    if (cblk * width + cc < A.channels) {
+      const float2 *m = A.maps + base * A.channels + cblk * width + cc;
+#pragma unroll 8
+      for (int j = j0; j < j1; ++j) {
+        const float2 f = __ldcg(m + (int64_t)j * A.channels);
+        // the chain's first tile holds the cut: only its L counts
+        const bool first = !from_group && j == 0;
+        l = first ? f.y : fmaf(f.x, l, f.y);
+        p = first ? 0.f : p * f.x;
+      }
+    }
+    parts[run * width + cc] = make_float2(p, l);
+  }
+  __syncthreads();
+  if (mine) {
+    float h = 0.f;
+    if (from_group) {
+      const uint2 *word = A.groups + (group - 1) * A.channels + at;
+      uint2 v = load_word(word);
+      uint32_t spins = 0;
+      while (v.y == 0u) {
+        if (++spins == kSpinLimit) {
+          late = true;
+          break;
+        }
+        v = load_word(word);
+      }
+      h = __uint_as_float(v.x);
+    }
+    for (int q = 0; q < runs; ++q) {
+      const float2 f = parts[q * width + c];
+      const bool first = !from_group && count > 0 && count * q / runs == 0 && count * (q + 1) / runs > 0;
+      h = first ? f.y : fmaf(f.x, h, f.y);
+    }
+    if (k % kGroup == kGroup - 1) store_word(&A.groups[group * A.channels + at], pass(cut, P, L, h));
+    carry[c] = h;
+  } else if (c < width) {
+    carry[c] = 0.f;
+  }
+  if (late) atomicCAS(A.status, 0u, (uint32_t)GS_ERR_DEVICE_TIMEOUT);
+  __syncthreads();
 }
 
 }  // namespace scan

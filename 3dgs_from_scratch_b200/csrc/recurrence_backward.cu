@@ -16,12 +16,16 @@
 namespace gs {
 namespace scan {
 
-template <typename XT, typename GT, int V, int R, bool SHARED, bool CHAINS>
+template <typename XT, typename GT, int V, int R, bool SHARED>
 __global__ void __launch_bounds__(kThreads) backward_kernel(const Args A) {
   __shared__ Tile<V, R> S;
-  __shared__ float sums[SHARED && !CHAINS ? kThreads * R : 1];
-  const int cblk = blockIdx.x % A.channel_blocks;
-  const int64_t tile = A.tiles - 1 - blockIdx.x / A.channel_blocks;
+  __shared__ float sums[SHARED ? kThreads * R : 1];
+  __shared__ float carry[kThreads];
+  __shared__ float2 parts[kThreads];
+  int64_t position;
+  int cblk;
+  take_tile(A, position, cblk);
+  const int64_t tile = A.tiles - 1 - position;
   const Place p = place_of<V, R, SHARED>(A, tile, cblk);
   Pack<XT, V> x[R], dh[R];
   Gates<GT, V, SHARED> g[R];
@@ -29,8 +33,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const Args A) {
   for (int i = 0; i < R; ++i)
     if (i < p.rows) {
       const int64_t row = row_of<R>(A, p, i);
-      if (!CHAINS)
-        x[i] = load_pack<XT, V>(reinterpret_cast<const XT *>(A.x) + row * A.x_stride + p.c);
+      x[i] = load_pack<XT, V>(reinterpret_cast<const XT *>(A.x) + row * A.x_stride + p.c);
       if (A.dh != nullptr) {
         dh[i] = load_pack<XT, V>(reinterpret_cast<const XT *>(A.dh) + row * A.dh_stride + p.c);
       } else {
@@ -42,45 +45,44 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const Args A) {
   tile_info(A, tile, S.info);
   float P[V], L[V], tp, tl;
   float before[R][V];  // the state before each row
-  if (!CHAINS) {
-    reduce_segment<XT, GT, V, R, SHARED>(A, p, S.info, x, g, P, L);
-    put_segment<V, R>(A, p, S, segment_cut<R>(p, S.info, 1), P, L);
-    __syncthreads();
-    fold_segments<V, R, false>(A, S, tp, tl);
-    __syncthreads();
-    if (p.on) {
-      float h[V];
-      enter_segment<V, R>(A, p, S, A.saved, h);
+  reduce_segment<XT, GT, V, R, SHARED>(A, p, S.info, x, g, P, L);
+  put_segment<V, R>(A, p, S, segment_cut<R>(p, S.info, 1), P, L);
+  if (threadIdx.x < A.tx * V) {
+    const int c = cblk * A.tx * V + threadIdx.x;
+    carry[threadIdx.x] = c < A.channels ? A.saved[tile * A.channels + c] : 0.f;
+  }
+  __syncthreads();
+  fold_segments<V, R, false>(A, S, tp, tl);
+  __syncthreads();
+  if (p.on) {
+    float h[V];
+    enter_segment<V, R>(A, p, S, carry, h);
 #pragma unroll
-      for (int i = 0; i < R; ++i) {
-        if (i >= p.rows) break;
-        const int in = S.info[p.sg * R + i];
-        if (in >= 0 && (in & 1)) load_state<V>(A.initial, A, in >> 2, p.c, h);
+    for (int i = 0; i < R; ++i) {
+      if (i >= p.rows) break;
+      const int in = S.info[p.sg * R + i];
+      if (in >= 0 && (in & 1)) load_state<V>(A.initial, A, in >> 2, p.c, h);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          before[i][v] = h[v];
-          h[v] = in < 0 ? 0.f : fmaf(g[i](v), h[v], to_f32<XT>(x[i].e[v]));
-        }
+      for (int v = 0; v < V; ++v) {
+        before[i][v] = h[v];
+        h[v] = in < 0 ? 0.f : fmaf(g[i](v), h[v], to_f32<XT>(x[i].e[v]));
       }
     }
-    __syncthreads();
   }
+  __syncthreads();
   reduce_segment_back<XT, GT, V, R, SHARED>(A, p, S.info, dh, g, P, L);
   put_segment<V, R>(A, p, S, segment_cut<R>(p, S.info, 2), P, L);
   __syncthreads();
   const bool cut = fold_segments<V, R, true>(A, S, tp, tl);
-  if (CHAINS) {
-    const int c = cblk * A.tx * V + threadIdx.x;
-    if (threadIdx.x < A.tx * V && c < A.channels) A.chains[tile * A.channels + c] = make_float2(tp, tl);
-    if (cblk == 0 && threadIdx.x == 0) A.cuts[tile] = cut;
-    return;
-  }
-  __syncthreads();
+  const int64_t left_rows = A.rows - p.t0;
+  const int rows = left_rows < A.tile_rows ? (int)left_rows : A.tile_rows;
+  join_chain<true>(A, position, cblk, A.tx * V, rows > 0 ? S.info[rows - 1] : -1, cut, tp, tl, carry,
+                   parts);
   const int c1 = (cblk + 1) * A.tx * V < A.channels ? (cblk + 1) * A.tx * V : A.channels;
   empty_sequences(A, tile, cblk * A.tx * V, c1, A.dfinal, A.dinitial);
   if (p.on) {
     float after[V];
-    enter_segment<V, R>(A, p, S, A.carry, after);
+    enter_segment<V, R>(A, p, S, carry, after);
 #pragma unroll
     for (int i = R - 1; i >= 0; --i) {
       if (i >= p.rows) continue;
@@ -110,8 +112,6 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const Args A) {
   // The sums of the threads that share a gate, in their order.
   __syncthreads();
   const int c0 = cblk * A.tx * V, first = c0 / A.per_gate, count = (c1 - 1) / A.per_gate - first + 1;
-  const int64_t left = A.rows - p.t0;
-  const int rows = left < A.tile_rows ? (int)left : A.tile_rows;
   for (int k = threadIdx.x; k < rows * count; k += kThreads) {
     const int i = k / count, gate = first + k % count;
     const int lo = gate * A.per_gate > c0 ? gate * A.per_gate : c0;
@@ -144,12 +144,7 @@ __global__ void __launch_bounds__(kThreads) join_gates_kernel(const Args A, int 
 template <typename XT, typename GT, int V, int R, bool SHARED>
 static void launch_backward(const Args &A, cudaStream_t st) {
   const unsigned grid = (unsigned)(A.tiles * A.channel_blocks);
-  if (A.carry != nullptr) {
-    backward_kernel<XT, GT, V, R, SHARED, true><<<grid, kThreads, 0, st>>>(A);
-    count_launch();
-    launch_carry(A, true, st);
-  }
-  backward_kernel<XT, GT, V, R, SHARED, false><<<grid, kThreads, 0, st>>>(A);
+  backward_kernel<XT, GT, V, R, SHARED><<<grid, kThreads, 0, st>>>(A);
   count_launch();
   if (A.partial != nullptr && A.rows > 0) {
     const int64_t want = (A.rows * A.gates + kThreads - 1) / kThreads;
@@ -226,13 +221,16 @@ extern "C" int gs_gated_scan_backward(int64_t rows, int sequences, int channels,
     if (scratch_bytes < gs_gated_scan_scratch_bytes(rows, channels, gates, x_type, gate_type, 1))
       return GS_ERR_CAPACITY;
   }
-  if (p.tiles > 1) place_chains(A, p, scratch);
   if (p.slots > 1)
     A.partial = reinterpret_cast<float *>(static_cast<char *>(scratch) + chain_bytes(p, channels));
   A.status = device_status_word();
   if (A.status == nullptr) return GS_ERR_CUDA;
   const bool same = x_type == gate_type;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (p.tiles > 1) {
+    const int failed = place_chain(A, p, scratch, st);
+    if (failed) return failed;
+  }
   if (x_type == GS_TYPE_F32) pick_backward<float, float>(A, p.vec, st);
   else if (x_type == GS_TYPE_BF16 && same) pick_backward<__nv_bfloat16, __nv_bfloat16>(A, p.vec, st);
   else if (x_type == GS_TYPE_BF16) pick_backward<__nv_bfloat16, float>(A, p.vec, st);

@@ -48,11 +48,14 @@ __device__ __forceinline__ void load_rows(const Args &A, const Place &p, Pack<XT
     }
 }
 
-template <typename XT, typename GT, int V, int R, bool SHARED, bool CHAINS>
+template <typename XT, typename GT, int V, int R, bool SHARED>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const Args A) {
   __shared__ Tile<V, R> S;
-  const int cblk = blockIdx.x % A.channel_blocks;
-  const int64_t tile = blockIdx.x / A.channel_blocks;
+  __shared__ float carry[kThreads];
+  __shared__ float2 parts[kThreads];
+  int64_t tile;
+  int cblk;
+  take_tile(A, tile, cblk);
   const Place p = place_of<V, R, SHARED>(A, tile, cblk);
   Pack<XT, V> x[R];
   Gates<GT, V, SHARED> g[R];
@@ -64,18 +67,12 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args A) {
   __syncthreads();
   float tp, tl;
   const bool cut = fold_segments<V, R, false>(A, S, tp, tl);
-  if (CHAINS) {
-    const int c = cblk * A.tx * V + threadIdx.x;
-    if (threadIdx.x < A.tx * V && c < A.channels) A.chains[tile * A.channels + c] = make_float2(tp, tl);
-    if (cblk == 0 && threadIdx.x == 0) A.cuts[tile] = cut;
-    return;
-  }
-  __syncthreads();
+  join_chain<false>(A, tile, cblk, A.tx * V, S.info[0], cut, tp, tl, carry, parts);
   const int c1 = (cblk + 1) * A.tx * V < A.channels ? (cblk + 1) * A.tx * V : A.channels;
   empty_sequences(A, tile, cblk * A.tx * V, c1, A.initial, A.final_state);
   if (!p.on) return;
   float h[V];
-  enter_segment<V, R>(A, p, S, A.carry, h);
+  enter_segment<V, R>(A, p, S, carry, h);
   if (A.saved != nullptr && p.sg == 0) {
 #pragma unroll
     for (int v = 0; v < V; ++v) A.saved[tile * A.channels + p.c + v] = h[v];
@@ -97,36 +94,10 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const Args A) {
   }
 }
 
-// The state that enters each tile, from the tiles' maps; one thread a channel.
-template <bool BACK>
-__global__ void __launch_bounds__(kThreads) carry_kernel(const Args A) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= A.channels) return;
-  float h = 0.f;
-  for (int64_t k = 0; k < A.tiles; ++k) {
-    const int64_t t = BACK ? A.tiles - 1 - k : k;
-    A.carry[t * A.channels + c] = h;
-    const float2 m = A.chains[t * A.channels + c];
-    h = pass(A.cuts[t] != 0u, m.x, m.y, h);
-  }
-}
-
-void launch_carry(const Args &A, bool back, cudaStream_t st) {
-  const unsigned grid = (unsigned)((A.channels + kThreads - 1) / kThreads);
-  if (back) carry_kernel<true><<<grid, kThreads, 0, st>>>(A);
-  else carry_kernel<false><<<grid, kThreads, 0, st>>>(A);
-  count_launch();
-}
-
 template <typename XT, typename GT, int V, int R, bool SHARED>
 static void launch_forward(const Args &A, cudaStream_t st) {
   const unsigned grid = (unsigned)(A.tiles * A.channel_blocks);
-  if (A.carry != nullptr) {
-    forward_kernel<XT, GT, V, R, SHARED, true><<<grid, kThreads, 0, st>>>(A);
-    count_launch();
-    launch_carry(A, false, st);
-  }
-  forward_kernel<XT, GT, V, R, SHARED, false><<<grid, kThreads, 0, st>>>(A);
+  forward_kernel<XT, GT, V, R, SHARED><<<grid, kThreads, 0, st>>>(A);
   count_launch();
 }
 
@@ -237,10 +208,14 @@ extern "C" int gs_gated_scan_forward(int64_t rows, int sequences, int channels, 
   if (p.tiles > 1) {
     if (scratch == nullptr || ((uintptr_t)scratch & 15)) return GS_ERR_INVALID_ARGUMENT;
     if (scratch_bytes < chain_bytes(p, channels)) return GS_ERR_CAPACITY;
-    place_chains(A, p, scratch);
   }
   A.status = device_status_word();
   if (A.status == nullptr) return GS_ERR_CUDA;
-  run_forward(A, p, x_type, gate_type, reinterpret_cast<cudaStream_t>(stream));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (p.tiles > 1) {
+    const int failed = place_chain(A, p, scratch, st);
+    if (failed) return failed;
+  }
+  run_forward(A, p, x_type, gate_type, st);
   return launch_status();
 }
