@@ -17,83 +17,101 @@ namespace gs {
 namespace scan {
 
 template <typename XT, typename GT, int V, int R, bool SHARED>
-__global__ void __launch_bounds__(kThreads) backward_kernel(const Args A) {
-  __shared__ Tile<V, R> S;
+__global__ void __launch_bounds__(kThreads, kResident) backward_kernel(const __grid_constant__ Args A) {
+  __shared__ Tile<V> S;
+  __shared__ int info[kThreads * R];
   __shared__ float sums[SHARED ? kThreads * R : 1];
-  __shared__ float carry[kThreads];
-  __shared__ float2 parts[kThreads];
   int64_t position;
   int cblk;
   take_tile(A, position, cblk);
   const int64_t tile = A.tiles - 1 - position;
-  const Place p = place_of<V, R, SHARED>(A, tile, cblk);
+  const int width = A.tx * V, c0 = cblk * width, c1 = c0 + width < A.channels ? c0 + width : A.channels;
+  Place p = place_of<V, R, SHARED>(A, tile, cblk);
   Pack<XT, V> x[R], dh[R];
   Gates<GT, V, SHARED> g[R];
+  {  // all loads in flight before the first use
+    const XT *from = reinterpret_cast<const XT *>(A.x) + p.row * A.x_stride + p.c;
+    const XT *grad = reinterpret_cast<const XT *>(A.dh) + p.row * A.dh_stride + p.c;
+    const GT *gate = reinterpret_cast<const GT *>(A.gate) + p.row * A.gate_stride + p.g;
+    const int64_t xs = along(A, A.x_stride), gs = along(A, A.gate_stride), ds = along(A, A.dh_stride);
 #pragma unroll
-  for (int i = 0; i < R; ++i)
-    if (i < p.rows) {
-      const int64_t row = row_of<R>(A, p, i);
-      x[i] = load_pack<XT, V>(reinterpret_cast<const XT *>(A.x) + row * A.x_stride + p.c);
-      if (A.dh != nullptr) {
-        dh[i] = load_pack<XT, V>(reinterpret_cast<const XT *>(A.dh) + row * A.dh_stride + p.c);
-      } else {
+    for (int i = 0; i < R; ++i)
+      if (i < p.rows) {
+        x[i] = load_pack<XT, V>(from);
+        g[i].load(gate);
+        if (A.dh != nullptr) {
+          dh[i] = load_pack<XT, V>(grad);
+          grad += ds;
+        } else {
 #pragma unroll
-        for (int v = 0; v < V; ++v) dh[i].e[v] = from_f32<XT>(0.f);
+          for (int v = 0; v < V; ++v) dh[i].e[v] = from_f32<XT>(0.f);
+        }
+        from += xs;
+        gate += gs;
       }
-      g[i].load(A, row, p.g);
-    }
-  tile_info(A, tile, S.info);
-  float P[V], L[V], tp, tl;
+  }
+  if (threadIdx.x < width)
+    S.carry[threadIdx.x] = c0 + threadIdx.x < A.channels ? A.saved[tile * A.channels + c0 + threadIdx.x] : 0.f;
+  if (A.offsets != nullptr) tile_info(A, tile, info);
+  int in[R];
+  segment_info<R>(A, p, info, in);
   float before[R][V];  // the state before each row
-  reduce_segment<XT, GT, V, R, SHARED>(A, p, S.info, x, g, P, L);
-  put_segment<V, R>(A, p, S, segment_cut<R>(p, S.info, 1), P, L);
-  if (threadIdx.x < A.tx * V) {
-    const int c = cblk * A.tx * V + threadIdx.x;
-    carry[threadIdx.x] = c < A.channels ? A.saved[tile * A.channels + c] : 0.f;
+  {
+    float P[V], L[V];
+    reduce_segment<XT, GT, V, R, SHARED>(A, p, in, x, g, P, L);
+    put_segment<V>(A, p, S, segment_cut<R>(p, in, 1), P, L);
   }
   __syncthreads();
-  fold_segments<V, R, false>(A, S, tp, tl);
+  fold_runs<V, false>(A, S);
   __syncthreads();
-  if (p.on) {
+  if (p.rows > 0) {
     float h[V];
-    enter_segment<V, R>(A, p, S, carry, h);
+    enter_segment<V, false>(A, p, S, h);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       if (i >= p.rows) break;
-      const int in = S.info[p.sg * R + i];
-      if (in >= 0 && (in & 1)) load_state<V>(A.initial, A, in >> 2, p.c, h);
+      const int row = p.plain ? 0 : in[i];
+      if (row > 0 && (row & 1)) load_state<V>(A.initial, A, row >> 2, p.c, h);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         before[i][v] = h[v];
-        h[v] = in < 0 ? 0.f : fmaf(g[i](v), h[v], to_f32<XT>(x[i].e[v]));
+        h[v] = row < 0 ? 0.f : fmaf(g[i](v), h[v], to_f32<XT>(x[i].e[v]));
       }
     }
   }
+  {
+    float P[V], L[V];
+    reduce_segment_back<XT, GT, V, R, SHARED>(A, p, in, dh, g, P, L);
+    __syncthreads();
+    put_segment<V>(A, p, S, segment_cut<R>(p, in, 2), P, L);
+  }
   __syncthreads();
-  reduce_segment_back<XT, GT, V, R, SHARED>(A, p, S.info, dh, g, P, L);
-  put_segment<V, R>(A, p, S, segment_cut<R>(p, S.info, 2), P, L);
+  fold_runs<V, true>(A, S);
   __syncthreads();
-  const bool cut = fold_segments<V, R, true>(A, S, tp, tl);
-  const int64_t left_rows = A.rows - p.t0;
-  const int rows = left_rows < A.tile_rows ? (int)left_rows : A.tile_rows;
-  join_chain<true>(A, position, cblk, A.tx * V, rows > 0 ? S.info[rows - 1] : -1, cut, tp, tl, carry,
-                   parts);
-  const int c1 = (cblk + 1) * A.tx * V < A.channels ? (cblk + 1) * A.tx * V : A.channels;
-  empty_sequences(A, tile, cblk * A.tx * V, c1, A.dfinal, A.dinitial);
-  if (p.on) {
+  const int64_t left = A.rows - p.t0;
+  const int rows = left < A.tile_rows ? (int)left : A.tile_rows;
+  join_chain<V, true>(A, S, position, cblk,
+                      rows <= 0              ? kOutside
+                      : A.offsets != nullptr ? info[rows - 1]
+                                             : even_info(A, p.t0 + rows - 1));
+  empty_sequences(A, tile, c0, c1, A.dfinal, A.dinitial);
+  if (p.rows > 0) {
     float after[V];
-    enter_segment<V, R>(A, p, S, carry, after);
+    enter_segment<V, true>(A, p, S, after);
+    const int64_t last = p.row + along(A, p.rows - 1);
+    XT *to = reinterpret_cast<XT *>(A.dx) + last * A.channels + p.c;
+    GT *gate = reinterpret_cast<GT *>(A.dgate) + last * A.gates + p.c;
+    const int64_t ts = along(A, A.channels), gs = along(A, A.gates);
 #pragma unroll
     for (int i = R - 1; i >= 0; --i) {
       if (i >= p.rows) continue;
-      const int in = S.info[p.sg * R + i];
-      const int64_t row = row_of<R>(A, p, i);
+      const int row = p.plain ? 0 : in[i];
       float u[V], dg[V], sum = 0.f;
-      if (in < 0) {
+      if (row < 0) {
 #pragma unroll
         for (int v = 0; v < V; ++v) u[v] = dg[v] = after[v] = 0.f;
       } else {
-        if (in & 2) load_state<V>(A.dfinal, A, in >> 2, p.c, after);
+        if (row & 2) load_state<V>(A.dfinal, A, row >> 2, p.c, after);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           u[v] = to_f32<XT>(dh[i].e[v]) + after[v];
@@ -101,17 +119,22 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const Args A) {
           after[v] = g[i](v) * u[v];
           sum += dg[v];
         }
-        if ((in & 1) && A.dinitial != nullptr) store_state<V>(A.dinitial, A, in >> 2, p.c, after);
+        if ((row & 1) && A.dinitial != nullptr) store_state<V>(A.dinitial, A, row >> 2, p.c, after);
       }
-      store_pack<XT, V>(reinterpret_cast<XT *>(A.dx) + row * A.channels + p.c, u);
-      if (SHARED) sums[(p.sg * R + i) * A.tx + p.tx] = sum;
-      else store_pack<GT, V>(reinterpret_cast<GT *>(A.dgate) + row * A.gates + p.c, dg);
+      store_pack<XT, V>(to, u);
+      to -= ts;
+      if (SHARED) {
+        sums[(p.sg * R + i) * A.tx + p.tx] = sum;
+      } else {
+        store_pack<GT, V>(gate, dg);
+        gate -= gs;
+      }
     }
   }
   if (!SHARED) return;
   // The sums of the threads that share a gate, in their order.
   __syncthreads();
-  const int c0 = cblk * A.tx * V, first = c0 / A.per_gate, count = (c1 - 1) / A.per_gate - first + 1;
+  const int first = c0 / A.per_gate, count = (c1 - 1) / A.per_gate - first + 1;
   for (int k = threadIdx.x; k < rows * count; k += kThreads) {
     const int i = k / count, gate = first + k % count;
     const int lo = gate * A.per_gate > c0 ? gate * A.per_gate : c0;
@@ -122,7 +145,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const Args A) {
     if (A.partial == nullptr) {
       reinterpret_cast<GT *>(A.dgate)[row * A.gates + gate] = from_f32<GT>(sum);
     } else {
-      const int slot = cblk - gate * A.per_gate / (A.tx * V);
+      const int slot = cblk - gate * A.per_gate / width;
       A.partial[((int64_t)slot * A.rows + row) * A.gates + gate] = sum;
     }
   }
@@ -143,8 +166,7 @@ __global__ void __launch_bounds__(kThreads) join_gates_kernel(const Args A, int 
 
 template <typename XT, typename GT, int V, int R, bool SHARED>
 static void launch_backward(const Args &A, cudaStream_t st) {
-  const unsigned grid = (unsigned)(A.tiles * A.channel_blocks);
-  backward_kernel<XT, GT, V, R, SHARED><<<grid, kThreads, 0, st>>>(A);
+  backward_kernel<XT, GT, V, R, SHARED><<<(unsigned)(A.tiles * A.channel_blocks), kThreads, 0, st>>>(A);
   count_launch();
   if (A.partial != nullptr && A.rows > 0) {
     const int64_t want = (A.rows * A.gates + kThreads - 1) / kThreads;
@@ -158,10 +180,10 @@ static void pick_backward(const Args &A, int vec, cudaStream_t st) {
   constexpr int kPer = 16 / (int)(sizeof(XT) > sizeof(GT) ? sizeof(XT) : sizeof(GT));
   constexpr int kShared = 16 / (int)sizeof(XT);
   const bool shared = A.per_gate > 1;
-  if (vec == 1 && shared) launch_backward<XT, GT, 1, kRowsScalar, true>(A, st);
-  else if (vec == 1) launch_backward<XT, GT, 1, kRowsScalar, false>(A, st);
-  else if (shared) launch_backward<XT, GT, kShared, kRowsVector, true>(A, st);
-  else launch_backward<XT, GT, kPer, kRowsVector, false>(A, st);
+  if (vec == 1 && shared) launch_backward<XT, GT, 1, segment_rows(1, true), true>(A, st);
+  else if (vec == 1) launch_backward<XT, GT, 1, segment_rows(1, true), false>(A, st);
+  else if (shared) launch_backward<XT, GT, kShared, segment_rows(kShared, true), true>(A, st);
+  else launch_backward<XT, GT, kPer, segment_rows(kPer, true), false>(A, st);
 }
 
 }  // namespace scan
@@ -195,7 +217,7 @@ extern "C" int gs_gated_scan_backward(int64_t rows, int sequences, int channels,
         (uintptr_t)saved) & 3))
     return GS_ERR_INVALID_ARGUMENT;
   Args A{};
-  fill_plan(A, p);
+  fill_plan(A, p, true);
   A.rows = rows;
   A.sequences = sequences;
   A.channels = channels;
@@ -216,21 +238,19 @@ extern "C" int gs_gated_scan_backward(int64_t rows, int sequences, int channels,
   A.dgate = grad_gate;
   A.dinitial = grad_initial;
   A.saved = const_cast<float *>(saved);
-  if (p.tiles > 1 || p.slots > 1) {
+  if (p.back_tiles > 1 || p.slots > 1) {
     if (scratch == nullptr || ((uintptr_t)scratch & 15)) return GS_ERR_INVALID_ARGUMENT;
     if (scratch_bytes < gs_gated_scan_scratch_bytes(rows, channels, gates, x_type, gate_type, 1))
       return GS_ERR_CAPACITY;
   }
   if (p.slots > 1)
-    A.partial = reinterpret_cast<float *>(static_cast<char *>(scratch) + chain_bytes(p, channels));
+    A.partial = reinterpret_cast<float *>(static_cast<char *>(scratch) + chain_bytes(p.back_tiles, channels));
   A.status = device_status_word();
   if (A.status == nullptr) return GS_ERR_CUDA;
   const bool same = x_type == gate_type;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (p.tiles > 1) {
-    const int failed = place_chain(A, p, scratch, st);
-    if (failed) return failed;
-  }
+  const int failed = place_chain(A, scratch, st);
+  if (failed) return failed;
   if (x_type == GS_TYPE_F32) pick_backward<float, float>(A, p.vec, st);
   else if (x_type == GS_TYPE_BF16 && same) pick_backward<__nv_bfloat16, __nv_bfloat16>(A, p.vec, st);
   else if (x_type == GS_TYPE_BF16) pick_backward<__nv_bfloat16, float>(A, p.vec, st);

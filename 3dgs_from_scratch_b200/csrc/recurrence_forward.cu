@@ -15,7 +15,6 @@ Plan make_plan(int64_t rows, int channels, int gates, int x_type, int gate_type)
   const bool shared = per > 1;
   const int wide = 16 / (shared ? xb : xb > gb ? xb : gb);
   p.vec = (shared ? per : channels) % wide == 0 ? wide : 1;
-  const int r = p.vec == 1 ? kRowsScalar : kRowsVector;
   const int vectors = channels / p.vec, most = p.vec == 1 ? 64 : 8;
   int tx = vectors < most ? vectors : most;
   if (shared && per / p.vec <= most) {  // whole gates in a block, where they fit
@@ -26,8 +25,10 @@ Plan make_plan(int64_t rows, int channels, int gates, int x_type, int gate_type)
   p.tx = tx;
   p.channel_blocks = (vectors + tx - 1) / tx;
   p.seg = kThreads / tx;
-  p.tile_rows = p.seg * r;
+  p.tile_rows = p.seg * segment_rows(p.vec, false);
+  p.back_rows = p.seg * segment_rows(p.vec, true);
   p.tiles = rows > 0 ? (rows + p.tile_rows - 1) / p.tile_rows : 1;
+  p.back_tiles = rows > 0 ? (rows + p.back_rows - 1) / p.back_rows : 1;
   // Blocks that hold a part of one gate's channels (1: none is split).
   const int width = tx * p.vec;
   p.slots = 1;
@@ -35,69 +36,85 @@ Plan make_plan(int64_t rows, int channels, int gates, int x_type, int gate_type)
   return p;
 }
 
-// Reads a thread's rows, all loads in flight before the first use.
 template <typename XT, typename GT, int V, int R, bool SHARED>
-__device__ __forceinline__ void load_rows(const Args &A, const Place &p, Pack<XT, V> (&x)[R],
-                                          Gates<GT, V, SHARED> (&g)[R]) {
-#pragma unroll
-  for (int i = 0; i < R; ++i)
-    if (i < p.rows) {
-      const int64_t row = row_of<R>(A, p, i);
-      x[i] = load_pack<XT, V>(reinterpret_cast<const XT *>(A.x) + row * A.x_stride + p.c);
-      g[i].load(A, row, p.g);
-    }
-}
-
-template <typename XT, typename GT, int V, int R, bool SHARED>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const Args A) {
-  __shared__ Tile<V, R> S;
-  __shared__ float carry[kThreads];
-  __shared__ float2 parts[kThreads];
+__global__ void __launch_bounds__(kThreads, kResident) forward_kernel(const __grid_constant__ Args A) {
+  __shared__ Tile<V> S;
+  __shared__ int info[kThreads * R];
   int64_t tile;
   int cblk;
   take_tile(A, tile, cblk);
-  const Place p = place_of<V, R, SHARED>(A, tile, cblk);
+  Place p = place_of<V, R, SHARED>(A, tile, cblk);
   Pack<XT, V> x[R];
   Gates<GT, V, SHARED> g[R];
-  load_rows<XT, GT, V, R, SHARED>(A, p, x, g);
-  tile_info(A, tile, S.info);
-  float P[V], L[V];
-  reduce_segment<XT, GT, V, R, SHARED>(A, p, S.info, x, g, P, L);
-  put_segment<V, R>(A, p, S, segment_cut<R>(p, S.info, 1), P, L);
-  __syncthreads();
-  float tp, tl;
-  const bool cut = fold_segments<V, R, false>(A, S, tp, tl);
-  join_chain<false>(A, tile, cblk, A.tx * V, S.info[0], cut, tp, tl, carry, parts);
-  const int c1 = (cblk + 1) * A.tx * V < A.channels ? (cblk + 1) * A.tx * V : A.channels;
-  empty_sequences(A, tile, cblk * A.tx * V, c1, A.initial, A.final_state);
-  if (!p.on) return;
-  float h[V];
-  enter_segment<V, R>(A, p, S, carry, h);
-  if (A.saved != nullptr && p.sg == 0) {
+  {  // all loads in flight before the first use
+    const XT *from = reinterpret_cast<const XT *>(A.x) + p.row * A.x_stride + p.c;
+    const GT *gate = reinterpret_cast<const GT *>(A.gate) + p.row * A.gate_stride + p.g;
+    const int64_t xs = along(A, A.x_stride), gs = along(A, A.gate_stride);
 #pragma unroll
-    for (int v = 0; v < V; ++v) A.saved[tile * A.channels + p.c + v] = h[v];
+    for (int i = 0; i < R; ++i)
+      if (i < p.rows) {
+        x[i] = load_pack<XT, V>(from);
+        g[i].load(gate);
+        from += xs;
+        gate += gs;
+      }
+  }
+  if (A.offsets != nullptr) tile_info(A, tile, info);
+  int in[R];
+  segment_info<R>(A, p, info, in);
+  {
+    float P[V], L[V];
+    reduce_segment<XT, GT, V, R, SHARED>(A, p, in, x, g, P, L);
+    put_segment<V>(A, p, S, segment_cut<R>(p, in, 1), P, L);
+  }
+  __syncthreads();
+  fold_runs<V, false>(A, S);
+  __syncthreads();
+  const int width = A.tx * V, c0 = cblk * width;
+  join_chain<V, false>(A, S, tile, cblk,
+                       A.offsets != nullptr ? info[0] : A.rows > 0 ? even_info(A, p.t0) : kOutside);
+  empty_sequences(A, tile, c0, c0 + width < A.channels ? c0 + width : A.channels, A.initial, A.final_state);
+  if (p.rows == 0) return;
+  float h[V];
+  enter_segment<V, false>(A, p, S, h);
+  XT *to = reinterpret_cast<XT *>(A.h) + p.row * A.channels + p.c;
+  const int64_t hs = along(A, A.channels);
+  // The backward's tiles begin in the middle of these, too.
+  const int at = p.sg * R, halves = A.tile_rows / A.saved_rows;
+  if (A.saved != nullptr && at == 0) store_state<V>(A.saved, A, tile * halves, p.c, h);
+  const bool middle = A.saved != nullptr && at <= A.saved_rows && A.saved_rows < at + R;
+  if (p.plain && !middle) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[v] = fmaf(g[i](v), h[v], to_f32<XT>(x[i].e[v]));
+      store_pack<XT, V>(to, h);
+      to += hs;
+    }
+    return;
   }
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     if (i >= p.rows) break;
-    const int in = S.info[p.sg * R + i];
-    if (in < 0) {
+    if (middle && at + i == A.saved_rows) store_state<V>(A.saved, A, tile * halves + 1, p.c, h);
+    const int row = p.plain ? 0 : in[i];
+    if (row < 0) {
 #pragma unroll
       for (int v = 0; v < V; ++v) h[v] = 0.f;
     } else {
-      if (in & 1) load_state<V>(A.initial, A, in >> 2, p.c, h);
+      if (row & 1) load_state<V>(A.initial, A, row >> 2, p.c, h);
 #pragma unroll
       for (int v = 0; v < V; ++v) h[v] = fmaf(g[i](v), h[v], to_f32<XT>(x[i].e[v]));
-      if ((in & 2) && A.final_state != nullptr) store_state<V>(A.final_state, A, in >> 2, p.c, h);
+      if ((row & 2) && A.final_state != nullptr) store_state<V>(A.final_state, A, row >> 2, p.c, h);
     }
-    store_pack<XT, V>(reinterpret_cast<XT *>(A.h) + row_of<R>(A, p, i) * A.channels + p.c, h);
+    store_pack<XT, V>(to, h);
+    to += hs;
   }
 }
 
 template <typename XT, typename GT, int V, int R, bool SHARED>
 static void launch_forward(const Args &A, cudaStream_t st) {
-  const unsigned grid = (unsigned)(A.tiles * A.channel_blocks);
-  forward_kernel<XT, GT, V, R, SHARED><<<grid, kThreads, 0, st>>>(A);
+  forward_kernel<XT, GT, V, R, SHARED><<<(unsigned)(A.tiles * A.channel_blocks), kThreads, 0, st>>>(A);
   count_launch();
 }
 
@@ -106,10 +123,10 @@ static void pick_forward(const Args &A, int vec, cudaStream_t st) {
   constexpr int kPer = 16 / (int)(sizeof(XT) > sizeof(GT) ? sizeof(XT) : sizeof(GT));
   constexpr int kShared = 16 / (int)sizeof(XT);
   const bool shared = A.per_gate > 1;
-  if (vec == 1 && shared) launch_forward<XT, GT, 1, kRowsScalar, true>(A, st);
-  else if (vec == 1) launch_forward<XT, GT, 1, kRowsScalar, false>(A, st);
-  else if (shared) launch_forward<XT, GT, kShared, kRowsVector, true>(A, st);
-  else launch_forward<XT, GT, kPer, kRowsVector, false>(A, st);
+  if (vec == 1 && shared) launch_forward<XT, GT, 1, segment_rows(1, false), true>(A, st);
+  else if (vec == 1) launch_forward<XT, GT, 1, segment_rows(1, false), false>(A, st);
+  else if (shared) launch_forward<XT, GT, kShared, segment_rows(kShared, false), true>(A, st);
+  else launch_forward<XT, GT, kPer, segment_rows(kPer, false), false>(A, st);
 }
 
 void run_forward(const Args &A, const Plan &p, int x_type, int gate_type, cudaStream_t st) {
@@ -135,7 +152,7 @@ int gs::scan::check_shape(int64_t rows, int sequences, int channels, int gates, 
     return GS_ERR_INVALID_ARGUMENT;
   if (offsets == nullptr && rows % sequences != 0) return GS_ERR_INVALID_ARGUMENT;
   const Plan p = make_plan(rows, channels, gates, x_type, gate_type);
-  if (p.tiles * p.channel_blocks > INT32_MAX) return GS_ERR_CAPACITY;
+  if (p.back_tiles * p.channel_blocks > INT32_MAX / 2) return GS_ERR_CAPACITY;
   return GS_OK;
 }
 
@@ -145,12 +162,13 @@ bool gs::scan::suits(const void *p, int64_t stride, int bytes, int vec) {
   return ((uintptr_t)p % align) == 0 && (stride * bytes) % align == 0;
 }
 
-void gs::scan::fill_plan(Args &A, const Plan &p) {
+void gs::scan::fill_plan(Args &A, const Plan &p, bool back) {
   A.tx = p.tx;
   A.seg = p.seg;
-  A.tile_rows = p.tile_rows;
+  A.tile_rows = back ? p.back_rows : p.tile_rows;
+  A.saved_rows = p.back_rows;
   A.channel_blocks = p.channel_blocks;
-  A.tiles = p.tiles;
+  A.tiles = back ? p.back_tiles : p.tiles;
   A.slots = p.slots;
 }
 
@@ -159,14 +177,14 @@ using namespace gs::scan;
 extern "C" size_t gs_gated_scan_saved_bytes(int64_t rows, int channels, int gates, int x_type,
                                             int gate_type) {
   if (check_shape(rows, 1, channels, gates, x_type, gate_type, nullptr)) return 0;
-  return (size_t)make_plan(rows, channels, gates, x_type, gate_type).tiles * channels * 4;
+  return (size_t)make_plan(rows, channels, gates, x_type, gate_type).back_tiles * channels * 4;
 }
 
 extern "C" size_t gs_gated_scan_scratch_bytes(int64_t rows, int channels, int gates, int x_type,
                                               int gate_type, int backward) {
   if (check_shape(rows, 1, channels, gates, x_type, gate_type, nullptr)) return 0;
   const Plan p = make_plan(rows, channels, gates, x_type, gate_type);
-  size_t bytes = chain_bytes(p, channels);
+  size_t bytes = chain_bytes(backward ? p.back_tiles : p.tiles, channels);
   if (backward && p.slots > 1) bytes += (size_t)p.slots * rows * gates * 4;
   return bytes;
 }
@@ -188,7 +206,7 @@ extern "C" int gs_gated_scan_forward(int64_t rows, int sequences, int channels, 
       (((uintptr_t)initial | (uintptr_t)final_state | (uintptr_t)offsets | (uintptr_t)saved) & 3))
     return GS_ERR_INVALID_ARGUMENT;
   Args A{};
-  fill_plan(A, p);
+  fill_plan(A, p, false);
   A.rows = rows;
   A.sequences = sequences;
   A.channels = channels;
@@ -207,15 +225,13 @@ extern "C" int gs_gated_scan_forward(int64_t rows, int sequences, int channels, 
   A.saved = saved;
   if (p.tiles > 1) {
     if (scratch == nullptr || ((uintptr_t)scratch & 15)) return GS_ERR_INVALID_ARGUMENT;
-    if (scratch_bytes < chain_bytes(p, channels)) return GS_ERR_CAPACITY;
+    if (scratch_bytes < chain_bytes(p.tiles, channels)) return GS_ERR_CAPACITY;
   }
   A.status = device_status_word();
   if (A.status == nullptr) return GS_ERR_CUDA;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (p.tiles > 1) {
-    const int failed = place_chain(A, p, scratch, st);
-    if (failed) return failed;
-  }
+  const int failed = place_chain(A, scratch, st);
+  if (failed) return failed;
   run_forward(A, p, x_type, gate_type, st);
   return launch_status();
 }
