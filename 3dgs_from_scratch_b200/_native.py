@@ -91,8 +91,8 @@ SIGNATURES = {
     "gs_ssim_forward": (I, [I, I, I, P, P, I, P, SZ, P, P]),
     "gs_ssim_backward": (I, [I, I, I, P, P, P, P, P, P]),
     "gs_l1_ssim_loss_grad": (I, [I, I, P, P, I, F, P, P, P, SZ, P]),
-    "gs_gated_scan_saved_bytes": (SZ, [I64, I, I, I, I]),
-    "gs_gated_scan_scratch_bytes": (SZ, [I64, I, I, I, I, I]),
+    "gs_gated_scan_saved_bytes": (SZ, [I64, I, I, I, I, I, I]),
+    "gs_gated_scan_scratch_bytes": (SZ, [I64, I, I, I, I, I, I, I]),
     "gs_gated_scan_forward": (I, [I64, I, I, I, I, I, P, I64, P, I64, P, P, I, P, P, P, P, SZ, P]),
     "gs_gated_scan_backward": (I, [I64, I, I, I, I, I, P, I64, P, I64, P, P, I, P, P, I64, P, P, P,
                                    P, P, SZ, P]),

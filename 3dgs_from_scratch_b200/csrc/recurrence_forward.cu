@@ -1,5 +1,5 @@
 // recurrence_forward.cu -- h_t = g_t h_{t-1} + x_t over packed sequences (see
-// recurrence.cuh for the tiles).
+// recurrence.cuh).
 #include "recurrence.cuh"
 
 namespace gs {
@@ -9,182 +9,248 @@ int type_bytes(int type) {
   return type == GS_TYPE_F32 ? 4 : type == GS_TYPE_BF16 || type == GS_TYPE_F16 ? 2 : 0;
 }
 
-Plan make_plan(int64_t rows, int channels, int gates, int x_type, int gate_type) {
+Plan make_plan(int64_t rows, int sequences, bool even, int channels, int gates, int x_type, int gate_type) {
   Plan p;
   const int xb = type_bytes(x_type), gb = type_bytes(gate_type), per = channels / gates;
   const bool shared = per > 1;
-  const int wide = 16 / (shared ? xb : xb > gb ? xb : gb);
+  // 8 bytes of the wider type a row and thread: 16 leave too few threads, and
+  // the backward short of registers.
+  const int wide = 8 / (shared ? xb : xb > gb ? xb : gb);
   p.vec = (shared ? per : channels) % wide == 0 ? wide : 1;
-  const int vectors = channels / p.vec, most = p.vec == 1 ? 64 : 8;
-  int tx = vectors < most ? vectors : most;
-  if (shared && per / p.vec <= most) {  // whole gates in a block, where they fit
-    const int one = per / p.vec;
-    tx = most / one * one;
-    if (tx > vectors) tx = vectors;
+  const int vectors = channels / p.vec, one = shared ? per / p.vec : 1;  // vectors of a gate
+  p.channel_blocks = (vectors + kThreads - 1) / kThreads;
+  p.tx = (vectors + p.channel_blocks - 1) / p.channel_blocks;
+  if (one <= kThreads) {  // whole gates in a block, where they fit
+    p.tx = (p.tx + one - 1) / one * one;
+    if (p.tx > kThreads) p.tx = kThreads / one * one;
+    p.channel_blocks = (vectors + p.tx - 1) / p.tx;
   }
-  p.tx = tx;
-  p.channel_blocks = (vectors + tx - 1) / tx;
-  p.seg = kThreads / tx;
-  p.tile_rows = p.seg * segment_rows(p.vec, false);
-  p.back_rows = p.seg * segment_rows(p.vec, true);
-  p.tiles = rows > 0 ? (rows + p.tile_rows - 1) / p.tile_rows : 1;
-  p.back_tiles = rows > 0 ? (rows + p.back_rows - 1) / p.back_rows : 1;
-  // Blocks that hold a part of one gate's channels (1: none is split).
-  const int width = tx * p.vec;
-  p.slots = 1;
-  if (shared && width % per != 0) p.slots = (per + width - 2) / width + 1;
+  p.cy = kThreads / p.tx;
+  // Rows of a chunk: about kFill threads on each of 148 SMs.
+  const int64_t want = rows * vectors / (148 * kFill);
+  const int64_t period = even ? rows / sequences : 0;
+  p.whole = even && period > 0 && (period <= 32 || (int64_t)sequences * vectors >= 148 * 256);
+  if (p.whole) {
+    const int64_t k = want / period;
+    p.chunk = (int)(period * (k < 1 ? 1 : k > 64 ? 64 : k));
+  } else {
+    int64_t chunk = 32;
+    while (chunk < want && chunk < 512) chunk *= 2;
+    p.chunk = (int)chunk;
+    if (rows <= p.chunk) p.whole = true;
+  }
+  p.chunks = rows > 0 ? (rows + p.chunk - 1) / p.chunk : 0;
+  p.kept = (p.chunk + kBatch - 1) / kBatch;
+  const int width = p.tx * p.vec;
+  p.slots = shared && width % per != 0 ? (per + width - 2) / width + 1 : 1;
   return p;
 }
 
-template <typename XT, typename GT, int V, int R, bool SHARED>
-__global__ void __launch_bounds__(kThreads, kResident) forward_kernel(const __grid_constant__ Args A) {
-  __shared__ Tile<V> S;
-  __shared__ int info[kThreads * R];
-  int64_t tile;
-  int cblk;
-  take_tile(A, tile, cblk);
-  Place p = place_of<V, R, SHARED>(A, tile, cblk);
-  Pack<XT, V> x[R];
-  Gates<GT, V, SHARED> g[R];
-  {  // all loads in flight before the first use
-    const XT *from = reinterpret_cast<const XT *>(A.x) + p.row * A.x_stride + p.c;
-    const GT *gate = reinterpret_cast<const GT *>(A.gate) + p.row * A.gate_stride + p.g;
-    const int64_t xs = along(A, A.x_stride), gs = along(A, A.gate_stride);
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-      if (i < p.rows) {
-        x[i] = load_pack<XT, V>(from);
-        g[i].load(gate);
-        from += xs;
-        gate += gs;
-      }
-  }
-  if (A.offsets != nullptr) tile_info(A, tile, info);
-  int in[R];
-  segment_info<R>(A, p, info, in);
-  {
-    float P[V], L[V];
-    reduce_segment<XT, GT, V, R, SHARED>(A, p, in, x, g, P, L);
-    put_segment<V>(A, p, S, segment_cut<R>(p, in, 1), P, L);
-  }
-  __syncthreads();
-  fold_runs<V, false>(A, S);
-  __syncthreads();
-  const int width = A.tx * V, c0 = cblk * width;
-  join_chain<V, false>(A, S, tile, cblk,
-                       A.offsets != nullptr ? info[0] : A.rows > 0 ? even_info(A, p.t0) : kOutside);
-  empty_sequences(A, tile, c0, c0 + width < A.channels ? c0 + width : A.channels, A.initial, A.final_state);
-  if (p.rows == 0) return;
-  float h[V];
-  enter_segment<V, false>(A, p, S, h);
-  XT *to = reinterpret_cast<XT *>(A.h) + p.row * A.channels + p.c;
-  const int64_t hs = along(A, A.channels);
-  // The backward's tiles begin in the middle of these, too.
-  const int at = p.sg * R, halves = A.tile_rows / A.saved_rows;
-  if (A.saved != nullptr && at == 0) store_state<V>(A.saved, A, tile * halves, p.c, h);
-  const bool middle = A.saved != nullptr && at <= A.saved_rows && A.saved_rows < at + R;
-  if (p.plain && !middle) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = fmaf(g[i](v), h[v], to_f32<XT>(x[i].e[v]));
-      store_pack<XT, V>(to, h);
-      to += hs;
-    }
+// A warp for each sequence, then a thread for each end of a chunk.
+__global__ void __launch_bounds__(kThreads) setup_kernel(const __grid_constant__ Args A,
+                                                         const float *__restrict__ src,
+                                                         float *__restrict__ dst) {
+  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t s = at / 32;
+  if (s < A.sequences) {
+    const int64_t a = A.offsets != nullptr ? A.offsets[s] : s * A.period;
+    const int64_t b = A.offsets != nullptr ? A.offsets[s + 1] : (s + 1) * A.period;
+    if (a == b && dst != nullptr)
+      for (int c = (int)lane_id(); c < A.channels; c += 32)
+        dst[s * A.channels + c] = src != nullptr ? src[s * A.channels + c] : 0.f;
+    if ((a < 0 || a > b || b > A.rows) && lane_id() == 0)
+      atomicCAS(A.status, 0u, (uint32_t)GS_ERR_INVALID_ARGUMENT);
     return;
   }
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    if (i >= p.rows) break;
-    if (middle && at + i == A.saved_rows) store_state<V>(A.saved, A, tile * halves + 1, p.c, h);
-    const int row = p.plain ? 0 : in[i];
-    if (row < 0) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = 0.f;
-    } else {
-      if (row & 1) load_state<V>(A.initial, A, row >> 2, p.c, h);
-#pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = fmaf(g[i](v), h[v], to_f32<XT>(x[i].e[v]));
-      if ((row & 2) && A.final_state != nullptr) store_state<V>(A.final_state, A, row >> 2, p.c, h);
-    }
-    store_pack<XT, V>(to, h);
-    to += hs;
+  const int64_t k = at - (int64_t)A.sequences * 32;
+  if (A.offsets == nullptr || k >= 2 * A.plan.chunks) return;
+  int64_t t = k * A.plan.chunk;  // the first row of chunk k, then the last one of k - chunks
+  if (k >= A.plan.chunks) t = (k - A.plan.chunks + 1) * A.plan.chunk - 1;
+  const int64_t p = row_at(A, t < A.rows ? t : A.rows - 1);
+  int lo = 0, hi = A.sequences - 1;  // the first sequence that ends behind p, or the last
+  while (lo < hi) {
+    const int mid = lo + (hi - lo) / 2;
+    if ((int64_t)A.offsets[mid + 1] <= p) lo = mid + 1;
+    else hi = mid;
+  }
+  A.hints[k] = lo;
+}
+
+int launch_setup(const Args &A, const float *src, float *dst, cudaStream_t st) {
+  if (A.offsets == nullptr && A.rows > 0) return GS_OK;  // even sequences, none empty
+  const int64_t threads = (int64_t)A.sequences * 32 + (A.offsets != nullptr ? 2 * A.plan.chunks : 0);
+  setup_kernel<<<(unsigned)((threads + kThreads - 1) / kThreads), kThreads, 0, st>>>(A, src, dst);
+  count_launch();
+  return launch_status();
+}
+
+// The state that enters each chunk, from the chunks' maps: 32 channels a block,
+// its 32 warps a run of chunks each, then the runs' maps in order, then the run
+// once more from the state before it.
+template <bool BACK>
+__global__ void __launch_bounds__(1024) carry_kernel(const __grid_constant__ Args A) {
+  __shared__ float2 runs[32][33];
+  __shared__ int run_cut[32];
+  const int c = blockIdx.x * 32 + (int)lane_id(), run = threadIdx.x / 32;
+  const bool on = c < A.channels;
+  const int64_t n = A.plan.chunks, k0 = n * run / 32, k1 = n * (run + 1) / 32;
+  const auto chunk_of = [&](int64_t k) { return BACK ? n - 1 - k : k; };
+  float P = 1.f, L = 0.f;
+  bool cut = false;
+#pragma unroll 8
+  for (int64_t k = k0; k < k1; ++k) {
+    const int64_t at = chunk_of(k);
+    const float2 m = on ? A.maps[at * A.channels + c] : make_float2(1.f, 0.f);
+    const bool here = A.cuts[at] != 0;
+    L = here ? m.y : fmaf(m.x, L, m.y);
+    P *= m.x;
+    cut = cut || here;
+  }
+  runs[run][lane_id()] = make_float2(P, L);
+  if (lane_id() == 0) run_cut[run] = cut;
+  __syncthreads();
+  float h = 0.f;
+  for (int q = 0; q < run; ++q) {
+    const float2 m = runs[q][lane_id()];
+    h = run_cut[q] ? m.y : fmaf(m.x, h, m.y);
+  }
+  if (!on) return;
+#pragma unroll 8
+  for (int64_t k = k0; k < k1; ++k) {
+    const int64_t at = chunk_of(k);
+    A.carry[at * A.channels + c] = h;
+    const float2 m = A.maps[at * A.channels + c];
+    h = A.cuts[at] != 0 ? m.y : fmaf(m.x, h, m.y);
   }
 }
 
-template <typename XT, typename GT, int V, int R, bool SHARED>
-static void launch_forward(const Args &A, cudaStream_t st) {
-  forward_kernel<XT, GT, V, R, SHARED><<<(unsigned)(A.tiles * A.channel_blocks), kThreads, 0, st>>>(A);
+int launch_carry(const Args &A, bool back, cudaStream_t st) {
+  const unsigned grid = (unsigned)((A.channels + 31) / 32);
+  if (back) carry_kernel<true><<<grid, 1024, 0, st>>>(A);
+  else carry_kernel<false><<<grid, 1024, 0, st>>>(A);
   count_launch();
+  return launch_status();
+}
+
+template <typename XT, typename GT, int V, bool SHARED>
+__global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant__ Args A) {
+  const Place p =
+      place_of<V, SHARED>(A, blockIdx.x / A.plan.channel_blocks, blockIdx.x % A.plan.channel_blocks);
+  if (!p.on) return;
+  int64_t row = row_at(A, p.t0);
+  const int64_t xs = along(A, A.x_stride), gs = along(A, A.gate_stride), hs = along(A, A.channels);
+  const XT *from = reinterpret_cast<const XT *>(A.x) + row * A.x_stride + p.c;
+  const GT *gate = reinterpret_cast<const GT *>(A.gate) + row * A.gate_stride + p.g;
+  XT *to = reinterpret_cast<XT *>(A.h) + row * A.channels + p.c;
+  Cursor q;
+  q.s = A.hints != nullptr ? A.hints[p.chunk] : 0;
+  q.seek(A, row);
+  float h[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) h[v] = 0.f;
+  if (A.carry != nullptr) load_kept<V>(A.carry, A, p.chunk, p.c, h);
+  int64_t kept = p.chunk * A.plan.kept;
+  for (int left = (int)(p.t1 - p.t0); left > 0; left -= kBatch) {
+    Pack<XT, V> x[kBatch];
+    Gates<GT, V, SHARED> g[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (k < left) {
+        x[k] = load_pack<XT, V>(from + k * xs);
+        g[k].load(gate + k * gs);
+      }
+    if (A.saved != nullptr) store_kept<V>(A.saved, A, kept++, p.c, h);
+    if (left >= kBatch && plain_rows(q, A.reverse ? row - (kBatch - 1) : row, kBatch)) {
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = fmaf(g[k](v), h[v], to_f32<XT>(x[k].e[v]));
+        store_pack<XT, V>(to + k * hs, h);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if (k >= left) break;
+        const int64_t at = A.reverse ? row - k : row + k;
+        if (!q.holds(at)) q.seek(A, at);
+        if (!q.holds(at)) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) h[v] = 0.f;
+        } else {
+          if (at == (A.reverse ? q.hi - 1 : q.lo)) load_state<V>(A.initial, A, q.s, p.c, h);
+#pragma unroll
+          for (int v = 0; v < V; ++v) h[v] = fmaf(g[k](v), h[v], to_f32<XT>(x[k].e[v]));
+          if (at == (A.reverse ? q.lo : q.hi - 1) && A.final_state != nullptr)
+            store_state<V>(A.final_state, A, q.s, p.c, h);
+        }
+        store_pack<XT, V>(to + k * hs, h);
+      }
+    }
+    row += A.reverse ? -kBatch : kBatch;
+    from += kBatch * xs;
+    gate += kBatch * gs;
+    to += kBatch * hs;
+  }
+}
+
+template <typename XT, typename GT, int V, bool SHARED>
+static int launch_forward(const Args &A, cudaStream_t st) {
+  if (A.carry != nullptr) {
+    maps_kernel<XT, GT, V, SHARED, false><<<grid_of(A.plan), kThreads, 0, st>>>(A);
+    count_launch();
+    const int rc = launch_carry(A, false, st);
+    if (rc) return rc;
+  }
+  forward_kernel<XT, GT, V, SHARED><<<grid_of(A.plan), kThreads, 0, st>>>(A);
+  count_launch();
+  return launch_status();
 }
 
 template <typename XT, typename GT>
-static void pick_forward(const Args &A, int vec, cudaStream_t st) {
-  constexpr int kPer = 16 / (int)(sizeof(XT) > sizeof(GT) ? sizeof(XT) : sizeof(GT));
-  constexpr int kShared = 16 / (int)sizeof(XT);
+static int pick_forward(const Args &A, cudaStream_t st) {
+  constexpr int kPer = 8 / (int)(sizeof(XT) > sizeof(GT) ? sizeof(XT) : sizeof(GT));
+  constexpr int kShared = 8 / (int)sizeof(XT);
   const bool shared = A.per_gate > 1;
-  if (vec == 1 && shared) launch_forward<XT, GT, 1, segment_rows(1, false), true>(A, st);
-  else if (vec == 1) launch_forward<XT, GT, 1, segment_rows(1, false), false>(A, st);
-  else if (shared) launch_forward<XT, GT, kShared, segment_rows(kShared, false), true>(A, st);
-  else launch_forward<XT, GT, kPer, segment_rows(kPer, false), false>(A, st);
+  if (A.plan.vec == 1) return shared ? launch_forward<XT, GT, 1, true>(A, st) : launch_forward<XT, GT, 1, false>(A, st);
+  return shared ? launch_forward<XT, GT, kShared, true>(A, st) : launch_forward<XT, GT, kPer, false>(A, st);
 }
 
-void run_forward(const Args &A, const Plan &p, int x_type, int gate_type, cudaStream_t st) {
-  const bool same = x_type == gate_type;
-  if (x_type == GS_TYPE_F32) pick_forward<float, float>(A, p.vec, st);
-  else if (x_type == GS_TYPE_BF16 && same) pick_forward<__nv_bfloat16, __nv_bfloat16>(A, p.vec, st);
-  else if (x_type == GS_TYPE_BF16) pick_forward<__nv_bfloat16, float>(A, p.vec, st);
-  else if (same) pick_forward<__half, __half>(A, p.vec, st);
-  else pick_forward<__half, float>(A, p.vec, st);
+// What both directions check of their sizes and types.
+int check_shape(int64_t rows, int sequences, int channels, int gates, int x_type, int gate_type, int even) {
+  if (rows < 0 || rows > INT32_MAX || sequences < 1 || sequences > (1 << 28) || channels < 1 ||
+      gates < 1 || channels % gates != 0 || !type_bytes(x_type) ||
+      (gate_type != x_type && gate_type != GS_TYPE_F32))
+    return GS_ERR_INVALID_ARGUMENT;
+  if (even && rows % sequences != 0) return GS_ERR_INVALID_ARGUMENT;
+  const Plan p = make_plan(rows, sequences, even, channels, gates, x_type, gate_type);
+  if ((p.chunks / p.cy + 1) * p.channel_blocks > INT32_MAX) return GS_ERR_CAPACITY;
+  return GS_OK;
+}
+
+// Whether a row pointer and stride suit the plan's vectors.
+bool suits(const void *p, int64_t stride, int bytes, int vec) {
+  return ((uintptr_t)p % (bytes * vec)) == 0 && stride % vec == 0;
 }
 
 }  // namespace scan
 }  // namespace gs
 
 using namespace gs;
-
-// What both directions check of their sizes, types and rows.
-int gs::scan::check_shape(int64_t rows, int sequences, int channels, int gates, int x_type,
-                          int gate_type, const int32_t *offsets) {
-  if (rows < 0 || rows > INT32_MAX || sequences < 1 || sequences > (1 << 28) || channels < 1 ||
-      gates < 1 || channels % gates != 0 || !type_bytes(x_type) ||
-      (gate_type != x_type && gate_type != GS_TYPE_F32))
-    return GS_ERR_INVALID_ARGUMENT;
-  if (offsets == nullptr && rows % sequences != 0) return GS_ERR_INVALID_ARGUMENT;
-  const Plan p = make_plan(rows, channels, gates, x_type, gate_type);
-  if (p.back_tiles * p.channel_blocks > INT32_MAX / 2) return GS_ERR_CAPACITY;
-  return GS_OK;
-}
-
-// Whether a row pointer and stride suit the plan's vectors.
-bool gs::scan::suits(const void *p, int64_t stride, int bytes, int vec) {
-  const int64_t align = (int64_t)bytes * vec > 16 ? 16 : (int64_t)bytes * vec;
-  return ((uintptr_t)p % align) == 0 && (stride * bytes) % align == 0;
-}
-
-void gs::scan::fill_plan(Args &A, const Plan &p, bool back) {
-  A.tx = p.tx;
-  A.seg = p.seg;
-  A.tile_rows = back ? p.back_rows : p.tile_rows;
-  A.saved_rows = p.back_rows;
-  A.channel_blocks = p.channel_blocks;
-  A.tiles = back ? p.back_tiles : p.tiles;
-  A.slots = p.slots;
-}
-
 using namespace gs::scan;
 
-extern "C" size_t gs_gated_scan_saved_bytes(int64_t rows, int channels, int gates, int x_type,
-                                            int gate_type) {
-  if (check_shape(rows, 1, channels, gates, x_type, gate_type, nullptr)) return 0;
-  return (size_t)make_plan(rows, channels, gates, x_type, gate_type).back_tiles * channels * 4;
+extern "C" size_t gs_gated_scan_saved_bytes(int64_t rows, int sequences, int even, int channels, int gates,
+                                            int x_type, int gate_type) {
+  if (check_shape(rows, sequences, channels, gates, x_type, gate_type, even)) return 0;
+  const Plan p = make_plan(rows, sequences, even, channels, gates, x_type, gate_type);
+  return (size_t)p.chunks * p.kept * channels * 4;
 }
 
-extern "C" size_t gs_gated_scan_scratch_bytes(int64_t rows, int channels, int gates, int x_type,
-                                              int gate_type, int backward) {
-  if (check_shape(rows, 1, channels, gates, x_type, gate_type, nullptr)) return 0;
-  const Plan p = make_plan(rows, channels, gates, x_type, gate_type);
-  size_t bytes = chain_bytes(backward ? p.back_tiles : p.tiles, channels);
+extern "C" size_t gs_gated_scan_scratch_bytes(int64_t rows, int sequences, int even, int channels, int gates,
+                                              int x_type, int gate_type, int backward) {
+  if (check_shape(rows, sequences, channels, gates, x_type, gate_type, even)) return 0;
+  const Plan p = make_plan(rows, sequences, even, channels, gates, x_type, gate_type);
+  if (even && p.whole && (!backward || p.slots == 1)) return 0;
+  size_t bytes = chain_bytes(p, channels);
   if (backward && p.slots > 1) bytes += (size_t)p.slots * rows * gates * 4;
   return bytes;
 }
@@ -195,24 +261,25 @@ extern "C" int gs_gated_scan_forward(int64_t rows, int sequences, int channels, 
                                      const float *initial, const int32_t *offsets, int reverse,
                                      void *h, float *final_state, float *saved, void *scratch,
                                      size_t scratch_bytes, void *stream) {
-  const int rc = check_shape(rows, sequences, channels, gates, x_type, gate_type, offsets);
+  const int even = offsets == nullptr;
+  int rc = check_shape(rows, sequences, channels, gates, x_type, gate_type, even);
   if (rc) return rc;
   if (rows > 0 && (x == nullptr || gate == nullptr || h == nullptr)) return GS_ERR_INVALID_ARGUMENT;
-  const Plan p = make_plan(rows, channels, gates, x_type, gate_type);
-  const int xb = type_bytes(x_type), gb = type_bytes(gate_type);
-  const bool shared = channels != gates;
-  if (!suits(x, x_row_stride, xb, p.vec) || !suits(h, channels, xb, p.vec) ||
-      !suits(gate, gate_row_stride, gb, shared ? 1 : p.vec) ||
-      (((uintptr_t)initial | (uintptr_t)final_state | (uintptr_t)offsets | (uintptr_t)saved) & 3))
-    return GS_ERR_INVALID_ARGUMENT;
   Args A{};
-  fill_plan(A, p, false);
+  A.plan = make_plan(rows, sequences, even, channels, gates, x_type, gate_type);
+  const int xb = type_bytes(x_type), gb = type_bytes(gate_type), vec = A.plan.vec;
+  const bool shared = channels != gates;
+  if (!suits(x, x_row_stride, xb, vec) || !suits(h, channels, xb, vec) ||
+      !suits(gate, gate_row_stride, gb, shared ? 1 : vec) ||
+      (((uintptr_t)initial | (uintptr_t)final_state | (uintptr_t)offsets) & 3) ||
+      ((uintptr_t)saved & 15))
+    return GS_ERR_INVALID_ARGUMENT;
   A.rows = rows;
   A.sequences = sequences;
   A.channels = channels;
   A.gates = gates;
   A.per_gate = channels / gates;
-  A.period = offsets == nullptr ? rows / sequences : 0;
+  A.period = even ? rows / sequences : 0;
   A.offsets = offsets;
   A.reverse = reverse != 0;
   A.x = x;
@@ -223,15 +290,21 @@ extern "C" int gs_gated_scan_forward(int64_t rows, int sequences, int channels, 
   A.h = h;
   A.final_state = final_state;
   A.saved = saved;
-  if (p.tiles > 1) {
+  const size_t need = gs_gated_scan_scratch_bytes(rows, sequences, even, channels, gates, x_type, gate_type, 0);
+  if (need > 0) {
     if (scratch == nullptr || ((uintptr_t)scratch & 15)) return GS_ERR_INVALID_ARGUMENT;
-    if (scratch_bytes < chain_bytes(p.tiles, channels)) return GS_ERR_CAPACITY;
+    if (scratch_bytes < need) return GS_ERR_CAPACITY;
+    place_chain(A, scratch);
+    if (even) A.hints = nullptr;
   }
   A.status = device_status_word();
   if (A.status == nullptr) return GS_ERR_CUDA;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int failed = place_chain(A, scratch, st);
-  if (failed) return failed;
-  run_forward(A, p, x_type, gate_type, st);
-  return launch_status();
+  rc = launch_setup(A, initial, final_state, st);
+  if (rc || rows == 0) return rc;
+  const bool same = x_type == gate_type;
+  if (x_type == GS_TYPE_F32) return pick_forward<float, float>(A, st);
+  if (x_type == GS_TYPE_BF16)
+    return same ? pick_forward<__nv_bfloat16, __nv_bfloat16>(A, st) : pick_forward<__nv_bfloat16, float>(A, st);
+  return same ? pick_forward<__half, __half>(A, st) : pick_forward<__half, float>(A, st);
 }

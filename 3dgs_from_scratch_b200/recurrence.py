@@ -95,11 +95,12 @@ def _forward(x, gate, initial, offsets, reverse, sequences, keep):
         if offsets.dtype == torch.int64:  # beyond 32 bits stays out of range
             offs = offsets.clamp(-1, 2 ** 31 - 1).to(torch.int32)
         offs = offs.contiguous()
+    sizes = (rows, sequences, int(offs is None), channels, gates, *types)
     saved = None
     if keep:
-        saved = torch.empty(nat.query("gs_gated_scan_saved_bytes", rows, channels, gates, *types) // 4,
+        saved = torch.empty(nat.query("gs_gated_scan_saved_bytes", *sizes) // 4,
                             dtype=torch.float32, device=dev)
-    nbytes = nat.query("gs_gated_scan_scratch_bytes", rows, channels, gates, *types, 0)
+    nbytes = nat.query("gs_gated_scan_scratch_bytes", *sizes, 0)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with on_device(dev):
         nat.call("gs_gated_scan_forward", rows, sequences, channels, gates, *types, xr.data_ptr(),
@@ -139,7 +140,8 @@ class _GatedScan(torch.autograd.Function):
         dh, dh_step = (None, channels) if grad_h is None else _rows_of(grad_h, channels)
         init = None if initial is None else initial.to(torch.float32).contiguous()
         dinit = torch.empty((sequences, channels), dtype=torch.float32, device=dev) if want else None
-        nbytes = nat.query("gs_gated_scan_scratch_bytes", rows, channels, gates, *types, 1)
+        nbytes = nat.query("gs_gated_scan_scratch_bytes", rows, sequences, int(offs is None), channels, gates,
+                           *types, 1)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         with on_device(dev):
             nat.call("gs_gated_scan_backward", rows, sequences, channels, gates, *types,

@@ -594,12 +594,13 @@ GS_API int gs_reset_opacities(int n, float *opacity_logits, float *exp_avg, floa
  * GS_ERR_INVALID_ARGUMENT in the device status word; what is written then is
  * undefined, but within the buffers. */
 
-/* What the forward keeps for the backward (the state before each of its
- * tiles), and the scratch of either direction (0: none; 16-byte aligned). */
-GS_API size_t gs_gated_scan_saved_bytes(int64_t rows, int channels, int gates, int x_type,
-                                        int gate_type);
-GS_API size_t gs_gated_scan_scratch_bytes(int64_t rows, int channels, int gates, int x_type,
-                                          int gate_type, int backward);
+/* What the forward keeps for the backward (the state before every few rows),
+ * and the scratch of either direction (0: none), both 16-byte aligned. even = 1:
+ * offsets will be NULL. */
+GS_API size_t gs_gated_scan_saved_bytes(int64_t rows, int sequences, int even, int channels,
+                                        int gates, int x_type, int gate_type);
+GS_API size_t gs_gated_scan_scratch_bytes(int64_t rows, int sequences, int even, int channels,
+                                          int gates, int x_type, int gate_type, int backward);
 
 /* initial NULL: zeros. final_state NULL: not written. saved NULL: no backward
  * follows. */

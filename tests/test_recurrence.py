@@ -123,7 +123,7 @@ def test_batches_of_even_sequences(gs, rows, sequences, channels, gates):
 @pytest.mark.parametrize("channels,gates", [(40, 40), (40, 1), (40, 5), (21, 21), (21, 7), (520, 2), (301, 1)])
 @pytest.mark.parametrize("reverse", [False, True])
 def test_types_and_ragged_sequences(gs, dtype, gate_dtype, channels, gates, reverse):
-    # empty ones at both ends and in the middle, one row, ends inside and at the edge of tiles,
+    # empty ones at both ends and in the middle, one row, ends inside and at the edge of chunks,
     # rows behind the last
     offsets = [0, 0, 1, 129, 129, 129, 257, 320, 321, 700, 700]
     check(gs, 713, 10, channels, gates, offsets=offsets, dtype=dtype, gate_dtype=gate_dtype,
@@ -369,12 +369,13 @@ def test_entry_points_refuse_bad_arguments(gs):
 
     for kw in (dict(rows=-1), dict(rows=2 ** 31), dict(seqs=0), dict(seqs=3), dict(channels=0), dict(gates=0),
                dict(gates=3), dict(xt=3), dict(xt=1, gt=2), dict(xt=0, gt=1), dict(x=P), dict(gate=P),
-               dict(h=P), dict(x=at + 4), dict(xs=9), dict(gst=10), dict(h=at + 8), dict(init=at + 2),
+               dict(h=P), dict(x=at + 4), dict(xs=9), dict(gst=11), dict(h=at + 4), dict(init=at + 2),
                dict(offs=at + 2), dict(rows=2 ** 20)):       # many tiles and no scratch
         assert fwd(**kw) == bad, kw
     assert lib.gs_gated_scan_backward(8, 2, 8, 8, 0, 0, at, 8, at, 8, P, P, 0, P, at, 8, P, at, at, P,
                                       P, 0, P) == bad         # nothing kept by the forward
-    assert lib.gs_gated_scan_saved_bytes(-1, 8, 8, 0, 0) == 0
-    assert lib.gs_gated_scan_saved_bytes(100, 8, 8, 0, 0) == 8 * 4
-    assert lib.gs_gated_scan_scratch_bytes(100, 8, 8, 0, 0, 0) == 0
-    assert lib.gs_gated_scan_scratch_bytes(1 << 20, 8, 8, 0, 0, 1) > 0
+    assert lib.gs_gated_scan_saved_bytes(-1, 1, 1, 8, 8, 0, 0) == 0
+    assert lib.gs_gated_scan_saved_bytes(100, 1, 1, 8, 8, 0, 0) >= 100 // 8 * 8 * 4
+    assert lib.gs_gated_scan_scratch_bytes(24, 1, 1, 8, 8, 0, 0, 0) == 0
+    assert lib.gs_gated_scan_scratch_bytes(1 << 20, 1, 1, 8, 8, 0, 0, 1) > 0
+    assert lib.gs_gated_scan_scratch_bytes(100, 5, 0, 8, 8, 0, 0, 0) > 0
