@@ -7,6 +7,7 @@ data_ptr()), streams as the raw cudaStream_t of torch's current stream.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 
@@ -162,6 +163,12 @@ def query(name: str, *args):
     return getattr(lib(), name)(*args)
 
 
+@functools.lru_cache(maxsize=4096)
+def size_query(name: str, *args) -> int:
+    """query() of a size that depends on its arguments alone."""
+    return query(name, *args)
+
+
 def launch_count() -> int:
     return int(lib().gs_launch_count())
 
@@ -169,4 +176,6 @@ def launch_count() -> int:
 def stream_ptr(device=None) -> int:
     import torch
 
+    if device is not None and device.index is not None:
+        return torch._C._cuda_getCurrentRawStream(device.index)
     return int(torch.cuda.current_stream(device).cuda_stream)

@@ -42,11 +42,10 @@ def _check_steps(name, steps, coefficients, eps):
 
 
 def _scratch(batch, rows, cols, kind, dev):
-    nbytes = nat.query("gs_orthogonalize_scratch_bytes", batch, rows, cols, kind)
+    nbytes = nat.size_query("gs_orthogonalize_scratch_bytes", batch, rows, cols, kind)
     return torch.empty(nbytes, dtype=torch.uint8, device=dev), nbytes
 
 
-@torch.no_grad()
 def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS,
                   eps: float = 1e-7) -> torch.Tensor:
     """The update with its singular values brought near 1 by `steps` of
@@ -74,7 +73,6 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=COEFFICIENT
     return out
 
 
-@torch.no_grad()
 def muon_step(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor, lr: float,
               beta: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
               scale: float | None = None, steps: int = 5, coefficients=COEFFICIENTS,

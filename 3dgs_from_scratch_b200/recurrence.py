@@ -23,11 +23,12 @@ from . import _native as nat
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on_device(dev):
     """The device's context where it is not the current one."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+    return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
 def _rows_of(t, channels):
@@ -77,38 +78,78 @@ def _check(x, gate, initial, offsets):
     return sequences
 
 
+def _work(name, sizes, dev, *more):
+    """Scratch of a size query (None, 0 where there is none)."""
+    nbytes = nat.size_query(name, *sizes, *more)
+    return (torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None), nbytes
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def _states(t):
+    """States as the kernels read them."""
+    if t is None or t.dtype == torch.float32 and t.is_contiguous():
+        return t
+    return t.to(torch.float32).contiguous()
+
+
 def _forward(x, gate, initial, offsets, reverse, sequences, keep):
     dev, channels, gates = x.device, x.shape[-1], gate.shape[-1]
     h = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    if sequences == 0:
-        return h, torch.empty((0, channels), dtype=torch.float32, device=dev), None, None
-    rows = x.numel() // channels
-    types = (_TYPES[x.dtype], _TYPES[gate.dtype])
     final = torch.empty((sequences, channels), dtype=torch.float32, device=dev)
-    if rows == 0:
+    rows = x.numel() // channels
+    if rows == 0 or sequences == 0:
         final.zero_() if initial is None else final.copy_(initial)
         return h, final, None, None
     (xr, x_step), (gr, g_step) = _rows_of(x, channels), _rows_of(gate, gates)
-    init = None if initial is None else initial.to(torch.float32).contiguous()
-    offs = offsets
-    if offsets is not None:
-        if offsets.dtype == torch.int64:  # beyond 32 bits stays out of range
-            offs = offsets.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    init, offs = _states(initial), offsets
+    if offs is not None:
+        if offs.dtype == torch.int64:  # beyond 32 bits stays out of range
+            offs = offs.clamp(-1, 2 ** 31 - 1).to(torch.int32)
         offs = offs.contiguous()
-    sizes = (rows, sequences, int(offs is None), channels, gates, *types)
-    saved = None
-    if keep:
-        saved = torch.empty(nat.query("gs_gated_scan_saved_bytes", *sizes) // 4,
-                            dtype=torch.float32, device=dev)
-    nbytes = nat.query("gs_gated_scan_scratch_bytes", *sizes, 0)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    sizes = (rows, sequences, int(offs is None), channels, gates, _TYPES[x.dtype], _TYPES[gate.dtype])
+    saved = _work("gs_gated_scan_saved_bytes", sizes, dev)[0] if keep else None
+    scratch, nbytes = _work("gs_gated_scan_scratch_bytes", sizes, dev, 0)
     with on_device(dev):
-        nat.call("gs_gated_scan_forward", rows, sequences, channels, gates, *types, xr.data_ptr(),
-                 x_step, gr.data_ptr(), g_step, 0 if init is None else init.data_ptr(),
-                 0 if offs is None else offs.data_ptr(), int(reverse), h.data_ptr(),
-                 final.data_ptr(), 0 if saved is None else saved.data_ptr(),
-                 0 if scratch is None else scratch.data_ptr(), nbytes, nat.stream_ptr(dev))
+        nat.call("gs_gated_scan_forward", rows, sequences, channels, gates, sizes[5], sizes[6],
+                 xr.data_ptr(), x_step, gr.data_ptr(), g_step, _ptr(init), _ptr(offs), int(reverse),
+                 h.data_ptr(), final.data_ptr(), _ptr(saved), _ptr(scratch), nbytes,
+                 nat.stream_ptr(dev))
     return h, final, saved, offs
+
+
+def _backward(ctx, grad_h, grad_final):
+    x, gate, initial, offs, saved = ctx.saved_tensors
+    dev, channels, gates, sequences = x.device, x.shape[-1], gate.shape[-1], ctx.sequences
+    want = initial is not None and ctx.needs_input_grad[2]
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
+    dfinal = _states(grad_final)
+    rows = x.numel() // channels
+    if sequences == 0 or rows == 0:
+        dinit = None
+        if want:
+            dinit = torch.zeros_like(initial) if dfinal is None else dfinal.to(initial.dtype)
+        return dx, dgate, dinit, None, None, None
+    (xr, x_step), (gr, g_step) = _rows_of(x, channels), _rows_of(gate, gates)
+    dh, dh_step = (None, channels) if grad_h is None else _rows_of(grad_h, channels)
+    init = _states(initial)
+    dinit = torch.empty((sequences, channels), dtype=torch.float32, device=dev) if want else None
+    sizes = (rows, sequences, int(offs is None), channels, gates, _TYPES[x.dtype], _TYPES[gate.dtype])
+    scratch, nbytes = _work("gs_gated_scan_scratch_bytes", sizes, dev, 1)
+    with on_device(dev):
+        nat.call("gs_gated_scan_backward", rows, sequences, channels, gates, sizes[5], sizes[6],
+                 xr.data_ptr(), x_step, gr.data_ptr(), g_step, _ptr(init), _ptr(offs),
+                 int(ctx.reverse), saved.data_ptr(), _ptr(dh), dh_step, _ptr(dfinal), dx.data_ptr(),
+                 dgate.data_ptr(), _ptr(dinit), _ptr(scratch), nbytes, nat.stream_ptr(dev))
+    if want and initial.dtype != torch.float32:
+        dinit = dinit.to(initial.dtype)
+    return dx, dgate, dinit, None, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class _GatedScan(torch.autograd.Function):
@@ -121,37 +162,9 @@ class _GatedScan(torch.autograd.Function):
         return h, final
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_h, grad_final):
-        x, gate, initial, offs, saved = ctx.saved_tensors
-        dev, channels, gates, sequences = x.device, x.shape[-1], gate.shape[-1], ctx.sequences
-        want = initial is not None and ctx.needs_input_grad[2]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
-        dfinal = None if grad_final is None else grad_final.to(torch.float32).contiguous()
-        rows = x.numel() // channels
-        if sequences == 0 or rows == 0:
-            dinit = None
-            if want:
-                dinit = torch.zeros_like(initial) if dfinal is None else dfinal.to(initial.dtype)
-            return dx, dgate, dinit, None, None, None
-        types = (_TYPES[x.dtype], _TYPES[gate.dtype])
-        (xr, x_step), (gr, g_step) = _rows_of(x, channels), _rows_of(gate, gates)
-        dh, dh_step = (None, channels) if grad_h is None else _rows_of(grad_h, channels)
-        init = None if initial is None else initial.to(torch.float32).contiguous()
-        dinit = torch.empty((sequences, channels), dtype=torch.float32, device=dev) if want else None
-        nbytes = nat.query("gs_gated_scan_scratch_bytes", rows, sequences, int(offs is None), channels, gates,
-                           *types, 1)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        with on_device(dev):
-            nat.call("gs_gated_scan_backward", rows, sequences, channels, gates, *types,
-                     xr.data_ptr(), x_step, gr.data_ptr(), g_step,
-                     0 if init is None else init.data_ptr(), 0 if offs is None else offs.data_ptr(),
-                     int(ctx.reverse), saved.data_ptr(), 0 if dh is None else dh.data_ptr(), dh_step,
-                     0 if dfinal is None else dfinal.data_ptr(), dx.data_ptr(), dgate.data_ptr(),
-                     0 if dinit is None else dinit.data_ptr(),
-                     0 if scratch is None else scratch.data_ptr(), nbytes, nat.stream_ptr(dev))
-        return (dx, dgate, dinit.to(initial.dtype) if want else None, None, None, None)
+        # a graph of the backward (create_graph) is refused when it is used
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad_h, grad_final)
 
 
 def gated_scan(x: torch.Tensor, gate: torch.Tensor, initial: torch.Tensor | None = None,
