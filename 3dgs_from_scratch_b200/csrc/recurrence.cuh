@@ -45,7 +45,7 @@ namespace scan {
 
 constexpr int kThreads = 256;
 constexpr int kBatch = 8;  // rows in flight, and from one kept state to the next
-constexpr int kFill = 640;  // threads on an SM that a chunk length aims at
+constexpr int kFill = 1280;  // threads on an SM that a chunk length aims at
 
 // How a problem is cut. It depends on the sizes and types alone, never on
 // pointers, so that the backward finds the states that the forward kept.
@@ -276,36 +276,28 @@ __global__ void __launch_bounds__(kThreads) maps_kernel(const __grid_constant__ 
     const GT *gate = reinterpret_cast<const GT *>(A.gate) + row * A.gate_stride + p.g;
     const int64_t step = up ? xs : -xs, gstep = up ? A.gate_stride : -A.gate_stride;
     const bool some = !BACK || A.dh != nullptr;
-    const auto walk = [&](const Pack<XT, V> &x, const Gates<GT, V, SHARED> &g) {
+    constexpr int kAhead = V == 1 ? 2 * kBatch : kBatch;
+    for (int left = n; left > 0; left -= kAhead) {
+      Pack<XT, V> x[kAhead];
+      Gates<GT, V, SHARED> g[kAhead];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float e = some ? to_f32<XT>(x.e[v]) : 0.f;
-        L[v] = BACK ? g(v) * (e + L[v]) : fmaf(g(v), L[v], e);
-        P[v] *= g(v);
-      }
-    };
-    int i = 0;
-    for (; i + kBatch <= n; i += kBatch) {
-      Pack<XT, V> x[kBatch];
-      Gates<GT, V, SHARED> g[kBatch];
+      for (int k = 0; k < kAhead; ++k)
+        if (k < left) {
+          if (some) x[k] = load_pack<XT, V>(from + k * step);
+          g[k].load(gate + k * gstep);
+        }
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        if (some) x[k] = load_pack<XT, V>(from + k * step);
-        g[k].load(gate + k * gstep);
-      }
+      for (int k = 0; k < kAhead; ++k)
+        if (k < left) {
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) walk(x[k], g[k]);
-      from += kBatch * step;
-      gate += kBatch * gstep;
-    }
-    for (; i < n; ++i) {
-      Pack<XT, V> x;
-      Gates<GT, V, SHARED> g;
-      if (some) x = load_pack<XT, V>(from);
-      g.load(gate);
-      walk(x, g);
-      from += step;
-      gate += gstep;
+          for (int v = 0; v < V; ++v) {
+            const float e = some ? to_f32<XT>(x[k].e[v]) : 0.f;
+            L[v] = BACK ? g[k](v) * (e + L[v]) : fmaf(g[k](v), L[v], e);
+            P[v] *= g[k](v);
+          }
+        }
+      from += kAhead * step;
+      gate += kAhead * gstep;
     }
   }
 #pragma unroll

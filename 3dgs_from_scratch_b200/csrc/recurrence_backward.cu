@@ -33,28 +33,39 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
 #pragma unroll
   for (int v = 0; v < V; ++v) v_in[v] = 0.f;
   if (A.carry != nullptr && p.on) load_kept<V>(A.carry, A, p.chunk, p.c, v_in);
-  for (int b = A.plan.kept - 1; b >= 0; --b) {
+  Pack<XT, V> x[kBatch], dh[kBatch];
+  Gates<GT, V, SHARED> g[kBatch];
+  const auto rows_of = [&](int b) {  // of batch b
     const int64_t t = p.t0 + (int64_t)b * kBatch;
-    const int n = !p.on || t >= p.t1 ? 0 : p.t1 - t < kBatch ? (int)(p.t1 - t) : kBatch;
-    if (n > 0) {
-      const int64_t row = row_at(A, t);
-      Pack<XT, V> x[kBatch], dh[kBatch];
-      Gates<GT, V, SHARED> g[kBatch];
-      const XT *from = reinterpret_cast<const XT *>(A.x) + row * A.x_stride + p.c;
-      const GT *gate = reinterpret_cast<const GT *>(A.gate) + row * A.gate_stride + p.g;
-      const XT *grad = reinterpret_cast<const XT *>(A.dh) + row * A.dh_stride + p.c;
+    return b < 0 || !p.on || t >= p.t1 ? 0 : p.t1 - t < kBatch ? (int)(p.t1 - t) : kBatch;
+  };
+  const auto load = [&](int b) {
+    const int n = rows_of(b);
+    const int64_t row = row_at(A, p.t0 + (int64_t)b * kBatch);
+    const XT *from = reinterpret_cast<const XT *>(A.x) + row * A.x_stride + p.c;
+    const GT *gate = reinterpret_cast<const GT *>(A.gate) + row * A.gate_stride + p.g;
+    const XT *grad = reinterpret_cast<const XT *>(A.dh) + row * A.dh_stride + p.c;
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k)
-        if (k < n) {
-          x[k] = load_pack<XT, V>(from + k * xs);
-          g[k].load(gate + k * gs);
-          if (A.dh != nullptr) {
-            dh[k] = load_pack<XT, V>(grad + k * ds);
-          } else {
+    for (int k = 0; k < kBatch; ++k)
+      if (k < n) {
+        x[k] = load_pack<XT, V>(from + k * xs);
+        g[k].load(gate + k * gs);
+        if (A.dh != nullptr) {
+          dh[k] = load_pack<XT, V>(grad + k * ds);
+        } else {
 #pragma unroll
-            for (int v = 0; v < V; ++v) dh[k].e[v] = from_f32<XT>(0.f);
-          }
+          for (int v = 0; v < V; ++v) dh[k].e[v] = from_f32<XT>(0.f);
         }
+      }
+  };
+  // Where the block adds up gates between two batches, the next one is on its
+  // way meanwhile.
+  if (SHARED) load(A.plan.kept - 1);
+  for (int b = A.plan.kept - 1; b >= 0; --b) {
+    const int n = rows_of(b);
+    if (!SHARED) load(b);
+    if (n > 0) {
+      const int64_t row = row_at(A, p.t0 + (int64_t)b * kBatch);
       float before[kBatch][V];  // the state before each row
       float h[V];
       load_kept<V>(A.saved, A, p.chunk * A.plan.kept + b, p.c, h);
@@ -123,19 +134,28 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
       }
     }
     if (SHARED) {
+      load(b - 1);
       // The sums of the threads that share a gate, in their order.
       __syncthreads();
       const int width = A.plan.tx * V, c0 = cblk * width, c1 = c0 + width < A.channels ? c0 + width : A.channels;
       const int first = c0 / A.per_gate, count = (c1 - 1) / A.per_gate - first + 1;
-      for (int k = threadIdx.x; k < A.plan.cy * kBatch * count; k += kThreads) {
-        const int line = k / count, at = first + k % count;
-        const int64_t chunk = group * A.plan.cy + line / kBatch;
-        const int64_t r = chunk * A.plan.chunk + b * kBatch + line % kBatch;
-        if (chunk >= A.plan.chunks || r >= A.rows || b * kBatch + line % kBatch >= A.plan.chunk) continue;
+      // A sum is shared out to as many adjacent lanes as there are threads for.
+      const int all = A.plan.cy * kBatch * count;
+      int parts = 1;
+      while (parts < 32 && parts * 2 * all <= kThreads) parts *= 2;
+      for (int j = threadIdx.x; j < (all * parts + 31) / 32 * 32; j += kThreads) {
+        const int k = j / parts, part = j % parts, line = k / count, at = first + k % count;
         const int lo = at * A.per_gate > c0 ? at * A.per_gate : c0;
         const int hi = (at + 1) * A.per_gate < c1 ? (at + 1) * A.per_gate : c1;
         float sum = 0.f;
-        for (int c = lo; c < hi; c += V) sum += sums[line * A.plan.tx + (c - c0) / V];
+        if (k < all)
+          for (int c = lo + part * V; c < hi; c += parts * V) sum += sums[line * A.plan.tx + (c - c0) / V];
+        for (int d = parts / 2; d > 0; d /= 2) sum += __shfl_down_sync(0xffffffffu, sum, d);
+        const int64_t chunk = group * A.plan.cy + line / kBatch;
+        const int64_t r = chunk * A.plan.chunk + b * kBatch + line % kBatch;
+        if (part != 0 || k >= all || chunk >= A.plan.chunks || r >= A.rows ||
+            b * kBatch + line % kBatch >= A.plan.chunk)
+          continue;
         const int64_t row = row_at(A, r);
         if (A.partial == nullptr) {
           reinterpret_cast<GT *>(A.dgate)[row * A.gates + at] = from_f32<GT>(sum);

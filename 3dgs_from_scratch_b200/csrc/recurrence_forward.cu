@@ -84,50 +84,68 @@ int launch_setup(const Args &A, const float *src, float *dst, cudaStream_t st) {
   return launch_status();
 }
 
-// The state that enters each chunk, from the chunks' maps: 32 channels a block,
-// its 32 warps a run of chunks each, then the runs' maps in order, then the run
-// once more from the state before it.
+// The state that enters each chunk, from the chunks' maps: 8 channels a block,
+// 128 threads a channel with a run of chunks each; the runs' maps are scanned in
+// shared memory, then each thread goes through its run once more from the state
+// before it.
+constexpr int kCarryChannels = 8, kRuns = 128;
+
 template <bool BACK>
-__global__ void __launch_bounds__(1024) carry_kernel(const __grid_constant__ Args A) {
-  __shared__ float2 runs[32][33];
-  __shared__ int run_cut[32];
-  const int c = blockIdx.x * 32 + (int)lane_id(), run = threadIdx.x / 32;
+__global__ void __launch_bounds__(kCarryChannels *kRuns) carry_kernel(const __grid_constant__ Args A) {
+  __shared__ float2 maps[2][kRuns][kCarryChannels];
+  __shared__ uint8_t cuts[2][kRuns];
+  const int lane = threadIdx.x % kCarryChannels, run = threadIdx.x / kCarryChannels;
+  const int c = blockIdx.x * kCarryChannels + lane;
   const bool on = c < A.channels;
-  const int64_t n = A.plan.chunks, k0 = n * run / 32, k1 = n * (run + 1) / 32;
-  const auto chunk_of = [&](int64_t k) { return BACK ? n - 1 - k : k; };
+  const int64_t n = A.plan.chunks, k0 = n * run / kRuns, k1 = n * (run + 1) / kRuns;
+  const int64_t step = BACK ? -1 : 1, first = BACK ? n - 1 - k0 : k0;
+  const float2 *__restrict__ map = A.maps + first * A.channels + (on ? c : 0);
+  const int *__restrict__ cut = A.cuts + first;
+  float *__restrict__ to = A.carry + first * A.channels + (on ? c : 0);
+  const int64_t row = step * A.channels;
   float P = 1.f, L = 0.f;
-  bool cut = false;
+  bool any = false;
 #pragma unroll 8
-  for (int64_t k = k0; k < k1; ++k) {
-    const int64_t at = chunk_of(k);
-    const float2 m = on ? A.maps[at * A.channels + c] : make_float2(1.f, 0.f);
-    const bool here = A.cuts[at] != 0;
+  for (int64_t k = 0; k < k1 - k0; ++k) {
+    const float2 m = map[k * row];
+    const bool here = cut[k * step] != 0;
     L = here ? m.y : fmaf(m.x, L, m.y);
     P *= m.x;
-    cut = cut || here;
+    any = any || here;
   }
-  runs[run][lane_id()] = make_float2(P, L);
-  if (lane_id() == 0) run_cut[run] = cut;
+  // Inclusive scan of the runs' maps, doubling the reach.
+  maps[0][run][lane] = make_float2(P, L);
+  if (lane == 0) cuts[0][run] = any;
   __syncthreads();
-  float h = 0.f;
-  for (int q = 0; q < run; ++q) {
-    const float2 m = runs[q][lane_id()];
-    h = run_cut[q] ? m.y : fmaf(m.x, h, m.y);
+  int at = 0;
+  for (int reach = 1; reach < kRuns; reach *= 2, at ^= 1) {
+    float2 m = maps[at][run][lane];
+    bool here = cuts[at][run];
+    if (run >= reach) {
+      const float2 before = maps[at][run - reach][lane];
+      const bool cut_before = cuts[at][run - reach];
+      if (!here) m.y = fmaf(m.x, before.y, m.y);
+      m.x *= before.x;
+      here = here || cut_before;
+    }
+    maps[at ^ 1][run][lane] = m;
+    if (lane == 0) cuts[at ^ 1][run] = here;
+    __syncthreads();
   }
   if (!on) return;
+  float h = run > 0 ? maps[at][run - 1][lane].y : 0.f;  // from a zero state
 #pragma unroll 8
-  for (int64_t k = k0; k < k1; ++k) {
-    const int64_t at = chunk_of(k);
-    A.carry[at * A.channels + c] = h;
-    const float2 m = A.maps[at * A.channels + c];
-    h = A.cuts[at] != 0 ? m.y : fmaf(m.x, h, m.y);
+  for (int64_t k = 0; k < k1 - k0; ++k) {
+    to[k * row] = h;
+    const float2 m = map[k * row];
+    h = cut[k * step] != 0 ? m.y : fmaf(m.x, h, m.y);
   }
 }
 
 int launch_carry(const Args &A, bool back, cudaStream_t st) {
-  const unsigned grid = (unsigned)((A.channels + 31) / 32);
-  if (back) carry_kernel<true><<<grid, 1024, 0, st>>>(A);
-  else carry_kernel<false><<<grid, 1024, 0, st>>>(A);
+  const unsigned grid = (unsigned)((A.channels + kCarryChannels - 1) / kCarryChannels);
+  if (back) carry_kernel<true><<<grid, kCarryChannels * kRuns, 0, st>>>(A);
+  else carry_kernel<false><<<grid, kCarryChannels * kRuns, 0, st>>>(A);
   count_launch();
   return launch_status();
 }
