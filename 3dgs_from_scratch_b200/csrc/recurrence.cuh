@@ -184,32 +184,40 @@ __device__ __forceinline__ void store_kept(float *__restrict__ p, const Args &A,
 
 // ---- where a row belongs ----------------------------------------------------------------
 
-// A sequence and its rows lo..hi-1. Offsets that do not ascend give wrong
-// sequences, but never an index outside [0, sequences).
+// A sequence and its rows lo..hi-1 (of the tensor; rows <= INT32_MAX). Offsets
+// that do not ascend give wrong sequences, but never an index outside
+// [0, sequences).
 struct Cursor {
-  int s;
-  int64_t lo, hi;
-  // Moves to the sequence of row p (of the tensor). Rows outside every sequence
-  // leave it at a neighbour that does not hold them.
-  __device__ __forceinline__ void seek(const Args &A, int64_t p) {
+  int s, lo, hi;
+  // Moves to the sequence of row p. Rows outside every sequence leave it at a
+  // neighbour that does not hold them.
+  __device__ __forceinline__ void seek(const Args &A, int p) {
     if (A.offsets == nullptr) {
-      s = (int)((uint32_t)p / (uint32_t)A.period);
-      lo = s * A.period;
-      hi = lo + A.period;
+      const int n = (int)A.period;
+      s = (int)((uint32_t)p / (uint32_t)n);
+      lo = s * n;
+      hi = lo + n;
       return;
     }
-    while (s + 1 < A.sequences && p >= (int64_t)A.offsets[s + 1]) ++s;
-    while (s > 0 && p < (int64_t)A.offsets[s]) --s;
+    while (s + 1 < A.sequences && p >= A.offsets[s + 1]) ++s;
+    while (s > 0 && p < A.offsets[s]) --s;
     lo = A.offsets[s];
     hi = A.offsets[s + 1];
   }
-  __device__ __forceinline__ bool holds(int64_t p) const { return p >= lo && p < hi; }
+  __device__ __forceinline__ bool holds(int p) const { return p >= lo && p < hi; }
+  // Rows p..p+n-1 are all inside and neither its first nor its last.
+  __device__ __forceinline__ bool plain(int p, int n) const { return p > lo && p < hi && hi - p > n; }
+  // Logical rows from row p on to the end of what p is in: its sequence, or the
+  // rows outside of every sequence. At least 1. The cursor has sought p.
+  __device__ __forceinline__ int rest(const Args &A, int p) const {
+    int n = INT32_MAX / 2;
+    if (holds(p)) n = A.reverse ? p - lo + 1 : hi - p;
+    else if (!A.reverse && p < lo) n = lo - p;
+    else if (A.reverse && p >= hi) n = p - hi + 1;
+    return n < 1 ? 1 : n;
+  }
+  __device__ __forceinline__ bool first(const Args &A, int p) const { return p == (A.reverse ? hi - 1 : lo); }
 };
-
-// Rows p..p+n-1, all inside the cursor's sequence and neither its first nor last.
-__device__ __forceinline__ bool plain_rows(const Cursor &q, int64_t p, int n) {
-  return p > q.lo && p + n < q.hi;
-}
 
 // The place of a thread: its channels and its chunk's logical rows t0..t1-1.
 struct Place {
@@ -249,7 +257,7 @@ __global__ void __launch_bounds__(kThreads) maps_kernel(const __grid_constant__ 
   const Place p = place_of<V, SHARED>(A, blockIdx.x / A.plan.channel_blocks, cblk);
   if (!p.on) return;
   const int64_t t_end = BACK ? p.t0 : p.t1 - 1;  // the chunk's last row along the chain
-  const int64_t row_end = row_at(A, t_end);
+  const int row_end = (int)row_at(A, t_end);
   Cursor q;
   q.s = A.hints != nullptr ? A.hints[p.chunk + (BACK ? 0 : A.plan.chunks)] : 0;
   q.seek(A, row_end);
@@ -261,9 +269,9 @@ __global__ void __launch_bounds__(kThreads) maps_kernel(const __grid_constant__ 
     cut = true;   // the sequence ends with the chunk, or the row is outside
     needed = false;
   } else {
-    const int64_t first = up ? q.lo : q.hi - 1;  // the sequence's first row along the chain
-    const int64_t in_chunk = (up ? row_end - first : first - row_end) + 1;
-    if (in_chunk <= n) n = (int)in_chunk, cut = true;
+    const int first = up ? q.lo : q.hi - 1;  // the sequence's first row along the chain
+    const int before = up ? row_end - first : first - row_end;
+    if (before < n) n = before + 1, cut = true;
   }
   float P[V], L[V];
 #pragma unroll

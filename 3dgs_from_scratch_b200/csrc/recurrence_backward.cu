@@ -17,9 +17,13 @@
 namespace gs {
 namespace scan {
 
+constexpr int kParts = 4;  // threads that share a sum over a gate's channels
+
 template <typename XT, typename GT, int V, bool SHARED>
 __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constant__ Args A) {
-  __shared__ float sums[SHARED ? kThreads * kBatch : 1];  // [chunk of the block][row][vector]
+  // [chunk of the block][row][vector], batches in turn: a batch's sums are read
+  // while the next one's are written, with one barrier between.
+  __shared__ float both[2][SHARED ? kThreads * kBatch : 1];
   const int cblk = blockIdx.x % A.plan.channel_blocks;
   const int64_t group = blockIdx.x / A.plan.channel_blocks;
   const Place p = place_of<V, SHARED>(A, group, cblk);
@@ -29,65 +33,66 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
   Cursor q;
   q.s = A.hints != nullptr && p.on ? A.hints[p.chunk + A.plan.chunks] : 0;
   q.lo = q.hi = 0;
+  const int one = A.reverse ? -1 : 1;
   float v_in[V];  // what the row after hands down
 #pragma unroll
   for (int v = 0; v < V; ++v) v_in[v] = 0.f;
   if (A.carry != nullptr && p.on) load_kept<V>(A.carry, A, p.chunk, p.c, v_in);
-  Pack<XT, V> x[kBatch], dh[kBatch];
-  Gates<GT, V, SHARED> g[kBatch];
-  const auto rows_of = [&](int b) {  // of batch b
-    const int64_t t = p.t0 + (int64_t)b * kBatch;
-    return b < 0 || !p.on || t >= p.t1 ? 0 : p.t1 - t < kBatch ? (int)(p.t1 - t) : kBatch;
-  };
-  const auto load = [&](int b) {
-    const int n = rows_of(b);
-    const int64_t row = row_at(A, p.t0 + (int64_t)b * kBatch);
-    const XT *from = reinterpret_cast<const XT *>(A.x) + row * A.x_stride + p.c;
-    const GT *gate = reinterpret_cast<const GT *>(A.gate) + row * A.gate_stride + p.g;
-    const XT *grad = reinterpret_cast<const XT *>(A.dh) + row * A.dh_stride + p.c;
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k)
-      if (k < n) {
-        x[k] = load_pack<XT, V>(from + k * xs);
-        g[k].load(gate + k * gs);
-        if (A.dh != nullptr) {
-          dh[k] = load_pack<XT, V>(grad + k * ds);
-        } else {
-#pragma unroll
-          for (int v = 0; v < V; ++v) dh[k].e[v] = from_f32<XT>(0.f);
-        }
-      }
-  };
-  // Where the block adds up gates between two batches, the next one is on its
-  // way meanwhile.
-  if (SHARED) load(A.plan.kept - 1);
   for (int b = A.plan.kept - 1; b >= 0; --b) {
-    const int n = rows_of(b);
-    if (!SHARED) load(b);
+    float *sums = both[b & 1];
+    const int64_t t = p.t0 + (int64_t)b * kBatch;
+    const int n = !p.on || t >= p.t1 ? 0 : p.t1 - t < kBatch ? (int)(p.t1 - t) : kBatch;
     if (n > 0) {
-      const int64_t row = row_at(A, p.t0 + (int64_t)b * kBatch);
+      const int row = (int)row_at(A, t);
+      Pack<XT, V> x[kBatch], dh[kBatch];
+      Gates<GT, V, SHARED> g[kBatch];
+      {
+        const XT *from = reinterpret_cast<const XT *>(A.x) + row * A.x_stride + p.c;
+        const GT *gate = reinterpret_cast<const GT *>(A.gate) + row * A.gate_stride + p.g;
+        const XT *grad = reinterpret_cast<const XT *>(A.dh) + row * A.dh_stride + p.c;
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+          if (k < n) {
+            x[k] = load_pack<XT, V>(from);
+            g[k].load(gate);
+            from += xs;
+            gate += gs;
+            if (A.dh != nullptr) {
+              dh[k] = load_pack<XT, V>(grad);
+              grad += ds;
+            } else {
+#pragma unroll
+              for (int v = 0; v < V; ++v) dh[k].e[v] = from_f32<XT>(0.f);
+            }
+          }
+      }
       float before[kBatch][V];  // the state before each row
       float h[V];
       load_kept<V>(A.saved, A, p.chunk * A.plan.kept + b, p.c, h);
-      XT *to = reinterpret_cast<XT *>(A.dx) + row * A.channels + p.c;
-      GT *out = reinterpret_cast<GT *>(A.dgate) + row * A.gates + p.c;
-      const auto finish = [&](int k) {  // row k, given what the row after it hands down
+      const int last = row + (n - 1) * one, low = A.reverse ? last : row;
+      XT *to = reinterpret_cast<XT *>(A.dx) + (int64_t)last * A.channels + p.c;
+      GT *out = reinterpret_cast<GT *>(A.dgate) + (int64_t)last * A.gates + p.c;
+      float *sum_at = sums + (SHARED ? p.cy * kBatch * A.plan.tx + p.tx : 0);
+      const auto finish = [&](int k, bool inside) {  // row k, given what the row after it hands down
         float dg[V], sum = 0.f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float u = to_f32<XT>(dh[k].e[v]) + v_in[v];
-          dg[v] = u * before[k][v];
+          const float u = inside ? to_f32<XT>(dh[k].e[v]) + v_in[v] : 0.f;
+          dg[v] = inside ? u * before[k][v] : 0.f;
           sum += dg[v];
           before[k][v] = u;
-          v_in[v] = g[k](v) * u;
+          v_in[v] = inside ? g[k](v) * u : 0.f;
         }
-        store_pack<XT, V>(to + k * ts, before[k]);
-        if (SHARED) sums[(p.cy * kBatch + k) * A.plan.tx + p.tx] = sum;
-        else store_pack<GT, V>(out + k * os, dg);
+        store_pack<XT, V>(to, before[k]);
+        to -= ts;
+        if (SHARED) {
+          sum_at[k * A.plan.tx] = sum;
+        } else {
+          store_pack<GT, V>(out, dg);
+          out -= os;
+        }
       };
-      const int64_t low = A.reverse ? row - (n - 1) : row;  // the batch's rows of the tensor
-      if (!q.holds(low)) q.seek(A, low);
-      if (n == kBatch && plain_rows(q, low, kBatch)) {
+      if (n == kBatch && q.plain(low, kBatch)) {
 #pragma unroll
         for (int k = 0; k < kBatch; ++k)
 #pragma unroll
@@ -96,65 +101,74 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
             h[v] = fmaf(g[k](v), h[v], to_f32<XT>(x[k].e[v]));
           }
 #pragma unroll
-        for (int k = kBatch - 1; k >= 0; --k) finish(k);
+        for (int k = kBatch - 1; k >= 0; --k) finish(k, true);
       } else {
-        int state[kBatch];  // 4 * sequence + 2 * (its last row) + (its first row), or -1
+        // Bit k: row k is its sequence's first, its last, outside every sequence.
+        uint32_t firsts = 0, lasts = 0, outside = 0;
+        for (int k = 0; k < n;) {
+          const int at = row + k * one;
+          q.seek(A, at);
+          const int rest = q.rest(A, at), end = rest < n - k ? k + rest : n;
+          if (!q.holds(at)) {
+            outside |= (1u << end) - (1u << k);
+          } else {
+            if (q.first(A, at)) firsts |= 1u << k;
+            if (rest <= n - k) lasts |= 1u << (end - 1);
+          }
+          k = end;
+        }
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
           if (k >= n) break;
-          const int64_t at = A.reverse ? row - k : row + k;
-          if (!q.holds(at)) q.seek(A, at);
-          const bool low_end = at == q.lo, high_end = at == q.hi - 1;
-          state[k] = !q.holds(at) ? -1
-                                  : q.s * 4 + ((A.reverse ? low_end : high_end) ? 2 : 0) +
-                                        ((A.reverse ? high_end : low_end) ? 1 : 0);
-          if (state[k] >= 0 && (state[k] & 1)) load_state<V>(A.initial, A, q.s, p.c, h);
+          if (firsts >> k & 1) {
+            q.seek(A, row + k * one);
+            load_state<V>(A.initial, A, q.s, p.c, h);
+          }
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             before[k][v] = h[v];
-            h[v] = state[k] < 0 ? 0.f : fmaf(g[k](v), h[v], to_f32<XT>(x[k].e[v]));
+            h[v] = outside >> k & 1 ? 0.f : fmaf(g[k](v), h[v], to_f32<XT>(x[k].e[v]));
           }
         }
 #pragma unroll
         for (int k = kBatch - 1; k >= 0; --k) {
           if (k >= n) continue;
-          if (state[k] < 0) {
-            const float zero[V] = {};
-#pragma unroll
-            for (int v = 0; v < V; ++v) v_in[v] = 0.f;
-            store_pack<XT, V>(to + k * ts, zero);
-            if (SHARED) sums[(p.cy * kBatch + k) * A.plan.tx + p.tx] = 0.f;
-            else store_pack<GT, V>(out + k * os, zero);
-            continue;
+          if (lasts >> k & 1) {
+            q.seek(A, row + k * one);
+            load_state<V>(A.dfinal, A, q.s, p.c, v_in);
           }
-          if (state[k] & 2) load_state<V>(A.dfinal, A, state[k] >> 2, p.c, v_in);
-          finish(k);
-          if ((state[k] & 1) && A.dinitial != nullptr) store_state<V>(A.dinitial, A, state[k] >> 2, p.c, v_in);
+          finish(k, !(outside >> k & 1));
+          if ((firsts >> k & 1) && A.dinitial != nullptr) {
+            q.seek(A, row + k * one);
+            store_state<V>(A.dinitial, A, q.s, p.c, v_in);
+          }
         }
       }
     }
     if (SHARED) {
-      load(b - 1);
       // The sums of the threads that share a gate, in their order.
       __syncthreads();
       const int width = A.plan.tx * V, c0 = cblk * width, c1 = c0 + width < A.channels ? c0 + width : A.channels;
       const int first = c0 / A.per_gate, count = (c1 - 1) / A.per_gate - first + 1;
-      // A sum is shared out to as many adjacent lanes as there are threads for.
+      // kParts adjacent lanes share a sum.
       const int all = A.plan.cy * kBatch * count;
-      int parts = 1;
-      while (parts < 32 && parts * 2 * all <= kThreads) parts *= 2;
-      for (int j = threadIdx.x; j < (all * parts + 31) / 32 * 32; j += kThreads) {
-        const int k = j / parts, part = j % parts, line = k / count, at = first + k % count;
+      for (int j = threadIdx.x / kParts; j < (all + 7) / 8 * 8; j += kThreads / kParts) {
+        const int line = count == 1 ? j : j / count, at = first + (count == 1 ? 0 : j % count);
         const int lo = at * A.per_gate > c0 ? at * A.per_gate : c0;
         const int hi = (at + 1) * A.per_gate < c1 ? (at + 1) * A.per_gate : c1;
         float sum = 0.f;
-        if (k < all)
-          for (int c = lo + part * V; c < hi; c += parts * V) sum += sums[line * A.plan.tx + (c - c0) / V];
-        for (int d = parts / 2; d > 0; d /= 2) sum += __shfl_down_sync(0xffffffffu, sum, d);
+        if (j < all) {
+          const float *from = sums + line * A.plan.tx, *end = from + (hi - c0) / V;
+#pragma unroll 4
+          for (from += (lo - c0) / V + threadIdx.x % kParts; from < end; from += kParts) sum += *from;
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         const int64_t chunk = group * A.plan.cy + line / kBatch;
-        const int64_t r = chunk * A.plan.chunk + b * kBatch + line % kBatch;
-        if (part != 0 || k >= all || chunk >= A.plan.chunks || r >= A.rows ||
-            b * kBatch + line % kBatch >= A.plan.chunk)
+        const int in_chunk = b * kBatch + line % kBatch;
+        const int64_t r = chunk * A.plan.chunk + in_chunk;
+        if (threadIdx.x % kParts != 0 || j >= all || chunk >= A.plan.chunks || r >= A.rows ||
+            in_chunk >= A.plan.chunk)
           continue;
         const int64_t row = row_at(A, r);
         if (A.partial == nullptr) {
@@ -164,7 +178,6 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
           A.partial[((int64_t)slot * A.rows + row) * A.gates + at] = sum;
         }
       }
-      __syncthreads();
     }
   }
 }

@@ -155,11 +155,12 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
   const Place p =
       place_of<V, SHARED>(A, blockIdx.x / A.plan.channel_blocks, blockIdx.x % A.plan.channel_blocks);
   if (!p.on) return;
-  int64_t row = row_at(A, p.t0);
+  int row = (int)row_at(A, p.t0);
   const int64_t xs = along(A, A.x_stride), gs = along(A, A.gate_stride), hs = along(A, A.channels);
+  const int one = A.reverse ? -1 : 1;
   const XT *from = reinterpret_cast<const XT *>(A.x) + row * A.x_stride + p.c;
   const GT *gate = reinterpret_cast<const GT *>(A.gate) + row * A.gate_stride + p.g;
-  XT *to = reinterpret_cast<XT *>(A.h) + row * A.channels + p.c;
+  XT *to = reinterpret_cast<XT *>(A.h) + (int64_t)row * A.channels + p.c;
   Cursor q;
   q.s = A.hints != nullptr ? A.hints[p.chunk] : 0;
   q.seek(A, row);
@@ -168,46 +169,53 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
   for (int v = 0; v < V; ++v) h[v] = 0.f;
   if (A.carry != nullptr) load_kept<V>(A.carry, A, p.chunk, p.c, h);
   int64_t kept = p.chunk * A.plan.kept;
+  // Rows to the next event: the first row of a sequence, or of rows outside.
+  bool inside = q.holds(row);
+  int event = inside && q.first(A, row) || !inside ? 0 : q.rest(A, row);
   for (int left = (int)(p.t1 - p.t0); left > 0; left -= kBatch) {
     Pack<XT, V> x[kBatch];
     Gates<GT, V, SHARED> g[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k)
       if (k < left) {
-        x[k] = load_pack<XT, V>(from + k * xs);
-        g[k].load(gate + k * gs);
+        x[k] = load_pack<XT, V>(from);
+        g[k].load(gate);
+        from += xs;
+        gate += gs;
       }
     if (A.saved != nullptr) store_kept<V>(A.saved, A, kept++, p.c, h);
-    if (left >= kBatch && plain_rows(q, A.reverse ? row - (kBatch - 1) : row, kBatch)) {
+    if (inside && event > kBatch && left >= kBatch) {
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = fmaf(g[k](v), h[v], to_f32<XT>(x[k].e[v]));
-        store_pack<XT, V>(to + k * hs, h);
+        store_pack<XT, V>(to, h);
+        to += hs;
       }
     } else {
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
         if (k >= left) break;
-        const int64_t at = A.reverse ? row - k : row + k;
-        if (!q.holds(at)) q.seek(A, at);
-        if (!q.holds(at)) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) h[v] = 0.f;
-        } else {
-          if (at == (A.reverse ? q.hi - 1 : q.lo)) load_state<V>(A.initial, A, q.s, p.c, h);
-#pragma unroll
-          for (int v = 0; v < V; ++v) h[v] = fmaf(g[k](v), h[v], to_f32<XT>(x[k].e[v]));
-          if (at == (A.reverse ? q.lo : q.hi - 1) && A.final_state != nullptr)
-            store_state<V>(A.final_state, A, q.s, p.c, h);
+        if (k == event) {
+          const int at = row + k * one;
+          q.seek(A, at);
+          inside = q.holds(at);
+          event += q.rest(A, at);
+          if (inside) load_state<V>(A.initial, A, q.s, p.c, h);
         }
-        store_pack<XT, V>(to + k * hs, h);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          h[v] = fmaf(g[k](v), h[v], to_f32<XT>(x[k].e[v]));
+          if (!inside) h[v] = 0.f;
+        }
+        if (k + 1 == event && inside && A.final_state != nullptr)
+          store_state<V>(A.final_state, A, q.s, p.c, h);
+        store_pack<XT, V>(to, h);
+        to += hs;
       }
     }
-    row += A.reverse ? -kBatch : kBatch;
-    from += kBatch * xs;
-    gate += kBatch * gs;
-    to += kBatch * hs;
+    row += kBatch * one;
+    event -= kBatch;
   }
 }
 
