@@ -73,11 +73,13 @@ struct Args {
   void *h, *dx, *dgate;
   float *final_state, *dinitial;
   float *saved;      // (chunks, kept, channels): the state before each batch of rows
-  int *hints;        // (2, chunks): the sequence of each chunk's first and last logical row, or
-                     // near it; null: even sequences
+  int *hints;        // (chunks): the sequence of the row where the chain leaves each chunk; null:
+                     // no state passes between chunks, or even sequences
   float2 *maps;      // (chunks, channels)
   int *cuts;         // (chunks): nothing of the state before the chunk passes through it
   float *carry;      // (chunks, channels): the state that enters each chunk; null: none does
+  const float *empty_src;  // what leaves an empty sequence: copied to empty_dst, zeros where null
+  float *empty_dst;
   float *partial;    // (slots, rows, gates): gate gradients of channel blocks, or nullptr
   uint32_t *status;
 };
@@ -86,24 +88,19 @@ int type_bytes(int type);
 Plan make_plan(int64_t rows, int sequences, bool even, int channels, int gates, int x_type, int gate_type);
 int check_shape(int64_t rows, int sequences, int channels, int gates, int x_type, int gate_type, int even);
 bool suits(const void *p, int64_t stride, int bytes, int vec);
-// What every launch sequence begins with: hints, empty sequences, the check of
-// the offsets (src -> dst is what leaves an empty sequence).
-int launch_setup(const Args &A, const float *src, float *dst, cudaStream_t st);
 int launch_carry(const Args &A, bool back, cudaStream_t st);
 
 inline size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 inline size_t chain_bytes(const Plan &p, int channels) {
   const size_t n = (size_t)p.chunks, c = (size_t)channels;
-  size_t bytes = round16(n * 8);
-  if (!p.whole) bytes += round16(n * c * 8) + round16(n * 4) + round16(n * c * 4);
-  return bytes;
+  return p.whole ? 0 : round16(n * 4) + round16(n * c * 8) + round16(n * 4) + round16(n * c * 4);
 }
 inline void place_chain(Args &A, void *scratch) {
   const size_t n = (size_t)A.plan.chunks, c = (size_t)A.channels;
-  char *b = static_cast<char *>(scratch);
-  A.hints = reinterpret_cast<int *>(b);
   if (A.plan.whole) return;
-  b += round16(n * 8);
+  char *b = static_cast<char *>(scratch);
+  if (A.offsets != nullptr) A.hints = reinterpret_cast<int *>(b);
+  b += round16(n * 4);
   A.maps = reinterpret_cast<float2 *>(b);
   b += round16(n * c * 8);
   A.cuts = reinterpret_cast<int *>(b);
@@ -219,6 +216,38 @@ struct Cursor {
   __device__ __forceinline__ bool first(const Args &A, int p) const { return p == (A.reverse ? hi - 1 : lo); }
 };
 
+// The sequence where a chunk's walk begins, given whether it walks against the
+// logical rows: the one that the chain left the neighbouring chunk with, or the
+// outermost one.
+template <bool BACK>
+__device__ __forceinline__ int first_hint(const Args &A, int64_t chunk) {
+  const int64_t next = chunk + (BACK ? 1 : -1);
+  if (A.hints != nullptr && next >= 0 && next < A.plan.chunks) return A.hints[next];
+  return (A.reverse != 0) == BACK ? 0 : A.sequences - 1;
+}
+
+// Blocks behind those of the first launch's chunks: a warp for each sequence
+// copies what passes an empty one by and checks that the offsets ascend within
+// [0, rows].
+constexpr int kSequences = kThreads / 32;
+inline unsigned extra_blocks(const Args &A) {
+  return A.offsets == nullptr && A.rows > 0 ? 0u : (unsigned)((A.sequences + kSequences - 1) / kSequences);
+}
+__device__ __forceinline__ void look_at_sequences(const Args &A, int64_t block) {
+  const int64_t s = block * kSequences + threadIdx.x / 32;
+  if (s >= A.sequences) return;
+  const int64_t a = A.offsets != nullptr ? A.offsets[s] : 0, b = A.offsets != nullptr ? A.offsets[s + 1] : 0;
+  if (a == b && A.empty_dst != nullptr)
+    for (int c = (int)lane_id(); c < A.channels; c += 32)
+      A.empty_dst[s * A.channels + c] = A.empty_src != nullptr ? A.empty_src[s * A.channels + c] : 0.f;
+  if ((a < 0 || a > b || b > A.rows) && lane_id() == 0)
+    atomicCAS(A.status, 0u, (uint32_t)GS_ERR_INVALID_ARGUMENT);
+}
+
+inline unsigned grid_of(const Plan &p) {
+  return (unsigned)(((p.chunks + p.cy - 1) / p.cy) * p.channel_blocks);
+}
+
 // The place of a thread: its channels and its chunk's logical rows t0..t1-1.
 struct Place {
   int tx, cy, c, g;     // vector and chunk in the block, first channel and its gate
@@ -252,14 +281,27 @@ __device__ __forceinline__ int64_t along(const Args &A, int64_t stride) { return
 // first row along the chain where the chunk holds it (the chain is cut there).
 
 template <typename XT, typename GT, int V, bool SHARED, bool BACK>
-__global__ void __launch_bounds__(kThreads) maps_kernel(const __grid_constant__ Args A) {
+__global__ void __launch_bounds__(kThreads) maps_kernel(const __grid_constant__ Args A, unsigned blocks) {
+  if (blockIdx.x >= blocks) {
+    look_at_sequences(A, blockIdx.x - blocks);
+    return;
+  }
   const int cblk = blockIdx.x % A.plan.channel_blocks;
   const Place p = place_of<V, SHARED>(A, blockIdx.x / A.plan.channel_blocks, cblk);
   if (!p.on) return;
   const int64_t t_end = BACK ? p.t0 : p.t1 - 1;  // the chunk's last row along the chain
   const int row_end = (int)row_at(A, t_end);
   Cursor q;
-  q.s = A.hints != nullptr ? A.hints[p.chunk + (BACK ? 0 : A.plan.chunks)] : 0;
+  q.s = 0;
+  if (A.offsets != nullptr) {  // the first sequence that ends behind the row, or the last
+    int hi = A.sequences - 1;
+    while (q.s < hi) {
+      const int mid = q.s + (hi - q.s) / 2;
+      if (A.offsets[mid + 1] <= row_end) q.s = mid + 1;
+      else hi = mid;
+    }
+    if (cblk == 0 && p.tx == 0) A.hints[p.chunk] = q.s;
+  }
   q.seek(A, row_end);
   // Rows of the tensor run up along the chain, or down.
   const bool up = (A.reverse != 0) == BACK;
@@ -311,10 +353,6 @@ __global__ void __launch_bounds__(kThreads) maps_kernel(const __grid_constant__ 
 #pragma unroll
   for (int v = 0; v < V; ++v) A.maps[p.chunk * A.channels + p.c + v] = make_float2(P[v], L[v]);
   if (cblk == 0 && p.tx == 0) A.cuts[p.chunk] = cut;
-}
-
-inline unsigned grid_of(const Plan &p) {
-  return (unsigned)(((p.chunks + p.cy - 1) / p.cy) * p.channel_blocks);
 }
 
 }  // namespace scan

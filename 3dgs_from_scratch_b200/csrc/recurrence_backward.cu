@@ -20,7 +20,11 @@ namespace scan {
 constexpr int kParts = 4;  // threads that share a sum over a gate's channels
 
 template <typename XT, typename GT, int V, bool SHARED>
-__global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constant__ Args A) {
+__global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constant__ Args A, unsigned blocks) {
+  if (blockIdx.x >= blocks) {
+    look_at_sequences(A, blockIdx.x - blocks);
+    return;
+  }
   // [chunk of the block][row][vector], batches in turn: a batch's sums are read
   // while the next one's are written, with one barrier between.
   __shared__ float both[2][SHARED ? kThreads * kBatch : 1];
@@ -31,7 +35,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
   const int64_t xs = along(A, A.x_stride), gs = along(A, A.gate_stride), ds = along(A, A.dh_stride);
   const int64_t ts = along(A, A.channels), os = along(A, A.gates);
   Cursor q;
-  q.s = A.hints != nullptr && p.on ? A.hints[p.chunk + A.plan.chunks] : 0;
+  q.s = first_hint<true>(A, p.chunk);
   q.lo = q.hi = 0;
   const int one = A.reverse ? -1 : 1;
   float v_in[V];  // what the row after hands down
@@ -198,15 +202,16 @@ __global__ void __launch_bounds__(kThreads) join_gates_kernel(const __grid_const
 
 template <typename XT, typename GT, int V, bool SHARED>
 static int launch_backward(const Args &A, cudaStream_t st) {
+  const unsigned blocks = grid_of(A.plan), extra = extra_blocks(A);
   if (A.carry != nullptr) {
-    maps_kernel<XT, GT, V, SHARED, true><<<grid_of(A.plan), kThreads, 0, st>>>(A);
+    maps_kernel<XT, GT, V, SHARED, true><<<blocks + extra, kThreads, 0, st>>>(A, blocks);
     count_launch();
     const int rc = launch_carry(A, true, st);
     if (rc) return rc;
   }
-  backward_kernel<XT, GT, V, SHARED><<<grid_of(A.plan), kThreads, 0, st>>>(A);
+  backward_kernel<XT, GT, V, SHARED><<<blocks + (A.carry == nullptr ? extra : 0), kThreads, 0, st>>>(A, blocks);
   count_launch();
-  if (A.partial != nullptr) {
+  if (A.partial != nullptr && A.rows > 0) {
     const int64_t want = (A.rows * A.gates + kThreads - 1) / kThreads;
     join_gates_kernel<GT><<<(unsigned)(want < 1184 ? want : 1184), kThreads, 0, st>>>(A);
     count_launch();
@@ -282,15 +287,14 @@ extern "C" int gs_gated_scan_backward(int64_t rows, int sequences, int channels,
     if (scratch == nullptr || ((uintptr_t)scratch & 15)) return GS_ERR_INVALID_ARGUMENT;
     if (scratch_bytes < need) return GS_ERR_CAPACITY;
     place_chain(A, scratch);
-    if (even) A.hints = nullptr;
     if (A.plan.slots > 1)
       A.partial = reinterpret_cast<float *>(static_cast<char *>(scratch) + chain_bytes(A.plan, channels));
   }
   A.status = device_status_word();
   if (A.status == nullptr) return GS_ERR_CUDA;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  rc = launch_setup(A, grad_final, grad_initial, st);
-  if (rc || rows == 0) return rc;
+  A.empty_src = grad_final;
+  A.empty_dst = grad_initial;
   const bool same = x_type == gate_type;
   if (x_type == GS_TYPE_F32) return pick_backward<float, float>(A, st);
   if (x_type == GS_TYPE_BF16)

@@ -46,44 +46,6 @@ Plan make_plan(int64_t rows, int sequences, bool even, int channels, int gates, 
   return p;
 }
 
-// A warp for each sequence, then a thread for each end of a chunk.
-__global__ void __launch_bounds__(kThreads) setup_kernel(const __grid_constant__ Args A,
-                                                         const float *__restrict__ src,
-                                                         float *__restrict__ dst) {
-  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  const int64_t s = at / 32;
-  if (s < A.sequences) {
-    const int64_t a = A.offsets != nullptr ? A.offsets[s] : s * A.period;
-    const int64_t b = A.offsets != nullptr ? A.offsets[s + 1] : (s + 1) * A.period;
-    if (a == b && dst != nullptr)
-      for (int c = (int)lane_id(); c < A.channels; c += 32)
-        dst[s * A.channels + c] = src != nullptr ? src[s * A.channels + c] : 0.f;
-    if ((a < 0 || a > b || b > A.rows) && lane_id() == 0)
-      atomicCAS(A.status, 0u, (uint32_t)GS_ERR_INVALID_ARGUMENT);
-    return;
-  }
-  const int64_t k = at - (int64_t)A.sequences * 32;
-  if (A.offsets == nullptr || k >= 2 * A.plan.chunks) return;
-  int64_t t = k * A.plan.chunk;  // the first row of chunk k, then the last one of k - chunks
-  if (k >= A.plan.chunks) t = (k - A.plan.chunks + 1) * A.plan.chunk - 1;
-  const int64_t p = row_at(A, t < A.rows ? t : A.rows - 1);
-  int lo = 0, hi = A.sequences - 1;  // the first sequence that ends behind p, or the last
-  while (lo < hi) {
-    const int mid = lo + (hi - lo) / 2;
-    if ((int64_t)A.offsets[mid + 1] <= p) lo = mid + 1;
-    else hi = mid;
-  }
-  A.hints[k] = lo;
-}
-
-int launch_setup(const Args &A, const float *src, float *dst, cudaStream_t st) {
-  if (A.offsets == nullptr && A.rows > 0) return GS_OK;  // even sequences, none empty
-  const int64_t threads = (int64_t)A.sequences * 32 + (A.offsets != nullptr ? 2 * A.plan.chunks : 0);
-  setup_kernel<<<(unsigned)((threads + kThreads - 1) / kThreads), kThreads, 0, st>>>(A, src, dst);
-  count_launch();
-  return launch_status();
-}
-
 // The state that enters each chunk, from the chunks' maps: 8 channels a block,
 // 128 threads a channel with a run of chunks each; the runs' maps are scanned in
 // shared memory, then each thread goes through its run once more from the state
@@ -151,7 +113,11 @@ int launch_carry(const Args &A, bool back, cudaStream_t st) {
 }
 
 template <typename XT, typename GT, int V, bool SHARED>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant__ Args A) {
+__global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant__ Args A, unsigned blocks) {
+  if (blockIdx.x >= blocks) {
+    look_at_sequences(A, blockIdx.x - blocks);
+    return;
+  }
   const Place p =
       place_of<V, SHARED>(A, blockIdx.x / A.plan.channel_blocks, blockIdx.x % A.plan.channel_blocks);
   if (!p.on) return;
@@ -162,7 +128,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
   const GT *gate = reinterpret_cast<const GT *>(A.gate) + row * A.gate_stride + p.g;
   XT *to = reinterpret_cast<XT *>(A.h) + (int64_t)row * A.channels + p.c;
   Cursor q;
-  q.s = A.hints != nullptr ? A.hints[p.chunk] : 0;
+  q.s = first_hint<false>(A, p.chunk);
   q.seek(A, row);
   float h[V];
 #pragma unroll
@@ -221,13 +187,14 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
 
 template <typename XT, typename GT, int V, bool SHARED>
 static int launch_forward(const Args &A, cudaStream_t st) {
+  const unsigned blocks = grid_of(A.plan), extra = extra_blocks(A);
   if (A.carry != nullptr) {
-    maps_kernel<XT, GT, V, SHARED, false><<<grid_of(A.plan), kThreads, 0, st>>>(A);
+    maps_kernel<XT, GT, V, SHARED, false><<<blocks + extra, kThreads, 0, st>>>(A, blocks);
     count_launch();
     const int rc = launch_carry(A, false, st);
     if (rc) return rc;
   }
-  forward_kernel<XT, GT, V, SHARED><<<grid_of(A.plan), kThreads, 0, st>>>(A);
+  forward_kernel<XT, GT, V, SHARED><<<blocks + (A.carry == nullptr ? extra : 0), kThreads, 0, st>>>(A, blocks);
   count_launch();
   return launch_status();
 }
@@ -249,7 +216,7 @@ int check_shape(int64_t rows, int sequences, int channels, int gates, int x_type
     return GS_ERR_INVALID_ARGUMENT;
   if (even && rows % sequences != 0) return GS_ERR_INVALID_ARGUMENT;
   const Plan p = make_plan(rows, sequences, even, channels, gates, x_type, gate_type);
-  if ((p.chunks / p.cy + 1) * p.channel_blocks > INT32_MAX) return GS_ERR_CAPACITY;
+  if ((p.chunks / p.cy + 1) * p.channel_blocks > INT32_MAX / 2) return GS_ERR_CAPACITY;
   return GS_OK;
 }
 
@@ -275,7 +242,6 @@ extern "C" size_t gs_gated_scan_scratch_bytes(int64_t rows, int sequences, int e
                                               int x_type, int gate_type, int backward) {
   if (check_shape(rows, sequences, channels, gates, x_type, gate_type, even)) return 0;
   const Plan p = make_plan(rows, sequences, even, channels, gates, x_type, gate_type);
-  if (even && p.whole && (!backward || p.slots == 1)) return 0;
   size_t bytes = chain_bytes(p, channels);
   if (backward && p.slots > 1) bytes += (size_t)p.slots * rows * gates * 4;
   return bytes;
@@ -321,13 +287,12 @@ extern "C" int gs_gated_scan_forward(int64_t rows, int sequences, int channels, 
     if (scratch == nullptr || ((uintptr_t)scratch & 15)) return GS_ERR_INVALID_ARGUMENT;
     if (scratch_bytes < need) return GS_ERR_CAPACITY;
     place_chain(A, scratch);
-    if (even) A.hints = nullptr;
   }
   A.status = device_status_word();
   if (A.status == nullptr) return GS_ERR_CUDA;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  rc = launch_setup(A, initial, final_state, st);
-  if (rc || rows == 0) return rc;
+  A.empty_src = initial;
+  A.empty_dst = final_state;
   const bool same = x_type == gate_type;
   if (x_type == GS_TYPE_F32) return pick_forward<float, float>(A, st);
   if (x_type == GS_TYPE_BF16)
