@@ -35,7 +35,6 @@
 // Padding to whole blocks is zero from the start and stays zero.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cstdlib>
 #include <type_traits>
 
 #include "tcgen05.cuh"
@@ -1094,24 +1093,37 @@ static SmallPlan small_plan(int m, int n) {
   return {128, n <= 512 ? 4 : 8};
 }
 
-// What a step costs in tiles of 128 ctas x bn, in microseconds: rounds of
-// tiles, each its K blocks at the slower of the copies (the L2 hands an SM
-// about 60 bytes a nanosecond) and the MMAs, and a constant for filling and
-// draining.
-static double cost_of(int batch, int m, int n, bool full, int bn, int ctas) {
-  const int tri = bn > 128 * ctas ? bn : 128 * ctas, rows = 128 * ctas;
-  const int sq = (m + tri - 1) / tri, per = tri / rows;  // superblocks, rows of tiles in one
-  const int64_t half = (int64_t)(sq * (sq + 1) / 2) * per * (tri / bn);
-  const int64_t whole = (int64_t)sq * per * ((n + bn - 1) / bn);
-  const int at_once = 148 / ctas, kn = (n + 63) / 64, km = (m + 63) / 64;
-  const auto block = [&](int planes_a, int planes_b, int products) {
-    const double copy = (planes_a * 128 + planes_b * (bn / ctas)) * 128 / 60e3;
-    const double mma = products * 4 * (bn == 64 ? 48 : bn / 2) / 1.7e3;
-    return copy > mma ? copy : mma;
+// What a step costs in tiles of 128 ctas x bn, in microseconds: each of its three
+// products a constant for filling, draining and the launch, and rounds of tiles
+// at so much a K block, both fitted to measurements between 256 x 256 and
+// 4096 x 4096. Small tiles start and end sooner and fill the device with small
+// matrices (512 x 512 fp32: 135 us a call in 128 x 64 tiles, 162 in pairs of
+// 128 x 128, 260 in pairs of 128 x 256), large ones read less through the L2
+// (4096 x 4096 bf16: 3.36, 2.01 and 1.54 ms). Full products gain nothing from the
+// largest (4096 x 4096 fp32: 3.31 ms against 3.20 in pairs of 128 x 128, which
+// also have room for the second accumulator).
+struct TileShape {
+  int bn, ctas;
+  double fixed_full, block_full;              // fp32 and fp16 results
+  double fixed_half, syrk_half, apply_half;   // bf16 results: A and A A, a X + B X
+};
+constexpr TileShape kShapes[] = {{64, 1, 5.0, 0.55, 4.1, 0.33, 0.38},
+                                 {128, 1, 6.2, 0.75, 4.2, 0.40, 0.47},
+                                 {128, 2, 6.4, 0.60, 4.9, 0.39, 0.45},
+                                 {256, 2, 0.0, 0.0, 7.1, 0.48, 0.72}};  // half only
+
+static double cost_of(int batch, int m, int n, bool full, const TileShape &t) {
+  const int rows = 128 * t.ctas, tri = t.bn > rows ? t.bn : rows;
+  const int64_t sq = (m + tri - 1) / tri, per = tri / rows;  // superblocks, rows of tiles in one
+  const int64_t half = sq * (sq + 1) / 2 * per * (tri / t.bn);
+  const int64_t whole = sq * per * ((n + t.bn - 1) / t.bn);
+  const int kn = (n + 63) / 64, km = (m + 63) / 64;
+  const auto product = [&](int64_t tiles, int k, double block) {
+    const double rounds = (double)((tiles * batch * t.ctas + 147) / 148);
+    return (full ? t.fixed_full : t.fixed_half) + rounds * (k * block + 1.0);
   };
-  const auto rounds = [&](int64_t tiles) { return (double)((tiles * batch + at_once - 1) / at_once); };
-  const double syrk = block(full ? 2 : 1, full ? 2 : 1, full ? 3 : 1), apply = block(full ? 2 : 1, 2, full ? 3 : 2);
-  return rounds(half) * (2.0 + kn * syrk) + rounds(half) * (2.0 + km * syrk) + rounds(whole) * (2.0 + km * apply);
+  const double syrk = full ? t.block_full : t.syrk_half, apply = full ? t.block_full : t.apply_half;
+  return product(half, kn, syrk) + product(half, km, syrk) + product(whole, km, apply);
 }
 
 static Plan make_plan(int batch, int rows, int cols, int type) {
@@ -1119,15 +1131,13 @@ static Plan make_plan(int batch, int rows, int cols, int type) {
   p.m = rows < cols ? rows : cols;
   p.n = rows < cols ? cols : rows;
   p.full = type != GS_TYPE_BF16;
-  const char *force = getenv("NS_FORCE");
   double best = 0.0;
   p.bn = 0;
-  const int shapes[4][2] = {{64, 1}, {128, 1}, {128, 2}, {256, 2}};
-  for (const auto &q : shapes) {
-    const double cost = cost_of(batch, p.m, p.n, p.full, q[0], q[1]);
-    if (p.bn == 0 || cost < best) best = cost, p.bn = q[0], p.ctas = q[1];
+  for (const TileShape &t : kShapes) {
+    if (p.full && t.bn == 256) continue;
+    const double cost = cost_of(batch, p.m, p.n, p.full, t);
+    if (p.bn == 0 || cost < best) best = cost, p.bn = t.bn, p.ctas = t.ctas;
   }
-  if (force) { p.bn = atoi(force) / 10; p.ctas = atoi(force) % 10; }
   const int tri = p.bn > 128 * p.ctas ? p.bn : 128 * p.ctas;
   const int mp = (p.m + tri - 1) / tri * tri, np = (p.n + p.bn - 1) / p.bn * p.bn;
   p.row_blocks = mp / 128;
@@ -1313,8 +1323,7 @@ static int run(int batch, const Plan &p, const Source &src, const Out &out, int 
   if (rc) return rc;
   count_launch(2);
   if (p.full)
-    return p.bn == 256   ? run_steps<256, true, 2>(A, p, batch, steps, out, st)
-           : p.bn == 128 && p.ctas == 2 ? run_steps<128, true, 2>(A, p, batch, steps, out, st)
+    return p.bn == 128 && p.ctas == 2 ? run_steps<128, true, 2>(A, p, batch, steps, out, st)
            : p.bn == 128 ? run_steps<128, true, 1>(A, p, batch, steps, out, st)
                          : run_steps<64, true, 1>(A, p, batch, steps, out, st);
   return p.bn == 256   ? run_steps<256, false, 2>(A, p, batch, steps, out, st)
