@@ -95,10 +95,9 @@ __device__ __forceinline__ int chunk_at(int r, int col) {
 // One plane's rows of an operand: `rows` rows from `row` on, K block kb, into
 // shared memory. Above or on the diagonal (of blocks of `tri`) of a symmetric
 // matrix, and always for X, as K-major rows; below it as the mirror image,
-// MN-major. Returns the bytes that will arrive.
-__device__ __forceinline__ uint32_t fetch_rows(char *plane, const Matrix &M, int batch, int row,
-                                               int rows, int kb, bool mirrored, char *dst,
-                                               uint64_t *bar) {
+// MN-major.
+__device__ __forceinline__ void fetch_rows(char *plane, const Matrix &M, int batch, int row, int rows,
+                                           int kb, bool mirrored, char *dst, uint64_t *bar) {
   if (!mirrored) {
     if (rows < 128) {
       bulk_load(dst, block_at(plane, M, batch, row / 128, kb) + (row % 128) * 128, rows * 128, bar);
@@ -112,7 +111,6 @@ __device__ __forceinline__ uint32_t fetch_rows(char *plane, const Matrix &M, int
                 block_at(plane, M, batch, kb / 2, row / 64 + u) + (kb & 1) * (kBlockBytes / 2),
                 kBlockBytes / 2, bar);
   }
-  return rows * 128;
 }
 
 // An operand's descriptor, and what 16 elements of K further add to it: 32
@@ -1280,6 +1278,7 @@ static int run(int batch, const Plan &p, const Source &src, const Out &out, int 
                float c, float eps, void *scratch, size_t scratch_bytes, cudaStream_t st) {
   if (scratch == nullptr || ((uintptr_t)scratch & 15)) return GS_ERR_INVALID_ARGUMENT;
   if (scratch_bytes < p.total) return GS_ERR_CAPACITY;
+  if ((int64_t)p.row_blocks * p.column_blocks * batch > INT32_MAX / 2) return GS_ERR_CAPACITY;
   Args A{};
   A.status = device_status_word();
   if (A.status == nullptr) return GS_ERR_CUDA;

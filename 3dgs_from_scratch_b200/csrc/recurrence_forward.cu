@@ -211,7 +211,7 @@ static int pick_forward(const Args &A, cudaStream_t st) {
 // What both directions check of their sizes and types.
 int check_shape(int64_t rows, int sequences, int channels, int gates, int x_type, int gate_type, int even) {
   if (rows < 0 || rows > INT32_MAX || sequences < 1 || sequences > (1 << 28) || channels < 1 ||
-      gates < 1 || channels % gates != 0 || !type_bytes(x_type) ||
+      channels > (1 << 30) || gates < 1 || channels % gates != 0 || !type_bytes(x_type) ||
       (gate_type != x_type && gate_type != GS_TYPE_F32))
     return GS_ERR_INVALID_ARGUMENT;
   if (even && rows % sequences != 0) return GS_ERR_INVALID_ARGUMENT;

@@ -306,6 +306,69 @@ def test_the_same_bits_every_time_and_from_a_graph(gs):
 
 
 @gpu
+def test_calls_side_by_side_on_their_own_streams(gs):
+    gen = torch.Generator(device=DEV).manual_seed(8)
+    x = torch.randn(3, 4000, 24, generator=gen, device=DEV)
+    g = torch.rand(3, 4000, 24, generator=gen, device=DEV)
+    ref = gs.gated_scan(x, g)
+    torch.cuda.synchronize()
+    got = []
+    for s in [torch.cuda.Stream() for _ in range(4)]:
+        with torch.cuda.stream(s):
+            got.append(gs.gated_scan(x, g))
+    torch.cuda.synchronize()
+    assert all(torch.equal(h, ref[0]) and torch.equal(f, ref[1]) for h, f in got)
+
+
+@gpu
+def test_a_first_call_inside_a_capture(gs):
+    x = torch.randn(2, 3000, 20, device=DEV)
+    g = torch.rand(2, 3000, 4, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h, final = gs.gated_scan(x, g, reverse=True)
+    graph.replay()
+    torch.cuda.synchronize()
+    again = gs.gated_scan(x, g, reverse=True)
+    assert torch.equal(h, again[0]) and torch.equal(final, again[1])
+
+
+@gpu
+def test_twice_differentiated_is_refused(gs):
+    x = torch.randn(2, 9, 4, device=DEV, requires_grad=True)
+    h, _ = gs.gated_scan(x, torch.rand(2, 9, 4, device=DEV, requires_grad=True))
+    (dx,) = torch.autograd.grad(h.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize("reverse", [False, True])
+def test_more_than_2_31_elements(gs, reverse):
+    rows, channels, tail = 1 << 21, 1100, 50           # 2.3e9 elements
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    x = torch.zeros(rows, channels, dtype=BF16, device=DEV)
+    g = torch.rand(rows, 1, generator=gen, device=DEV)
+    ends = slice(0, tail) if reverse else slice(rows - tail, rows)  # what the chain reaches last
+    x[ends] = torch.randn(tail, channels, generator=gen, device=DEV).to(BF16)
+    small_x, small_g = x[ends].clone().requires_grad_(True), g[ends].clone().requires_grad_(True)
+    h0, f0 = gs.gated_scan(small_x, small_g, reverse=reverse)
+    up = torch.randn(tail, channels, generator=gen, device=DEV).to(BF16)
+    d0 = torch.autograd.grad(h0, (small_x, small_g), up)
+    x.requires_grad_(True), g.requires_grad_(True)
+    h, final = gs.gated_scan(x, g, reverse=reverse)
+    full = torch.zeros_like(h)
+    full[ends] = up
+    d = torch.autograd.grad(h, (x, g), full)
+    # the same rows in the same order of batches or another: fp32 sums of at most 50 rows
+    near = lambda a, b, t: torch.allclose(a.float(), b.float(), rtol=torch.finfo(t).eps, atol=1e-3)  # noqa: E731
+    assert near(h[ends], h0, BF16) and near(final, f0, F32) and near(d[0][ends], d0[0], BF16)
+    assert near(d[1][ends], d0[1], F32)
+    other = slice(tail, tail + 1000) if reverse else slice(rows - tail - 1000, rows - tail)
+    assert float(h.detach()[other].abs().max()) == 0.0
+
+
+@gpu
 def test_offsets_that_do_not_ascend_are_reported(gs):
     """The kernels index within the buffers whatever the offsets hold (checked by reading: a
     sequence number is below the count, a row below rows); the fault is in the status word."""
@@ -367,7 +430,7 @@ def test_entry_points_refuse_bad_arguments(gs):
         return lib.gs_gated_scan_forward(rows, seqs, channels, gates, xt, gt, x, xs, gate, gst, init,
                                          offs, 0, h, P, P, scratch, nbytes, P)
 
-    for kw in (dict(rows=-1), dict(rows=2 ** 31), dict(seqs=0), dict(seqs=3), dict(channels=0), dict(gates=0),
+    for kw in (dict(rows=-1), dict(rows=2 ** 31), dict(seqs=0), dict(seqs=3), dict(channels=0), dict(channels=(1 << 30) + 8), dict(gates=0),
                dict(gates=3), dict(xt=3), dict(xt=1, gt=2), dict(xt=0, gt=1), dict(x=P), dict(gate=P),
                dict(h=P), dict(x=at + 4), dict(xs=9), dict(gst=11), dict(h=at + 4), dict(init=at + 2),
                dict(offs=at + 2), dict(rows=2 ** 20)):       # many tiles and no scratch
