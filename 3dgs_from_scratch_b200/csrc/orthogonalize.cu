@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(Shape<BN, KIND, FULL, CTAS>::kThreads, 1)
   __shared__ uint64_t full[kMaxStages], peer[kMaxStages], empty[kMaxStages], ready[2], drained[2];
   __shared__ uint32_t tmem_base, failed;
   const int warp = threadIdx.x / 32;
-  const int rank = CTAS == 2 ? (int)tc::cluster_rank() : 0;
+  const int rank = CTAS == 2 ? (int)cluster_rank() : 0;
   const int k_blocks = KIND == kGram ? A.k_blocks_n : A.k_blocks_m;
   const int chunks = (k_blocks + S::kChunk - 1) / S::kChunk;
   const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS, total = A.tiles * A.batches;
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(Shape<BN, KIND, FULL, CTAS>::kThreads, 1)
   if (warp == 1) tc::tmem_alloc<CTAS>(&tmem_base, S::kColumns);
   tc::fence_before();
   __syncthreads();
-  if (CTAS == 2) tc::cluster_sync();
+  if (CTAS == 2) cluster_sync();
   tc::fence_after();
   const uint32_t tmem = tmem_base;
   start_next();
@@ -523,7 +523,7 @@ __global__ void __launch_bounds__(Shape<BN, KIND, FULL, CTAS>::kThreads, 1)
   __syncwarp();
   tc::fence_before();
   __syncthreads();
-  if (CTAS == 2) tc::cluster_sync();  // neither block leaves while the other may reach into it
+  if (CTAS == 2) cluster_sync();  // neither block leaves while the other may reach into it
   if (threadIdx.x == 0 && failed) atomicCAS(A.status, 0u, (uint32_t)GS_ERR_DEVICE_TIMEOUT);
   if (warp == 1) {
     tc::fence_after();
@@ -830,7 +830,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
   __shared__ uint32_t tmem_base, failed;
   __shared__ double warp_sums[kSmallThreads / 32], block_sum;
   const int warp = threadIdx.x / 32, lane = (int)lane_id();
-  const int C = A.cluster, rank = C > 1 ? (int)tc::cluster_rank() : 0, batch = blockIdx.x / C;
+  const int C = A.cluster, rank = C > 1 ? (int)cluster_rank() : 0, batch = blockIdx.x / C;
   const int col_base = rank * NC;  // of X
   const Source &s = A.src;
   if (threadIdx.x == 0) {
@@ -896,8 +896,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
   }
   double total = 0.0;
   if (C > 1) {
-    tc::cluster_sync();
-    for (int k = 0; k < C; ++k) total += tc::cluster_load_f64(tc::cluster_addr(&block_sum, k));
+    cluster_sync();
+    for (int k = 0; k < C; ++k) total += cluster_load_f64(cluster_addr(&block_sum, k));
   } else {
     __syncthreads();
     total = block_sum;
@@ -981,7 +981,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
       }
     }
     if (S::kPart > 0 && C > 1) {
-      tc::cluster_sync();
+      cluster_sync();
       const int rows = MC / C;
       for (int k = threadIdx.x; k < rows * (MC / 8); k += kSmallThreads) {
         const int row = rank * rows + k / (MC / 8), c = k % (MC / 8) * 8;
@@ -989,9 +989,9 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
 #pragma unroll
         for (int q = 0; q < 8; ++q)
           if (q < C) {
-            const uint32_t from = tc::cluster_addr(part, q) + row * (MC * 4);
-            f[q] = tc::cluster_load(from + (((c / 4) ^ (row & (MC / 4 - 1))) << 4));
-            g[q] = tc::cluster_load(from + (((c / 4 + 1) ^ (row & (MC / 4 - 1))) << 4));
+            const uint32_t from = cluster_addr(part, q) + row * (MC * 4);
+            f[q] = cluster_load(from + (((c / 4) ^ (row & (MC / 4 - 1))) << 4));
+            g[q] = cluster_load(from + (((c / 4 + 1) ^ (row & (MC / 4 - 1))) << 4));
           }
         float w[8] = {};
 #pragma unroll
@@ -1008,13 +1008,13 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
 #pragma unroll
         for (int q = 0; q < 8; ++q)
           if (q < C) {
-            tc::cluster_store(tc::cluster_addr(sq_hi + to, q), hi);
-            tc::cluster_store(tc::cluster_addr(sq_lo + to, q), lo);
+            cluster_store(cluster_addr(sq_hi + to, q), hi);
+            cluster_store(cluster_addr(sq_lo + to, q), lo);
           }
       }
       asm volatile("fence.proxy.async;" ::: "memory");
       __syncwarp();
-      tc::cluster_sync();
+      cluster_sync();
     }
     run([&] {
       small_product<MC, false>(tmem, cross, smem_addr(sq_hi), smem_addr(sq_lo), smem_addr(sq_hi),
@@ -1060,7 +1060,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
   }
   tc::fence_before();
   __syncthreads();
-  if (C > 1) tc::cluster_sync();  // no block leaves while another may reach into it
+  if (C > 1) cluster_sync();  // no block leaves while another may reach into it
   if (threadIdx.x == 0 && failed) atomicCAS(A.status, 0u, (uint32_t)GS_ERR_DEVICE_TIMEOUT);
   if (warp == 0) {
     tc::fence_after();

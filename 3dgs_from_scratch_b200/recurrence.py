@@ -97,7 +97,7 @@ def _states(t):
 
 def _forward(x, gate, initial, offsets, reverse, sequences, keep):
     dev, channels, gates = x.device, x.shape[-1], gate.shape[-1]
-    h = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    h = torch.empty_like(x, memory_format=torch.contiguous_format)
     final = torch.empty((sequences, channels), dtype=torch.float32, device=dev)
     rows = x.numel() // channels
     if rows == 0 or sequences == 0:
@@ -124,8 +124,8 @@ def _backward(ctx, grad_h, grad_final):
     x, gate, initial, offs, saved = ctx.saved_tensors
     dev, channels, gates, sequences = x.device, x.shape[-1], gate.shape[-1], ctx.sequences
     want = initial is not None and ctx.needs_input_grad[2]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dgate = torch.empty_like(gate, memory_format=torch.contiguous_format)
     dfinal = _states(grad_final)
     rows = x.numel() // channels
     if sequences == 0 or rows == 0:
