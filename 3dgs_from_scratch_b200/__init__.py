@@ -5,6 +5,10 @@ three autograd Functions mirror src/cuda/wrapper.py, `cuda_rasterizer`
 mirrors the reference's native module, and every computation runs in the
 hand-written sm_100a kernels of lib3dgs_b200.so (C ABI: include/gs_b200.h).
 
+`gated_scan` (a gated linear recurrence with its gradients), `orthogonalize`
+and `muon_step` (orthogonalised matrix updates) serve scenes that carry
+learned state next to the Gaussians.
+
 The package directory name starts with a digit, so import it with
 importlib.import_module("3dgs_from_scratch_b200").
 """

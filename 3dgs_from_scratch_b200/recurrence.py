@@ -78,10 +78,17 @@ def _check(x, gate, initial, offsets):
     return sequences
 
 
-def _work(name, sizes, dev, *more):
-    """Scratch of a size query (None, 0 where there is none)."""
+def _work(name, sizes, like, *more):
+    """Memory of a size query (None, 0 where there is none), on `like`'s device."""
     nbytes = nat.size_query(name, *sizes, *more)
-    return (torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None), nbytes
+    return (like.new_empty(-(-nbytes // like.element_size())) if nbytes else None), nbytes
+
+
+def _states_like(initial, shape, like):
+    """An empty tensor of one fp32 state a sequence."""
+    if initial is not None and initial.dtype == torch.float32:
+        return torch.empty_like(initial, memory_format=torch.contiguous_format)
+    return like.new_empty(shape, dtype=torch.float32)
 
 
 def _ptr(t):
@@ -98,7 +105,7 @@ def _states(t):
 def _forward(x, gate, initial, offsets, reverse, sequences, keep):
     dev, channels, gates = x.device, x.shape[-1], gate.shape[-1]
     h = torch.empty_like(x, memory_format=torch.contiguous_format)
-    final = torch.empty((sequences, channels), dtype=torch.float32, device=dev)
+    final = _states_like(initial, (sequences, channels), x)
     rows = x.numel() // channels
     if rows == 0 or sequences == 0:
         final.zero_() if initial is None else final.copy_(initial)
@@ -110,8 +117,8 @@ def _forward(x, gate, initial, offsets, reverse, sequences, keep):
             offs = offs.clamp(-1, 2 ** 31 - 1).to(torch.int32)
         offs = offs.contiguous()
     sizes = (rows, sequences, int(offs is None), channels, gates, _TYPES[x.dtype], _TYPES[gate.dtype])
-    saved = _work("gs_gated_scan_saved_bytes", sizes, dev)[0] if keep else None
-    scratch, nbytes = _work("gs_gated_scan_scratch_bytes", sizes, dev, 0)
+    saved = _work("gs_gated_scan_saved_bytes", sizes, h)[0] if keep else None
+    scratch, nbytes = _work("gs_gated_scan_scratch_bytes", sizes, h, 0)
     with on_device(dev):
         nat.call("gs_gated_scan_forward", rows, sequences, channels, gates, sizes[5], sizes[6],
                  xr.data_ptr(), x_step, gr.data_ptr(), g_step, _ptr(init), _ptr(offs), int(reverse),
@@ -136,9 +143,9 @@ def _backward(ctx, grad_h, grad_final):
     (xr, x_step), (gr, g_step) = _rows_of(x, channels), _rows_of(gate, gates)
     dh, dh_step = (None, channels) if grad_h is None else _rows_of(grad_h, channels)
     init = _states(initial)
-    dinit = torch.empty((sequences, channels), dtype=torch.float32, device=dev) if want else None
+    dinit = _states_like(initial, (sequences, channels), dx) if want else None
     sizes = (rows, sequences, int(offs is None), channels, gates, _TYPES[x.dtype], _TYPES[gate.dtype])
-    scratch, nbytes = _work("gs_gated_scan_scratch_bytes", sizes, dev, 1)
+    scratch, nbytes = _work("gs_gated_scan_scratch_bytes", sizes, dx, 1)
     with on_device(dev):
         nat.call("gs_gated_scan_backward", rows, sequences, channels, gates, sizes[5], sizes[6],
                  xr.data_ptr(), x_step, gr.data_ptr(), g_step, _ptr(init), _ptr(offs),
