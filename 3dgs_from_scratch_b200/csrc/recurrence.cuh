@@ -53,6 +53,8 @@ constexpr int kBatch = 8;  // rows in flight, and from one kept state to the nex
 // backward of 8 x 2048 x 1024: 212, 184 and 189 us, of 524,288 x 35: 410, 402 and
 // 495 us with 640, 1280 and 2560).
 constexpr int kFill = 1280;
+// Rows that a thread walks in the time that the chain's two launches take (12 us).
+constexpr int kShort = 128;
 
 // How a problem is cut. It depends on the sizes and types alone, never on
 // pointers, so that the backward finds the states that the forward kept.

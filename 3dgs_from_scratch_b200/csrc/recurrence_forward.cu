@@ -30,7 +30,7 @@ Plan make_plan(int64_t rows, int sequences, bool even, int channels, int gates, 
   // Rows of a chunk: about kFill threads on each of 148 SMs.
   const int64_t want = rows * vectors / (148 * kFill);
   const int64_t period = even ? rows / sequences : 0;
-  p.whole = even && period > 0 && (period <= 32 || (int64_t)sequences * vectors >= 148 * 256);
+  p.whole = even && period > 0 && (period <= kShort || (int64_t)sequences * vectors >= 148 * 256);
   if (p.whole) {
     const int64_t k = want / period;
     p.chunk = (int)(period * (k < 1 ? 1 : k > 64 ? 64 : k));
@@ -38,7 +38,8 @@ Plan make_plan(int64_t rows, int sequences, bool even, int channels, int gates, 
     int64_t chunk = 32;
     while (chunk < want && chunk < 512) chunk *= 2;
     p.chunk = (int)chunk;
-    if (rows <= p.chunk) p.whole = true;
+    if (rows <= kShort) p.chunk = kShort;
+    p.whole = rows <= p.chunk;
   }
   p.chunks = rows > 0 ? (rows + p.chunk - 1) / p.chunk : 0;
   p.kept = (p.chunk + kBatch - 1) / kBatch;

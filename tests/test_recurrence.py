@@ -190,7 +190,11 @@ def test_other_layouts_give_the_same(gs):
     assert float((d1 - d2).detach().abs().max()) <= 2 * (4 * 70 + 32 + 24) * U * 24 * float(sizes)
     offs = torch.arange(0, 351, 70, device=DEV)                # int64 offsets of the same sequences
     h6, f6 = gs.gated_scan(x.reshape(350, 24), g.reshape(350, 24), offsets=offs)
-    assert torch.equal(h6.reshape(5, 70, 24), h) and torch.equal(f6, final)
+    # Even sequences and offsets may be cut into other chunks: each is within (2 n + 16) u of the
+    # recurrence on absolute values from the exact states (n = 70), so they are within twice that.
+    most = 2 * (2 * 70 + 16) * U * float(gs.gated_scan(x.abs(), g)[0].max())
+    assert float((h6.reshape(5, 70, 24) - h).abs().max()) <= most
+    assert float((f6 - final).abs().max()) <= most
     tail = torch.randn(351 * 24, device=DEV)[1:350 * 24 + 1].reshape(350, 24)  # not at 16 bytes
     h7, _ = gs.gated_scan(tail, g.reshape(350, 24), offsets=offs)
     h8, _ = gs.gated_scan(tail.clone(), g.reshape(350, 24), offsets=offs)
@@ -441,4 +445,4 @@ def test_entry_points_refuse_bad_arguments(gs):
     assert lib.gs_gated_scan_saved_bytes(100, 1, 1, 8, 8, 0, 0) >= 100 // 8 * 8 * 4
     assert lib.gs_gated_scan_scratch_bytes(24, 1, 1, 8, 8, 0, 0, 0) == 0
     assert lib.gs_gated_scan_scratch_bytes(1 << 20, 1, 1, 8, 8, 0, 0, 1) > 0
-    assert lib.gs_gated_scan_scratch_bytes(100, 5, 0, 8, 8, 0, 0, 0) > 0
+    assert lib.gs_gated_scan_scratch_bytes(1 << 20, 5, 0, 8, 8, 0, 0, 0) > 0
