@@ -10,7 +10,7 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-// Every thread of both blocks.
+// Every thread of every block of the cluster.
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -21,14 +21,6 @@ __device__ __forceinline__ uint32_t cluster_addr(const void *p, uint32_t rank) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
   return a;
-}
-__device__ __forceinline__ float4 cluster_load(uint32_t at) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(at)
-               : "memory");
-  return v;
 }
 __device__ __forceinline__ float2 cluster_load2(uint32_t at) {
   float2 v;
@@ -44,11 +36,6 @@ __device__ __forceinline__ double cluster_load_f64(uint32_t at) {
   double v;
   asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(at) : "memory");
   return v;
-}
-__device__ __forceinline__ void cluster_store(uint32_t at, const uint4 &v) {
-  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z),
-               "r"(v.w)
-               : "memory");
 }
 
 }  // namespace gs

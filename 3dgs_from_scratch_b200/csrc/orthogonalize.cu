@@ -760,8 +760,10 @@ __global__ void __launch_bounds__(256) split_kernel(const Source s, const double
 // A in shared memory, in the same block images, and runs norm, steps and result
 // in one launch. A launch for each product took 5 to 6 us each, 17 of them.
 // In a cluster every block forms the part of A = X X^T that its columns give;
-// block k adds the parts of its 128 / C rows in the blocks' order and hands the
-// result to all. B = b A + c A A is cheap enough to be formed by each block.
+// block k adds the parts of its MC / C rows in the blocks' order, and every block
+// fetches all of A. Both go through global memory (L2), between cluster barriers:
+// through the blocks' shared memory they took 8 us a step, 5 here. B = b A +
+// c A A is cheap enough to be formed by each block.
 constexpr int kSmallThreads = 512;  // four warps for each quarter of tensor memory's lanes
 
 struct SmallArgs {
@@ -770,6 +772,7 @@ struct SmallArgs {
   int cluster, steps;
   float a, b, c;
   double eps;
+  char *shared;  // of a matrix's blocks: their parts of A, then A's planes
   uint32_t *status;
 };
 
@@ -780,12 +783,16 @@ struct SmallShape {
   static constexpr int kBlocks = NC / 64;
   static constexpr int kX = kBlocks * kBlockBytes;          // a plane of X
   static constexpr int kSq = MC / 64 * kBlockBytes;         // a plane of A or B
-  static constexpr int kPart = NC == 128 ? MC * MC * 4 : 0;  // a block's part of A (clusters)
-  static constexpr int kTurn = kSmallThreads / 32 * 32 * 33 * 4;  // in place of A and the part, or behind
-  static constexpr int kRest = 2 * kSq + kPart > kTurn ? 2 * kSq + kPart : kTurn;
+  static constexpr int kTurn = kSmallThreads / 32 * 32 * 33 * 4;  // in place of A, and behind
+  static constexpr int kRest = 2 * kSq > kTurn ? 2 * kSq : kTurn;
   static constexpr int kBytes = 2 * kX + kRest;
   static constexpr int kTop = NC > MC ? NC : MC;            // columns of an accumulator
 };
+
+// What a matrix's blocks share in global memory: their parts of A, A's planes.
+__host__ __device__ constexpr int64_t shared_bytes(int mc, int cluster) {
+  return cluster == 1 ? 0 : (int64_t)cluster * mc * mc * 4 + 2 * (mc / 64) * kBlockBytes;
+}
 
 // All MMAs of D = P Q^T (or P Q, Q's rows along K) over `blocks` K blocks:
 // hi hi into main, hi lo + lo hi into cross.
@@ -825,7 +832,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
   using S = SmallShape<MC, NC>;
   extern __shared__ char raw[];
   char *x_hi = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023), *x_lo = x_hi + S::kX;
-  char *sq_hi = x_lo + S::kX, *sq_lo = sq_hi + S::kSq, *part = sq_lo + S::kSq;
+  char *sq_hi = x_lo + S::kX, *sq_lo = sq_hi + S::kSq;
   __shared__ uint64_t done;
   __shared__ uint32_t tmem_base, failed;
   __shared__ double warp_sums[kSmallThreads / 32], block_sum;
@@ -916,6 +923,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
     *reinterpret_cast<uint4 *>(x_hi + to) = hi;
     *reinterpret_cast<uint4 *>(x_lo + to) = lo;
   }
+  float *part = reinterpret_cast<float *>(A.shared + (int64_t)batch * shared_bytes(MC, C));
+  char *whole = reinterpret_cast<char *>(part + C * MC * MC);
   const uint32_t tmem = tmem_base, cross = tmem + S::kTop;
   const int quarter = warp & 3, group = warp / 4, r = quarter * 32 + lane;
   const bool on = quarter * 32 < MC;  // the warp's rows are X's
@@ -973,25 +982,25 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
           const int to = (c + g) / 64 * kBlockBytes + chunk_at(r, c + g);
           put(sq_hi + to, sq_lo + to, w);
         }
-      } else if (S::kPart > 0) {  // rows of MC floats, their 16-byte chunks swizzled
+      } else {  // column by column, so that the warp writes adjacent rows
 #pragma unroll
-        for (int g = 0; g < 32; g += 4)
-          *reinterpret_cast<float4 *>(part + r * (MC * 4) + ((((c + g) / 4) ^ (r & (MC / 4 - 1))) << 4)) =
-              make_float4(v[g], v[g + 1], v[g + 2], v[g + 3]);
+        for (int e = 0; e < 32; ++e) __stcg(part + rank * (MC * MC) + (c + e) * MC + r, v[e]);
       }
     }
-    if (S::kPart > 0 && C > 1) {
+    if (C > 1) {
+      __threadfence();
       cluster_sync();
+      // A is symmetric: its row `row` is what lies in column `row` of the parts.
       const int rows = MC / C;
       for (int k = threadIdx.x; k < rows * (MC / 8); k += kSmallThreads) {
         const int row = rank * rows + k / (MC / 8), c = k % (MC / 8) * 8;
+        const float4 *from = reinterpret_cast<const float4 *>(part + row * MC + c);
         float4 f[8], g[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q)
           if (q < C) {
-            const uint32_t from = cluster_addr(part, q) + row * (MC * 4);
-            f[q] = cluster_load(from + (((c / 4) ^ (row & (MC / 4 - 1))) << 4));
-            g[q] = cluster_load(from + (((c / 4 + 1) ^ (row & (MC / 4 - 1))) << 4));
+            f[q] = __ldcg(from + q * (MC * MC / 4));
+            g[q] = __ldcg(from + q * (MC * MC / 4) + 1);
           }
         float w[8] = {};
 #pragma unroll
@@ -1005,16 +1014,24 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
         uint4 hi, lo;
         split8(w, hi, lo);
         const int to = c / 64 * kBlockBytes + chunk_at(row, c);
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (q < C) {
-            cluster_store(cluster_addr(sq_hi + to, q), hi);
-            cluster_store(cluster_addr(sq_lo + to, q), lo);
-          }
+        __stcg(reinterpret_cast<uint4 *>(whole + to), hi);
+        __stcg(reinterpret_cast<uint4 *>(whole + S::kSq + to), lo);
       }
-      asm volatile("fence.proxy.async;" ::: "memory");
+      __threadfence();
       __syncwarp();
       cluster_sync();
+      // Rows beyond MC of the images are neither written nor read.
+      constexpr int kCopies = 2 * MC / 64 * MC * 8 / kSmallThreads;
+      uint4 q[kCopies];
+      int at[kCopies];
+#pragma unroll
+      for (int k = 0; k < kCopies; ++k) {
+        const int e = k * kSmallThreads + threadIdx.x;  // chunks of MC rows, image after image
+        at[k] = e / (MC * 8) * kBlockBytes + e % (MC * 8) * 16;
+        q[k] = __ldcg(reinterpret_cast<const uint4 *>(whole + at[k]));
+      }
+#pragma unroll
+      for (int k = 0; k < kCopies; ++k) *reinterpret_cast<uint4 *>(sq_hi + at[k]) = q[k];
     }
     run([&] {
       small_product<MC, false>(tmem, cross, smem_addr(sq_hi), smem_addr(sq_lo), smem_addr(sq_hi),
@@ -1084,11 +1101,11 @@ struct SmallPlan {
   int columns, cluster;
 };
 static SmallPlan small_plan(int m, int n) {
-  if (m > 128 || n > 1024) return {0, 0};
+  if (m > 128 || n > 2048) return {0, 0};
   if (n <= 64) return {64, 1};
   if (n <= 128) return {128, 1};
   if (n <= 256) return {256, 1};
-  return {128, n <= 512 ? 4 : 8};
+  return {n <= 1024 ? 128 : 256, n <= 512 ? 4 : 8};
 }
 
 // What a step costs in tiles of 128 ctas x bn, in microseconds: each of its three
@@ -1147,7 +1164,8 @@ static Plan make_plan(int batch, int rows, int cols, int type) {
   p.x_bytes = (size_t)batch * p.row_blocks * p.column_blocks * kBlockBytes;
   p.sq_bytes = (size_t)batch * p.row_blocks * p.sq_column_blocks * kBlockBytes;
   p.total = 4 * p.x_bytes + (p.full ? 4 : 2) * p.sq_bytes + (size_t)batch * p.parts * 8;
-  if (small_plan(p.m, p.n).columns) p.total = 16;  // all on chip
+  const SmallPlan small = small_plan(p.m, p.n);
+  if (small.columns) p.total = 16 + (size_t)batch * shared_bytes(p.m <= 64 ? 64 : 128, small.cluster);
   return p;
 }
 
@@ -1284,7 +1302,7 @@ static int run(int batch, const Plan &p, const Source &src, const Out &out, int 
   if (A.status == nullptr) return GS_ERR_CUDA;
   const SmallPlan small = small_plan(p.m, p.n);
   if (small.columns) {
-    const SmallArgs B{src, out, small.cluster, steps, a, b, c, (double)eps, A.status};
+    const SmallArgs B{src, out, small.cluster, steps, a, b, c, (double)eps, static_cast<char *>(scratch), A.status};
     if (p.m <= 64)
       return small.columns == 64    ? launch_small<64, 64>(B, batch, st)
              : small.columns == 128 ? launch_small<64, 128>(B, batch, st)

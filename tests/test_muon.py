@@ -51,7 +51,8 @@ def strong(m, n, rank, dtype=F32, batch=None, seed=0, scale=1e-3):
 SIZES = [(1, 1), (1, 70), (70, 1), (16, 16), (63, 65), (64, 64), (128, 128), (129, 127), (45, 3000), (200, 130),
          (257, 255), (384, 640), (1000, 300),
          # on chip in 1, 4 and 8 blocks, and just beyond
-         (100, 256), (100, 257), (512, 128), (90, 513), (128, 1024), (1000, 17), (128, 1025), (129, 1024)]
+         (100, 256), (100, 257), (512, 128), (90, 513), (128, 1024), (1000, 17), (128, 1025), (129, 1024), (60, 1500),
+         (2048, 128), (33, 2049)]
 
 
 @gpu
