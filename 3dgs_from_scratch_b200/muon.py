@@ -113,3 +113,5 @@ def muon_step(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor, l
         nat.call("gs_muon_step", batch, rows, cols, _TYPES[grad.dtype], param.data_ptr(),
                  grad.data_ptr(), momentum.data_ptr(), lr, beta, int(nesterov), weight_decay, scale,
                  int(steps), *coefficients, eps, scratch.data_ptr(), nbytes, nat.stream_ptr(dev))
+    # written behind autograd's back: a graph that still holds the old values says so
+    torch.autograd.graph.increment_version((param, momentum))

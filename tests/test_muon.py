@@ -85,6 +85,62 @@ def test_five_steps(gs, m, n, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("batch,m,n,dtype", [
+    (12, 256, 512, BF16), (1, 1536, 1536, BF16), (1, 2048, 4096, BF16), (1, 3001, 3501, BF16),
+    (32, 384, 384, F32), (1, 1333, 1000, F32), (1, 2100, 2050, F16), (7, 130, 2300, F32)])
+def test_every_tile_shape(gs, batch, m, n, dtype):
+    """Sizes whose products are cut into each of the tile shapes, some of them into more
+    rounds of tiles than one; the formulas run on the GPU, in 64 bits and (the yardstick) 32."""
+    gen = torch.Generator(device=DEV).manual_seed(m)
+    u = torch.randn(batch, m, n, generator=gen, device=DEV)
+    u = (1e-3 * (u + 0.2 * torch.randn(batch, m, 8, generator=gen, device=DEV) @
+                 torch.randn(batch, 8, n, generator=gen, device=DEV))).to(dtype)
+
+    def formula(kind):
+        x = u.double()
+        x = (x / torch.linalg.matrix_norm(x, keepdim=True)).to(kind)
+        x = x.mT if m > n else x
+        for _ in range(5):
+            g = x @ x.mT
+            x = ABC[0] * x + (ABC[1] * g + ABC[2] * g @ g) @ x
+        return (x.mT if m > n else x).double()
+
+    ref = formula(torch.float64)
+    yard = float((formula(F32) - ref).norm() / ref.norm())
+    got = gs.orthogonalize(u).double()
+    round_off = {F32: 0.0, F16: 2.0 ** -12, BF16: 2 * 2.0 ** -9}[dtype]
+    assert float((got - ref).norm() / ref.norm()) <= 4 * yard + 2 ** -22 + round_off
+    # no tile of its own may be off: 128 x 128 pieces against twice the whole's bound
+    worst = 0.0
+    for i in range(0, m, 128):
+        for j in range(0, n, 128):
+            a, b = got[:, i:i + 128, j:j + 128], ref[:, i:i + 128, j:j + 128]
+            worst = max(worst, float((a - b).norm() / b.norm()))
+    assert worst <= 2 * (4 * yard + 2 ** -22 + round_off)
+
+
+@gpu
+@pytest.mark.parametrize("m,n", [(100, 300), (64, 900), (90, 1700)])
+def test_stacks_of_matrices_in_clusters(gs, m, n):
+    u = strong(m, n, 5, batch=4, seed=m).to(DEV)
+    whole = gs.orthogonalize(u)
+    for k in range(4):
+        assert torch.equal(gs.orthogonalize(u[k]), whole[k])   # the same cut, the same sums
+    w, m1 = torch.zeros_like(u), torch.zeros_like(u)
+    gs.muon_step(w, u, m1, 0.5, beta=0.0, nesterov=False, scale=1.0)
+    assert rel(w, -0.5 * whole.double().cpu()) <= 2.0 ** -22
+
+
+@gpu
+def test_a_graph_of_the_old_weights_is_refused(gs):
+    w = torch.randn(20, 30, device=DEV, requires_grad=True)
+    loss = (w * w).sum()
+    gs.muon_step(w, torch.randn(20, 30, device=DEV), torch.zeros(20, 30, device=DEV), 0.1)
+    with pytest.raises(RuntimeError):
+        loss.backward()
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_stacks_and_strides(gs, dtype):
     u = strong(60, 100, 4, dtype, batch=5, seed=1).to(DEV)
