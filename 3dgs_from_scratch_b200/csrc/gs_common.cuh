@@ -154,6 +154,18 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
+// ---- launches of one call that overlap ------------------------------------------
+// Each may start its set-up while the one before it still runs (launched with
+// overlapping()), and reads what that one writes only behind wait_for_previous().
+__device__ __forceinline__ void start_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+inline cudaLaunchAttribute overlapping() {
+  cudaLaunchAttribute a{};
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  return a;
+}
+
 // ---- projection -------------------------------------------------------------
 
 struct Cam {

@@ -75,14 +75,6 @@ struct Args {
   uint32_t *status;
 };
 
-// Launches of one call overlap: each may start its set-up while the one before
-// it still runs, and touches global memory only after that one is complete.
-__device__ __forceinline__ void start_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_previous() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("fence.proxy.async.global;" ::: "memory");  // the bulk copies read what it wrote
-}
-
 __device__ __forceinline__ char *block_at(char *plane, const Matrix &M, int batch, int rb, int cb) {
   return plane + (int64_t)batch * M.batch_bytes + ((int64_t)rb * M.column_blocks + cb) * kBlockBytes;
 }
@@ -311,6 +303,7 @@ __global__ void __launch_bounds__(Shape<BN, KIND, FULL, CTAS>::kThreads, 1)
   const uint32_t tmem = tmem_base;
   start_next();
   wait_for_previous();
+  asm volatile("fence.proxy.async.global;" ::: "memory");  // the bulk copies read what it wrote
   // Tile t: its matrix, row of tiles and column of tiles.
   struct Spot {
     int batch, i, j;
@@ -1167,13 +1160,6 @@ static Plan make_plan(int batch, int rows, int cols, int type) {
   const SmallPlan small = small_plan(p.m, p.n);
   if (small.columns) p.total = 16 + (size_t)batch * shared_bytes(p.m <= 64 ? 64 : 128, small.cluster);
   return p;
-}
-
-static cudaLaunchAttribute overlapping() {
-  cudaLaunchAttribute a{};
-  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  a.val.programmaticStreamSerializationAllowed = 1;
-  return a;
 }
 
 template <int BN, int KIND, bool FULL, int CTAS>

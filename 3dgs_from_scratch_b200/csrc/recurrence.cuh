@@ -257,6 +257,23 @@ inline unsigned grid_of(const Plan &p) {
   return (unsigned)(((p.chunks + p.cy - 1) / p.cy) * p.channel_blocks);
 }
 
+// The walk after the two launches of the chain, or alone.
+template <typename Kernel>
+inline int launch_walk(Kernel kernel, const Args &A, cudaStream_t st) {
+  const unsigned blocks = grid_of(A.plan);
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr = overlapping();
+  cfg.attrs = &attr;
+  cfg.numAttrs = A.carry != nullptr ? 1 : 0;
+  cfg.gridDim = dim3(blocks + (A.carry == nullptr ? extra_blocks(A) : 0));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  const int rc = cuda_status(cudaLaunchKernelEx(&cfg, kernel, A, blocks));
+  if (rc) return rc;
+  count_launch();
+  return GS_OK;
+}
+
 // The place of a thread: its channels and its chunk's logical rows t0..t1-1.
 struct Place {
   int tx, cy, c, g;     // vector and chunk in the block, first channel and its gate
@@ -291,6 +308,7 @@ __device__ __forceinline__ int64_t along(const Args &A, int64_t stride) { return
 
 template <typename XT, typename GT, int V, bool SHARED, bool BACK>
 __global__ void __launch_bounds__(kThreads) maps_kernel(const __grid_constant__ Args A, unsigned blocks) {
+  start_next();
   if (blockIdx.x >= blocks) {
     look_at_sequences(A, blockIdx.x - blocks);
     return;

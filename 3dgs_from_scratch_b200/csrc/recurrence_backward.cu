@@ -34,6 +34,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
   if (!SHARED && !p.on) return;
   const int64_t xs = along(A, A.x_stride), gs = along(A, A.gate_stride), ds = along(A, A.dh_stride);
   const int64_t ts = along(A, A.channels), os = along(A, A.gates);
+  wait_for_previous();
   Cursor q;
   q.s = first_hint<true>(A, p.chunk);
   q.lo = q.hi = 0;
@@ -202,15 +203,15 @@ __global__ void __launch_bounds__(kThreads) join_gates_kernel(const __grid_const
 
 template <typename XT, typename GT, int V, bool SHARED>
 static int launch_backward(const Args &A, cudaStream_t st) {
-  const unsigned blocks = grid_of(A.plan), extra = extra_blocks(A);
   if (A.carry != nullptr) {
-    maps_kernel<XT, GT, V, SHARED, true><<<blocks + extra, kThreads, 0, st>>>(A, blocks);
+    const unsigned blocks = grid_of(A.plan);
+    maps_kernel<XT, GT, V, SHARED, true><<<blocks + extra_blocks(A), kThreads, 0, st>>>(A, blocks);
     count_launch();
     const int rc = launch_carry(A, true, st);
     if (rc) return rc;
   }
-  backward_kernel<XT, GT, V, SHARED><<<blocks + (A.carry == nullptr ? extra : 0), kThreads, 0, st>>>(A, blocks);
-  count_launch();
+  const int rc = launch_walk(backward_kernel<XT, GT, V, SHARED>, A, st);
+  if (rc) return rc;
   if (A.partial != nullptr && A.rows > 0) {
     const int64_t want = (A.rows * A.gates + kThreads - 1) / kThreads;
     join_gates_kernel<GT><<<(unsigned)(want < 1184 ? want : 1184), kThreads, 0, st>>>(A);

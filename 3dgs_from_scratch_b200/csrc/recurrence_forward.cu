@@ -59,6 +59,8 @@ template <bool BACK>
 __global__ void __launch_bounds__(kCarryChannels *kRuns) carry_kernel(const __grid_constant__ Args A, int blocks) {
   __shared__ float2 maps[2][kRuns][kCarryChannels];
   __shared__ uint32_t cuts[2][kRuns];
+  start_next();
+  wait_for_previous();
   const int lane = threadIdx.x % kCarryChannels, run = threadIdx.x / kCarryChannels;
   const int rank = blocks > 1 ? (int)cluster_rank() : 0;
   const int c = blockIdx.x / blocks * kCarryChannels + lane;
@@ -143,12 +145,13 @@ int launch_carry(const Args &A, bool back, cudaStream_t st) {
   // 941 chunks take 8 us in one block and 20 in a cluster, 2048 take 19 and 9.
   const int blocks = A.plan.chunks > 12 * kRuns ? kCarryBlocks : 1;
   cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = blocks;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0] = overlapping();
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = blocks;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = blocks > 1 ? 2 : 1;
   cfg.gridDim = dim3((unsigned)((A.channels + kCarryChannels - 1) / kCarryChannels) * blocks);
   cfg.blockDim = dim3(kCarryChannels * kRuns);
   cfg.stream = st;
@@ -174,6 +177,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
   const XT *from = reinterpret_cast<const XT *>(A.x) + row * A.x_stride + p.c;
   const GT *gate = reinterpret_cast<const GT *>(A.gate) + row * A.gate_stride + p.g;
   XT *to = reinterpret_cast<XT *>(A.h) + (int64_t)row * A.channels + p.c;
+  wait_for_previous();
   Cursor q;
   q.s = first_hint<false>(A, p.chunk);
   q.seek(A, row);
@@ -234,16 +238,14 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
 
 template <typename XT, typename GT, int V, bool SHARED>
 static int launch_forward(const Args &A, cudaStream_t st) {
-  const unsigned blocks = grid_of(A.plan), extra = extra_blocks(A);
   if (A.carry != nullptr) {
-    maps_kernel<XT, GT, V, SHARED, false><<<blocks + extra, kThreads, 0, st>>>(A, blocks);
+    const unsigned blocks = grid_of(A.plan);
+    maps_kernel<XT, GT, V, SHARED, false><<<blocks + extra_blocks(A), kThreads, 0, st>>>(A, blocks);
     count_launch();
     const int rc = launch_carry(A, false, st);
     if (rc) return rc;
   }
-  forward_kernel<XT, GT, V, SHARED><<<blocks + (A.carry == nullptr ? extra : 0), kThreads, 0, st>>>(A, blocks);
-  count_launch();
-  return launch_status();
+  return launch_walk(forward_kernel<XT, GT, V, SHARED>, A, st);
 }
 
 template <typename XT, typename GT>
