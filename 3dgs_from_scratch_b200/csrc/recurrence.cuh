@@ -9,8 +9,8 @@
 //   (P2, L2) after (P1, L1) = (P1 P2, P2 L1 + L2).
 //
 // Memory is what bounds both directions (a handful of operations an element).
-// So a thread does nothing but walk rows: it owns V adjacent channels of a
-// chunk of rows, keeps the state in registers and reads and writes each row
+// So a thread does nothing but walk rows: it owns V channels of a chunk of
+// rows, keeps the state in registers and reads and writes each row
 // once, a batch of rows in flight at a time. Chunks are as long as leaves
 // enough threads to fill the device. Sequence bounds need no chunks of their
 // own: at a sequence's first row the initial state takes the place of the
@@ -59,8 +59,10 @@ constexpr int kShort = 128;
 // How a problem is cut. It depends on the sizes and types alone, never on
 // pointers, so that the backward finds the states that the forward kept.
 struct Plan {
-  int vec;             // channels of a thread
-  int tx, cy;          // vectors of channels across a block, chunks in it
+  int vec;             // channels of a thread: adjacent ones, read as one vector,
+  int step;            // or (step > 0) apart by so many: where rows are no whole vectors
+  int tx, cy;          // threads across the channels of a block, chunks in it
+  int width;           // channels of a block
   int channel_blocks;  // blocks across the channels
   int chunk;           // rows of a chunk
   int64_t chunks;
@@ -138,54 +140,81 @@ struct alignas(V * sizeof(T) >= 16 ? 16 : V * sizeof(T)) Pack {
   T e[V];
 };
 
-template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> load_pack(const T *p) {
-  return *reinterpret_cast<const Pack<T, V> *>(p);
-}
+// The place of a thread: its channels and its chunk's logical rows t0..t1-1. ST:
+// its channels lie apart; where the block has no second one for it, the first
+// stands in, and the thread writes the same values twice.
+template <int V, bool ST>
+struct Place {
+  int tx, cy, c, g;  // c, g: its first channel and that channel's gate
+  int to[V];         // ST: from there to its others
+  int64_t chunk, t0, t1;
+  bool on;
+  __device__ __forceinline__ int at(int v) const { return ST ? to[v] : v; }
+};
 
-template <typename T, int V>
-__device__ __forceinline__ void store_pack(T *p, const float (&v)[V]) {
+template <typename T, int V, bool ST, typename P>
+__device__ __forceinline__ Pack<T, V> load_pack(const T *p, const P &at) {
+  if (!ST) return *reinterpret_cast<const Pack<T, V> *>(p);
   Pack<T, V> o;
 #pragma unroll
-  for (int i = 0; i < V; ++i) o.e[i] = from_f32<T>(v[i]);
-  *reinterpret_cast<Pack<T, V> *>(p) = o;
+  for (int v = 0; v < V; ++v) o.e[v] = p[at.at(v)];
+  return o;
 }
 
-// The gate of a thread's channel v: one for each channel, or one for the whole
-// vector (the plan cuts vectors at gate bounds).
-template <typename GT, int V, bool SHARED>
+template <typename T, int V, bool ST>
+__device__ __forceinline__ void store_pack(T *p, const float (&x)[V], const Place<V, ST> &at) {
+  Pack<T, V> o;
+#pragma unroll
+  for (int v = 0; v < V; ++v) o.e[v] = from_f32<T>(x[v]);
+  if (!ST) {
+    *reinterpret_cast<Pack<T, V> *>(p) = o;
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) p[at.at(v)] = o.e[v];
+  }
+}
+
+// The gates of a thread's channels: one each, or one for the whole vector (the
+// plan cuts vectors at gate bounds).
+template <typename GT, int V, bool SHARED, bool ST>
 struct Gates {
   Pack<GT, SHARED ? 1 : V> g;
   __device__ __forceinline__ float operator()(int v) const { return to_f32<GT>(g.e[SHARED ? 0 : v]); }
-  __device__ __forceinline__ void load(const GT *p) { g = load_pack<GT, SHARED ? 1 : V>(p); }
+  __device__ __forceinline__ void load(const GT *p, const Place<V, ST> &at) {
+    if (SHARED)
+      g.e[0] = p[0];
+    else
+      g = load_pack<GT, SHARED ? 1 : V, ST>(p, at);
+  }
 };
 
-// Row `at` of a (n, channels) fp32 tensor, channels c.. (zeros without one).
-template <int V>
-__device__ __forceinline__ void load_state(const float *__restrict__ p, const Args &A, int64_t at, int c,
-                                           float (&out)[V]) {
+// Row `row` of a (n, channels) fp32 tensor (zeros without one).
+template <int V, bool ST>
+__device__ __forceinline__ void load_state(const float *__restrict__ p, const Args &A, int64_t row,
+                                           const Place<V, ST> &at, float (&out)[V]) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) out[v] = p != nullptr ? p[at * A.channels + c + v] : 0.f;
+  for (int v = 0; v < V; ++v)
+    out[v] = p != nullptr ? p[row * A.channels + at.c + at.at(v)] : 0.f;
 }
-template <int V>
-__device__ __forceinline__ void store_state(float *__restrict__ p, const Args &A, int64_t at, int c,
-                                            const float (&in)[V]) {
+template <int V, bool ST>
+__device__ __forceinline__ void store_state(float *__restrict__ p, const Args &A, int64_t row,
+                                            const Place<V, ST> &at, const float (&in)[V]) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) p[at * A.channels + c + v] = in[v];
+  for (int v = 0; v < V; ++v) p[row * A.channels + at.c + at.at(v)] = in[v];
 }
 
 // The same in buffers of our own, whose rows start at whole vectors.
-template <int V>
-__device__ __forceinline__ void load_kept(const float *__restrict__ p, const Args &A, int64_t at, int c,
-                                          float (&out)[V]) {
-  const Pack<float, V> q = load_pack<float, V>(p + at * A.channels + c);
+template <int V, bool ST>
+__device__ __forceinline__ void load_kept(const float *__restrict__ p, const Args &A, int64_t row,
+                                          const Place<V, ST> &at, float (&out)[V]) {
+  const Pack<float, V> q = load_pack<float, V, ST>(p + row * A.channels + at.c, at);
 #pragma unroll
   for (int v = 0; v < V; ++v) out[v] = q.e[v];
 }
-template <int V>
-__device__ __forceinline__ void store_kept(float *__restrict__ p, const Args &A, int64_t at, int c,
-                                           const float (&in)[V]) {
-  store_pack<float, V>(p + at * A.channels + c, in);
+template <int V, bool ST>
+__device__ __forceinline__ void store_kept(float *__restrict__ p, const Args &A, int64_t row,
+                                           const Place<V, ST> &at, const float (&in)[V]) {
+  store_pack<float, V, ST>(p + row * A.channels + at.c, in, at);
 }
 
 // ---- where a row belongs ----------------------------------------------------------------
@@ -274,22 +303,18 @@ inline int launch_walk(Kernel kernel, const Args &A, cudaStream_t st) {
   return GS_OK;
 }
 
-// The place of a thread: its channels and its chunk's logical rows t0..t1-1.
-struct Place {
-  int tx, cy, c, g;     // vector and chunk in the block, first channel and its gate
-  int64_t chunk, t0, t1;
-  bool on;
-};
-
-template <int V, bool SHARED>
-__device__ __forceinline__ Place place_of(const Args &A, int64_t group, int cblk) {
-  Place p;
+template <int V, bool SHARED, bool ST>
+__device__ __forceinline__ Place<V, ST> place_of(const Args &A, int64_t group, int cblk) {
+  Place<V, ST> p;
   p.tx = threadIdx.x % A.plan.tx;
   p.cy = threadIdx.x / A.plan.tx;
-  p.c = (cblk * A.plan.tx + p.tx) * V;
+  p.c = cblk * A.plan.width + p.tx * (ST ? 1 : V);
+  const int end = (cblk + 1) * A.plan.width < A.channels ? (cblk + 1) * A.plan.width : A.channels;
   p.g = SHARED ? p.c / A.per_gate : p.c;
+#pragma unroll
+  for (int v = 0; v < V; ++v) p.to[v] = ST && p.c + v * A.plan.step < end ? v * A.plan.step : 0;
   p.chunk = group * A.plan.cy + p.cy;
-  p.on = p.cy < A.plan.cy && p.chunk < A.plan.chunks && p.c < A.channels;
+  p.on = p.cy < A.plan.cy && p.chunk < A.plan.chunks && p.c < end;
   p.t0 = p.chunk * A.plan.chunk;
   p.t1 = p.t0 + A.plan.chunk < A.rows ? p.t0 + A.plan.chunk : A.rows;
   return p;
@@ -306,7 +331,7 @@ __device__ __forceinline__ int64_t along(const Args &A, int64_t stride) { return
 // rows of the sequence that reaches over the chunk's end, from that sequence's
 // first row along the chain where the chunk holds it (the chain is cut there).
 
-template <typename XT, typename GT, int V, bool SHARED, bool BACK>
+template <typename XT, typename GT, int V, bool SHARED, bool ST, bool BACK>
 __global__ void __launch_bounds__(kThreads) maps_kernel(const __grid_constant__ Args A, unsigned blocks) {
   start_next();
   if (blockIdx.x >= blocks) {
@@ -314,7 +339,7 @@ __global__ void __launch_bounds__(kThreads) maps_kernel(const __grid_constant__ 
     return;
   }
   const int cblk = blockIdx.x % A.plan.channel_blocks;
-  const Place p = place_of<V, SHARED>(A, blockIdx.x / A.plan.channel_blocks, cblk);
+  const auto p = place_of<V, SHARED, ST>(A, blockIdx.x / A.plan.channel_blocks, cblk);
   if (!p.on) return;
   const int64_t t_end = BACK ? p.t0 : p.t1 - 1;  // the chunk's last row along the chain
   const int row_end = (int)row_at(A, t_end);
@@ -346,22 +371,22 @@ __global__ void __launch_bounds__(kThreads) maps_kernel(const __grid_constant__ 
 #pragma unroll
   for (int v = 0; v < V; ++v) P[v] = 1.f, L[v] = 0.f;
   if (needed) {
-    if (cut) load_state<V>(BACK ? A.dfinal : A.initial, A, q.s, p.c, L);
+    if (cut) load_state(BACK ? A.dfinal : A.initial, A, q.s, p, L);
     const int64_t row = up ? row_end - (n - 1) : row_end + (n - 1);
     const int64_t xs = BACK ? A.dh_stride : A.x_stride;
     const XT *from = reinterpret_cast<const XT *>(BACK ? A.dh : A.x) + row * xs + p.c;
     const GT *gate = reinterpret_cast<const GT *>(A.gate) + row * A.gate_stride + p.g;
     const int64_t step = up ? xs : -xs, gstep = up ? A.gate_stride : -A.gate_stride;
     const bool some = !BACK || A.dh != nullptr;
-    constexpr int kAhead = V == 1 ? 2 * kBatch : kBatch;
+    constexpr int kAhead = ST || V == 1 ? 2 * kBatch : kBatch;
     for (int left = n; left > 0; left -= kAhead) {
       Pack<XT, V> x[kAhead];
-      Gates<GT, V, SHARED> g[kAhead];
+      Gates<GT, V, SHARED, ST> g[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
         if (k < left) {
-          if (some) x[k] = load_pack<XT, V>(from + k * step);
-          g[k].load(gate + k * gstep);
+          if (some) x[k] = load_pack<XT, V, ST>(from + k * step, p);
+          g[k].load(gate + k * gstep, p);
         }
 #pragma unroll
       for (int k = 0; k < kAhead; ++k)
@@ -378,7 +403,8 @@ __global__ void __launch_bounds__(kThreads) maps_kernel(const __grid_constant__ 
     }
   }
 #pragma unroll
-  for (int v = 0; v < V; ++v) A.maps[p.chunk * A.channels + p.c + v] = make_float2(P[v], L[v]);
+  for (int v = 0; v < V; ++v)
+    A.maps[p.chunk * A.channels + p.c + p.at(v)] = make_float2(P[v], L[v]);
   if (cblk == 0 && p.tx == 0) A.cuts[p.chunk] = cut;
 }
 

@@ -19,7 +19,7 @@ namespace scan {
 
 constexpr int kParts = 4;  // threads that share a sum over a gate's channels
 
-template <typename XT, typename GT, int V, bool SHARED>
+template <typename XT, typename GT, int V, bool SHARED, bool ST>
 __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constant__ Args A, unsigned blocks) {
   if (blockIdx.x >= blocks) {
     look_at_sequences(A, blockIdx.x - blocks);
@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
   __shared__ float both[2][SHARED ? kThreads * kBatch : 1];
   const int cblk = blockIdx.x % A.plan.channel_blocks;
   const int64_t group = blockIdx.x / A.plan.channel_blocks;
-  const Place p = place_of<V, SHARED>(A, group, cblk);
+  const auto p = place_of<V, SHARED, ST>(A, group, cblk);
   if (!SHARED && !p.on) return;
   const int64_t xs = along(A, A.x_stride), gs = along(A, A.gate_stride), ds = along(A, A.dh_stride);
   const int64_t ts = along(A, A.channels), os = along(A, A.gates);
@@ -42,7 +42,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
   float v_in[V];  // what the row after hands down
 #pragma unroll
   for (int v = 0; v < V; ++v) v_in[v] = 0.f;
-  if (A.carry != nullptr && p.on) load_kept<V>(A.carry, A, p.chunk, p.c, v_in);
+  if (A.carry != nullptr && p.on) load_kept(A.carry, A, p.chunk, p, v_in);
   for (int b = A.plan.kept - 1; b >= 0; --b) {
     float *sums = both[b & 1];
     const int64_t t = p.t0 + (int64_t)b * kBatch;
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
     if (n > 0) {
       const int row = (int)row_at(A, t);
       Pack<XT, V> x[kBatch], dh[kBatch];
-      Gates<GT, V, SHARED> g[kBatch];
+      Gates<GT, V, SHARED, ST> g[kBatch];
       {
         const XT *from = reinterpret_cast<const XT *>(A.x) + row * A.x_stride + p.c;
         const GT *gate = reinterpret_cast<const GT *>(A.gate) + row * A.gate_stride + p.g;
@@ -58,12 +58,12 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
 #pragma unroll
         for (int k = 0; k < kBatch; ++k)
           if (k < n) {
-            x[k] = load_pack<XT, V>(from);
-            g[k].load(gate);
+            x[k] = load_pack<XT, V, ST>(from, p);
+            g[k].load(gate, p);
             from += xs;
             gate += gs;
             if (A.dh != nullptr) {
-              dh[k] = load_pack<XT, V>(grad);
+              dh[k] = load_pack<XT, V, ST>(grad, p);
               grad += ds;
             } else {
 #pragma unroll
@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
       }
       float before[kBatch][V];  // the state before each row
       float h[V];
-      load_kept<V>(A.saved, A, p.chunk * A.plan.kept + b, p.c, h);
+      load_kept(A.saved, A, p.chunk * A.plan.kept + b, p, h);
       const int last = row + (n - 1) * one, low = A.reverse ? last : row;
       XT *to = reinterpret_cast<XT *>(A.dx) + (int64_t)last * A.channels + p.c;
       GT *out = reinterpret_cast<GT *>(A.dgate) + (int64_t)last * A.gates + p.c;
@@ -88,12 +88,12 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
           before[k][v] = u;
           v_in[v] = inside ? g[k](v) * u : 0.f;
         }
-        store_pack<XT, V>(to, before[k]);
+        store_pack<XT, V, ST>(to, before[k], p);
         to -= ts;
         if (SHARED) {
           sum_at[k * A.plan.tx] = sum;
         } else {
-          store_pack<GT, V>(out, dg);
+          store_pack<GT, V, ST>(out, dg, p);
           out -= os;
         }
       };
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
           if (k >= n) break;
           if (firsts >> k & 1) {
             q.seek(A, row + k * one);
-            load_state<V>(A.initial, A, q.s, p.c, h);
+            load_state(A.initial, A, q.s, p, h);
           }
 #pragma unroll
           for (int v = 0; v < V; ++v) {
@@ -140,12 +140,12 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
           if (k >= n) continue;
           if (lasts >> k & 1) {
             q.seek(A, row + k * one);
-            load_state<V>(A.dfinal, A, q.s, p.c, v_in);
+            load_state(A.dfinal, A, q.s, p, v_in);
           }
           finish(k, !(outside >> k & 1));
           if ((firsts >> k & 1) && A.dinitial != nullptr) {
             q.seek(A, row + k * one);
-            store_state<V>(A.dinitial, A, q.s, p.c, v_in);
+            store_state(A.dinitial, A, q.s, p, v_in);
           }
         }
       }
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
     if (SHARED) {
       // The sums of the threads that share a gate, in their order.
       __syncthreads();
-      const int width = A.plan.tx * V, c0 = cblk * width, c1 = c0 + width < A.channels ? c0 + width : A.channels;
+      const int width = A.plan.width, c0 = cblk * width, c1 = c0 + width < A.channels ? c0 + width : A.channels;
       const int first = c0 / A.per_gate, count = (c1 - 1) / A.per_gate - first + 1;
       // kParts adjacent lanes share a sum.
       const int all = A.plan.cy * kBatch * count;
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
 // The gates whose channels lie in several blocks: their parts added in order.
 template <typename GT>
 __global__ void __launch_bounds__(kThreads) join_gates_kernel(const __grid_constant__ Args A) {
-  const int width = A.plan.tx * A.plan.vec;
+  const int width = A.plan.width;
   const int64_t n = A.rows * A.gates, stride = (int64_t)gridDim.x * kThreads;
   for (int64_t k = (int64_t)blockIdx.x * kThreads + threadIdx.x; k < n; k += stride) {
     const int gate = (int)(k % A.gates);
@@ -201,16 +201,16 @@ __global__ void __launch_bounds__(kThreads) join_gates_kernel(const __grid_const
   }
 }
 
-template <typename XT, typename GT, int V, bool SHARED>
+template <typename XT, typename GT, int V, bool SHARED, bool ST>
 static int launch_backward(const Args &A, cudaStream_t st) {
   if (A.carry != nullptr) {
     const unsigned blocks = grid_of(A.plan);
-    maps_kernel<XT, GT, V, SHARED, true><<<blocks + extra_blocks(A), kThreads, 0, st>>>(A, blocks);
+    maps_kernel<XT, GT, V, SHARED, ST, true><<<blocks + extra_blocks(A), kThreads, 0, st>>>(A, blocks);
     count_launch();
     const int rc = launch_carry(A, true, st);
     if (rc) return rc;
   }
-  const int rc = launch_walk(backward_kernel<XT, GT, V, SHARED>, A, st);
+  const int rc = launch_walk(backward_kernel<XT, GT, V, SHARED, ST>, A, st);
   if (rc) return rc;
   if (A.partial != nullptr && A.rows > 0) {
     const int64_t want = (A.rows * A.gates + kThreads - 1) / kThreads;
@@ -224,10 +224,13 @@ template <typename XT, typename GT>
 static int pick_backward(const Args &A, cudaStream_t st) {
   constexpr int kPer = 8 / (int)(sizeof(XT) > sizeof(GT) ? sizeof(XT) : sizeof(GT));
   constexpr int kShared = 8 / (int)sizeof(XT);
+  constexpr bool kApart = sizeof(XT) == 2 && sizeof(GT) == 2;
   const bool shared = A.per_gate > 1;
+  if (A.plan.step) return launch_backward<XT, GT, kApart ? 2 : 1, false, kApart>(A, st);
   if (A.plan.vec == 1)
-    return shared ? launch_backward<XT, GT, 1, true>(A, st) : launch_backward<XT, GT, 1, false>(A, st);
-  return shared ? launch_backward<XT, GT, kShared, true>(A, st) : launch_backward<XT, GT, kPer, false>(A, st);
+    return shared ? launch_backward<XT, GT, 1, true, false>(A, st) : launch_backward<XT, GT, 1, false, false>(A, st);
+  return shared ? launch_backward<XT, GT, kShared, true, false>(A, st)
+                : launch_backward<XT, GT, kPer, false, false>(A, st);
 }
 
 }  // namespace scan
@@ -253,7 +256,7 @@ extern "C" int gs_gated_scan_backward(int64_t rows, int sequences, int channels,
     return GS_ERR_INVALID_ARGUMENT;
   Args A{};
   A.plan = make_plan(rows, sequences, even, channels, gates, x_type, gate_type);
-  const int xb = type_bytes(x_type), gb = type_bytes(gate_type), vec = A.plan.vec;
+  const int xb = type_bytes(x_type), gb = type_bytes(gate_type), vec = A.plan.step ? 1 : A.plan.vec;
   const bool shared = channels != gates;
   if (!suits(x, x_row_stride, xb, vec) || !suits(grad_x, channels, xb, vec) ||
       !suits(grad_h, grad_h_row_stride, xb, vec) ||

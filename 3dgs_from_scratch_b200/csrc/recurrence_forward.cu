@@ -17,16 +17,34 @@ Plan make_plan(int64_t rows, int sequences, bool even, int channels, int gates, 
   // 8 bytes of the wider type a row and thread: 16 leave too few threads, and
   // the backward short of registers.
   const int wide = 8 / (shared ? xb : xb > gb ? xb : gb);
-  p.vec = (shared ? per : channels) % wide == 0 ? wide : 1;
-  const int vectors = channels / p.vec, one = shared ? per / p.vec : 1;  // vectors of a gate
-  p.channel_blocks = (vectors + kThreads - 1) / kThreads;
-  p.tx = (vectors + p.channel_blocks - 1) / p.channel_blocks;
-  if (one <= kThreads) {  // whole gates in a block, where they fit
-    p.tx = (p.tx + one - 1) / one * one;
-    if (p.tx > kThreads) p.tx = kThreads / one * one;
-    p.channel_blocks = (vectors + p.tx - 1) / p.tx;
+  if ((shared ? per : channels) % wide == 0) {
+    p.vec = wide;
+    p.step = 0;
+  } else {
+    // In 16 bits two channels a thread, tx apart, so that the threads of a row
+    // still read adjacent ones (bf16, 65,536 rows x 333 channels: forward 76 us
+    // against 146 with one, with the backward 197 against 264; 524,288 x 35: 64
+    // against 83, 158 against 175; few rows even out, 4096 x 35: 13.1 against
+    // 13.9, 32 against 28). One a thread in 32 bits (524,288 x 35: 80 and 191
+    // against 93 and 212 with two), where channels share gates (333 with one
+    // gate: 205 against 213 with the backward) and up to a warp's channels
+    // (2,097,152 x 3: 230 against 258).
+    p.step = !shared && xb == 2 && gb == 2 && channels > 32;
+    p.vec = p.step ? 2 : 1;
   }
+  const int most = kThreads * p.vec, one = shared ? per : 1;  // channels of a block, of a gate
+  p.channel_blocks = (channels + most - 1) / most;
+  p.width = (channels + p.channel_blocks - 1) / p.channel_blocks;
+  if (!p.step) p.width = (p.width + p.vec - 1) / p.vec * p.vec;
+  if (one <= most) {  // whole gates in a block, where they fit
+    p.width = (p.width + one - 1) / one * one;
+    if (p.width > most) p.width = most / one * one;
+  }
+  p.channel_blocks = (channels + p.width - 1) / p.width;
+  p.tx = (p.width + p.vec - 1) / p.vec;
+  p.step *= p.tx;
   p.cy = kThreads / p.tx;
+  const int vectors = (channels + p.vec - 1) / p.vec;
   // Rows of a chunk: about kFill threads on each of 148 SMs.
   const int64_t want = rows * vectors / (148 * kFill);
   const int64_t period = even ? rows / sequences : 0;
@@ -43,8 +61,7 @@ Plan make_plan(int64_t rows, int sequences, bool even, int channels, int gates, 
   }
   p.chunks = rows > 0 ? (rows + p.chunk - 1) / p.chunk : 0;
   p.kept = (p.chunk + kBatch - 1) / kBatch;
-  const int width = p.tx * p.vec;
-  p.slots = shared && width % per != 0 ? (per + width - 2) / width + 1 : 1;
+  p.slots = shared && p.width % per != 0 ? (per + p.width - 2) / p.width + 1 : 1;
   return p;
 }
 
@@ -162,14 +179,14 @@ int launch_carry(const Args &A, bool back, cudaStream_t st) {
   return GS_OK;
 }
 
-template <typename XT, typename GT, int V, bool SHARED>
+template <typename XT, typename GT, int V, bool SHARED, bool ST>
 __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant__ Args A, unsigned blocks) {
   if (blockIdx.x >= blocks) {
     look_at_sequences(A, blockIdx.x - blocks);
     return;
   }
-  const Place p =
-      place_of<V, SHARED>(A, blockIdx.x / A.plan.channel_blocks, blockIdx.x % A.plan.channel_blocks);
+  const auto p =
+      place_of<V, SHARED, ST>(A, blockIdx.x / A.plan.channel_blocks, blockIdx.x % A.plan.channel_blocks);
   if (!p.on) return;
   int row = (int)row_at(A, p.t0);
   const int64_t xs = along(A, A.x_stride), gs = along(A, A.gate_stride), hs = along(A, A.channels);
@@ -184,29 +201,29 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
   float h[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) h[v] = 0.f;
-  if (A.carry != nullptr) load_kept<V>(A.carry, A, p.chunk, p.c, h);
+  if (A.carry != nullptr) load_kept(A.carry, A, p.chunk, p, h);
   int64_t kept = p.chunk * A.plan.kept;
   // Rows to the next event: the first row of a sequence, or of rows outside.
   bool inside = q.holds(row);
   int event = inside && q.first(A, row) || !inside ? 0 : q.rest(A, row);
   for (int left = (int)(p.t1 - p.t0); left > 0; left -= kBatch) {
     Pack<XT, V> x[kBatch];
-    Gates<GT, V, SHARED> g[kBatch];
+    Gates<GT, V, SHARED, ST> g[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k)
       if (k < left) {
-        x[k] = load_pack<XT, V>(from);
-        g[k].load(gate);
+        x[k] = load_pack<XT, V, ST>(from, p);
+        g[k].load(gate, p);
         from += xs;
         gate += gs;
       }
-    if (A.saved != nullptr) store_kept<V>(A.saved, A, kept++, p.c, h);
+    if (A.saved != nullptr) store_kept(A.saved, A, kept++, p, h);
     if (inside && event > kBatch && left >= kBatch) {
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = fmaf(g[k](v), h[v], to_f32<XT>(x[k].e[v]));
-        store_pack<XT, V>(to, h);
+        store_pack<XT, V, ST>(to, h, p);
         to += hs;
       }
     } else {
@@ -218,7 +235,7 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
           q.seek(A, at);
           inside = q.holds(at);
           event += q.rest(A, at);
-          if (inside) load_state<V>(A.initial, A, q.s, p.c, h);
+          if (inside) load_state(A.initial, A, q.s, p, h);
         }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -226,8 +243,8 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
           if (!inside) h[v] = 0.f;
         }
         if (k + 1 == event && inside && A.final_state != nullptr)
-          store_state<V>(A.final_state, A, q.s, p.c, h);
-        store_pack<XT, V>(to, h);
+          store_state(A.final_state, A, q.s, p, h);
+        store_pack<XT, V, ST>(to, h, p);
         to += hs;
       }
     }
@@ -236,25 +253,29 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const __grid_constant
   }
 }
 
-template <typename XT, typename GT, int V, bool SHARED>
+template <typename XT, typename GT, int V, bool SHARED, bool ST>
 static int launch_forward(const Args &A, cudaStream_t st) {
   if (A.carry != nullptr) {
     const unsigned blocks = grid_of(A.plan);
-    maps_kernel<XT, GT, V, SHARED, false><<<blocks + extra_blocks(A), kThreads, 0, st>>>(A, blocks);
+    maps_kernel<XT, GT, V, SHARED, ST, false><<<blocks + extra_blocks(A), kThreads, 0, st>>>(A, blocks);
     count_launch();
     const int rc = launch_carry(A, false, st);
     if (rc) return rc;
   }
-  return launch_walk(forward_kernel<XT, GT, V, SHARED>, A, st);
+  return launch_walk(forward_kernel<XT, GT, V, SHARED, ST>, A, st);
 }
 
 template <typename XT, typename GT>
 static int pick_forward(const Args &A, cudaStream_t st) {
   constexpr int kPer = 8 / (int)(sizeof(XT) > sizeof(GT) ? sizeof(XT) : sizeof(GT));
   constexpr int kShared = 8 / (int)sizeof(XT);
+  constexpr bool kApart = sizeof(XT) == 2 && sizeof(GT) == 2;
   const bool shared = A.per_gate > 1;
-  if (A.plan.vec == 1) return shared ? launch_forward<XT, GT, 1, true>(A, st) : launch_forward<XT, GT, 1, false>(A, st);
-  return shared ? launch_forward<XT, GT, kShared, true>(A, st) : launch_forward<XT, GT, kPer, false>(A, st);
+  if (A.plan.step) return launch_forward<XT, GT, kApart ? 2 : 1, false, kApart>(A, st);
+  if (A.plan.vec == 1)
+    return shared ? launch_forward<XT, GT, 1, true, false>(A, st) : launch_forward<XT, GT, 1, false, false>(A, st);
+  return shared ? launch_forward<XT, GT, kShared, true, false>(A, st)
+                : launch_forward<XT, GT, kPer, false, false>(A, st);
 }
 
 // What both directions check of their sizes and types.
@@ -308,7 +329,7 @@ extern "C" int gs_gated_scan_forward(int64_t rows, int sequences, int channels, 
   if (rows > 0 && (x == nullptr || gate == nullptr || h == nullptr)) return GS_ERR_INVALID_ARGUMENT;
   Args A{};
   A.plan = make_plan(rows, sequences, even, channels, gates, x_type, gate_type);
-  const int xb = type_bytes(x_type), gb = type_bytes(gate_type), vec = A.plan.vec;
+  const int xb = type_bytes(x_type), gb = type_bytes(gate_type), vec = A.plan.step ? 1 : A.plan.vec;
   const bool shared = channels != gates;
   if (!suits(x, x_row_stride, xb, vec) || !suits(h, channels, xb, vec) ||
       !suits(gate, gate_row_stride, gb, shared ? 1 : vec) ||

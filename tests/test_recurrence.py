@@ -131,6 +131,15 @@ def test_types_and_ragged_sequences(gs, dtype, gate_dtype, channels, gates, reve
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("channels", [33, 34, 75, 513, 1025, 1282])
+def test_sixteen_bit_channels_that_fill_no_vectors(gs, dtype, channels):
+    check(gs, 300, 5, channels, channels, offsets=[0, 131, 131, 250, 251, 297], dtype=dtype,
+          gate_dtype=dtype, reverse=channels % 2 == 0, seed=channels)
+    check(gs, 96, 3, channels, channels, dtype=dtype, gate_dtype=dtype, with_initial=False, seed=channels)
+
+
+@gpu
 @pytest.mark.parametrize("reverse", [False, True])
 def test_rows_before_the_first_sequence_and_no_rows_inside(gs, reverse):
     check(gs, 300, 2, 24, 24, offsets=[130, 135, 200], reverse=reverse)
