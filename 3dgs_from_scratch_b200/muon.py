@@ -85,7 +85,8 @@ def muon_step(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor, l
     sqrt(max(1, rows / cols)).
 
     param and momentum are float32 and contiguous, (rows, cols) or a
-    (batch, rows, cols) stack; grad has their shape, of any supported type.
+    (batch, rows, cols) stack; grad has their shape, of any supported type. The
+    three share no memory.
     Like the Adam step it is skipped while the device status word holds an
     error of an earlier kernel (gs_check_status)."""
     _check_matrices("muon_step", param)
@@ -99,6 +100,10 @@ def muon_step(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor, l
         raise ValueError("muon_step runs on CUDA tensors of one device")
     if not param.is_contiguous() or not momentum.is_contiguous():
         raise ValueError("muon_step updates contiguous tensors")
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+                   for t in (param, momentum, grad) if t.is_contiguous())
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("param, grad and momentum must not share memory")
     if not 0.0 <= beta < 1.0:
         raise ValueError("beta must be in [0, 1)")
     dev, (rows, cols) = param.device, param.shape[-2:]

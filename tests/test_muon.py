@@ -294,6 +294,18 @@ def test_refuses_wrong_steps_and_parameters(gs):
         gs.muon_step(x, x, x, 0.1, beta=1.0)
 
 
+@gpu
+def test_refuses_tensors_that_share_memory(gs):
+    whole = torch.ones(3, 4, 6, device=DEV)
+    a, b, c = whole
+    flat = whole.reshape(-1)
+    for args in ((a, b, a), (a, a, b), (a, b, b), (a, flat[30:54].view(4, 6), c),
+                 (flat[12:36].view(4, 6), c, a)):
+        with pytest.raises(ValueError, match="share"):
+            gs.muon_step(*args, 0.1)
+    gs.muon_step(a, b, c, 0.1)  # neighbours
+
+
 def test_entry_points_refuse_bad_arguments(gs):
     lib = gs.load_native()
     nat = importlib.import_module("3dgs_from_scratch_b200._native")
