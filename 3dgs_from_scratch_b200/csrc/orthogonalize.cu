@@ -8,9 +8,10 @@
 //
 // Numbers. The products run on the tensor cores with fp16 operands and fp32
 // accumulators. A value is held as hi + lo, two fp16 numbers (22 bits), scaled
-// by 2^12 so that neither leaves fp16's range: |X|_2 and |B|_2 stay below 8
-// (checked by the host for the given coefficients), and a typical entry of
-// even the largest matrix is far above the smallest normal number.
+// by 2^12 so that neither leaves fp16's range, which ends at 15.99: |X|_2 and
+// |B|_2 stay below 8 and |A|_2 = |X|_2^2 below 15 (checked by the host for the
+// given coefficients), and a typical entry of even the largest matrix is far
+// above the smallest normal number.
 //   full (fp32 and fp16 results): every product is hi hi + hi lo + lo hi. The
 //     tensor core cuts its fp32 sums off instead of rounding them, a bias that
 //     grows with the number of additions (2.6e-5 of the result at 4096 x 4096
@@ -1253,14 +1254,17 @@ static int launch_small(const SmallArgs &A, int batch, cudaStream_t st) {
   return GS_OK;
 }
 
-// The largest |X|_2 and |b A + c A A|_2 that the steps can reach from
-// |X|_2 <= 1, from the extremes of the two polynomials on [0, r]. Both have to
-// stay below 8 for the fp16 range.
+// The largest |X|_2, |A|_2 and |b A + c A A|_2 that the steps can reach from
+// |X|_2 <= 1, from the extremes of the two polynomials on [0, r]. X and B have
+// to stay below 8 for the fp16 range, and A = X X^T, which each step starts
+// with, below 15: 6% below the range's end, for the rounding of what led there.
+constexpr double kMostA = 15.0;
 static bool in_range(int steps, double a, double b, double c) {
   double r = 1.0;
   for (int k = 0; k < steps; ++k) {
     const auto p = [&](double s) { return fabs(s * (a + s * s * (b + s * s * c))); };
     const auto q = [&](double y) { return fabs(y * (b + y * c)); };
+    if (!(r * r < kMostA)) return false;
     double most = p(r), poly = q(r * r);
     // p'(s) = a + 3 b s^2 + 5 c s^4
     const double disc = 9 * b * b - 20 * a * c;

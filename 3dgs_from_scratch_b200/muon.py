@@ -53,8 +53,8 @@ def orthogonalize(update: torch.Tensor, steps: int = 5, coefficients=COEFFICIENT
 
     (rows, cols) or (batch, rows, cols), each matrix by itself; any strides;
     float32, bfloat16 or float16. Returns a new contiguous tensor of the same
-    shape and type. Coefficients under which the singular values or the
-    products' polynomial could pass 8 are refused. Not differentiable: the
+    shape and type. Coefficients under which the singular values or b A + c A A
+    could pass 8, or A itself 15, are refused. Not differentiable: the
     result is detached."""
     _check_matrices("orthogonalize", update)
     _check_steps("orthogonalize", steps, coefficients, eps)

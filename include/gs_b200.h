@@ -635,7 +635,8 @@ GS_API int gs_gated_scan_backward(int64_t rows, int sequences, int channels, int
  *
  * 1 <= batch <= 65535, rows and cols <= 2^24, the smaller <= 2^15;
  * 1 <= steps <= 100; eps > 0. The coefficients have to keep |X|_2 and |B|_2
- * below 8 through all steps (GS_ERR_INVALID_ARGUMENT otherwise). Strides of U
+ * below 8 and |A|_2 below 15 through all steps (GS_ERR_INVALID_ARGUMENT
+ * otherwise): so X has to be below 3.87 where a step follows. Strides of U
  * in elements, any that are not negative; out is contiguous (batch, rows,
  * cols) of U's type and does not overlap U. Scratch: 16-byte aligned. A
  * non-finite U gives non-finite results. */

@@ -330,3 +330,45 @@ def test_entry_points_refuse_bad_arguments(gs):
     assert lib.gs_orthogonalize_scratch_bytes(0, 8, 8, 0) == 0
     one = lib.gs_orthogonalize_scratch_bytes(1, 300, 500, 0)
     assert 0 < one < lib.gs_orthogonalize_scratch_bytes(2, 300, 500, 0)
+
+
+# Quintics whose steps stay below 8 in X and in b A + c A A while A passes fp16's range at 2^12
+# (15.99): the second step starts from |X|_2 = 4.2, 4.7 and (a Chebyshev polynomial on [0, 7.9]) 4.68.
+TOO_LARGE = [(4.5, -0.3, 0.0), (5.0, -0.3, 0.0), (5.0, -20.0 / 7.9 ** 2, 16.0 / 7.9 ** 4)]
+LARGEST = (3.9, -0.2, 0.0)      # from 3.7: A reaches 13.7
+
+
+def test_coefficients_under_which_the_gram_matrix_leaves_the_range_are_refused(gs):
+    lib = gs.load_native()
+    nat = importlib.import_module("3dgs_from_scratch_b200._native")
+    at = 0x10000
+
+    def run(steps, abc, rows=8):
+        ortho = lib.gs_orthogonalize(1, rows, 300, 0, at, 0, 300, 1, at, steps, *abc, 1e-7, at, 0, None)
+        muon = lib.gs_muon_step(1, rows, 300, 0, at, at, at, 0.1, 0.9, 1, 0.0, 1.0, steps, *abc, 1e-7, at, 0, None)
+        assert ortho == muon
+        return ortho
+
+    for rows in (8, 200):
+        for abc in TOO_LARGE:
+            assert run(2, abc, rows) == nat.GS_ERR_INVALID_ARGUMENT, abc
+            assert run(1, abc, rows) == nat.GS_ERR_CAPACITY, abc     # A of the only step is at most 1
+        assert run(2, LARGEST, rows) == nat.GS_ERR_CAPACITY
+
+
+@gpu
+@pytest.mark.parametrize("m,n", [(1, 70), (60, 90), (100, 900), (300, 500)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_the_largest_values_that_are_accepted(gs, m, n, dtype):
+    """One entry: X is 1, 3.7 and then 3.9 * 3.7 - 0.2 * 3.7^3 = 4.30, and sums have one term. Values
+    are held to e = 2^-22 (bf16 runs: A, B and the X inside A to e = 2^-11). The first step's error is
+    at most (3.9 2^-22 + 6 * 0.2 e) / 3.7, which the second multiplies by |p'| s / p = 3.7, and that
+    one's own (3.9 * 3.7 * 2^-22 + 6 * 0.2 * 3.7^3 e) / 4.3: 23 * 2^-22, or 16 * 2^-11 in bf16."""
+    u = torch.zeros(m, n)
+    u[m // 2, n // 3] = 2.0
+    got = gs.orthogonalize(u.to(DEV, dtype), steps=2, coefficients=LARGEST).double().cpu()
+    ref = plain(u, 2, LARGEST)
+    assert abs(float(ref.max()) - 4.2994) < 1e-4
+    tol = (23 * 2.0 ** -22 if dtype != BF16 else 16 * 2.0 ** -11) + torch.finfo(dtype).eps / 2
+    assert float((got - ref).abs().max()) <= tol * float(ref.max())
+    assert int((got != 0).sum()) == 1
