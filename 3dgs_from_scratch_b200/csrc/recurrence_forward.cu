@@ -72,12 +72,67 @@ Plan make_plan(int64_t rows, int sequences, bool even, int channels, int gates, 
 // each other's maps: one SM alone takes 14 us for 4096 chunks.
 constexpr int kCarryChannels = 4, kRuns = 128, kCarryBlocks = 8;
 
-template <bool BACK>
-__global__ void __launch_bounds__(kCarryChannels *kRuns) carry_kernel(const __grid_constant__ Args A, int blocks) {
-  __shared__ float2 maps[2][kRuns][kCarryChannels];
-  __shared__ uint32_t cuts[2][kRuns];
-  start_next();
-  wait_for_previous();
+// A run's map with P in fp32, for products of at most 1, and in the form that
+// holds any product.
+struct Narrow {
+  static constexpr int kAhead = 16;  // chunks on their way at a time; a run of no more is read once
+  float P, L;
+  __device__ static Narrow nothing() { return {1.f, 0.f}; }
+  __device__ static Narrow of(const Args &A, int64_t at) {
+    const float2 m = A.maps[at];
+    return {m.x, m.y};
+  }
+  __device__ bool cut() const { return __float_as_uint(P) == kCut; }
+  // What leaves the run that a state enters.
+  __device__ float through(float state) const { return cut() ? L : fmaf(P, state, L); }
+  // Becomes the map of `before` and then this.
+  __device__ void follow(const Narrow &before) {
+    L = through(before.L);
+    P = cut() ? P : before.cut() ? before.P : P * before.P;
+  }
+  __device__ bool grown() const { return !cut() && !(fabsf(P) <= 1.f); }
+};
+struct Broad {
+  static constexpr int kAhead = 4;
+  static constexpr int kCutExponent = INT32_MIN, kFarOut = 1 << 20;  // sums of two exponents stay integers
+  Wide P;
+  float L;
+  __device__ static Broad nothing() { return {{1.f, 0}, 0.f}; }
+  __device__ static Broad of(const Args &A, int64_t at) {
+    const float2 m = A.maps[at];
+    if (__float_as_uint(m.x) == kCut) return {{0.f, kCutExponent}, m.y};
+    const float size = fabsf(m.x);
+    return {size >= FLT_MIN && size <= FLT_MAX ? normal(m.x, 0) : A.products[at], m.y};
+  }
+  __device__ bool cut() const { return P.e == kCutExponent; }
+  // In three factors of 2^100 at most, which take any state of fp32 to 0 or to
+  // infinity, and a zero state to 0.
+  __device__ float through(float state) const {
+    const int e1 = within(P.e, 100), e2 = within(P.e - e1, 100), e3 = within(P.e - e1 - e2, 100);
+    return cut() ? L : fmaf(state * power_of_2(e1) * power_of_2(e2), P.m * power_of_2(e3), L);
+  }
+  __device__ void follow(const Broad &before) {
+    L = through(before.L);
+    if (cut()) return;
+    if (before.cut()) P = before.P;
+    else P = normal(P.m * before.P.m, within(P.e + before.P.e, kFarOut));
+  }
+  __device__ bool grown() const { return false; }
+};
+
+// What a block keeps in shared memory. More than these 9 KB would keep it from
+// running next to the walk, which starts before the scan has ended.
+template <class M>
+struct Scanned {
+  static constexpr int kBuffers = sizeof(M) == 8 ? 2 : 1;
+  M maps[kBuffers][kRuns][kCarryChannels];
+  M others[kCarryBlocks][kCarryChannels];
+  int grown;
+};
+
+// Returns whether (in the cluster) a chunk's product has grown; nothing is written then.
+template <bool BACK, class M>
+__device__ __forceinline__ bool carry_chunks(const Args &A, int blocks, Scanned<M> &S) {
   const int lane = threadIdx.x % kCarryChannels, run = threadIdx.x / kCarryChannels;
   const int rank = blocks > 1 ? (int)cluster_rank() : 0;
   const int c = blockIdx.x / blocks * kCarryChannels + lane;
@@ -85,76 +140,89 @@ __global__ void __launch_bounds__(kCarryChannels *kRuns) carry_kernel(const __gr
   const int64_t n = A.plan.chunks, b0 = n * rank / blocks, b1 = n * (rank + 1) / blocks;
   const int64_t k0 = b0 + (b1 - b0) * run / kRuns, k1 = b0 + (b1 - b0) * (run + 1) / kRuns;
   const int64_t step = BACK ? -1 : 1, first = BACK ? n - 1 - k0 : k0;
-  const float2 *__restrict__ map = A.maps + first * A.channels + (on ? c : 0);
-  const int *__restrict__ cut = A.cuts + first;
-  float *__restrict__ to = A.carry + first * A.channels + (on ? c : 0);
-  const int64_t row = step * A.channels;
-  // 16 chunks on their way at a time; a run of no more is read once.
-  constexpr int kAhead = 16;
+  float *__restrict__ to = A.carry + first * A.channels + c;
   const int len = (int)(k1 - k0);
-  float2 m[kAhead];
-  uint32_t here = 0;
+  M m[M::kAhead];
   const auto load = [&](int from) {
-    here = 0;
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (from + k < len) {
-        m[k] = map[(from + k) * row];
-        here |= cut[(from + k) * step] != 0 ? 1u << k : 0u;
-      }
+    for (int k = 0; k < M::kAhead; ++k)
+      if (from + k < len) m[k] = M::of(A, (first + (from + k) * step) * A.channels + (on ? c : 0));
   };
-  float P = 1.f, L = 0.f;
-  bool any = false;
-  for (int from = 0; from < len; from += kAhead) {
+  M mine = M::nothing();
+  bool grown = false;
+  for (int from = 0; from < len; from += M::kAhead) {
     load(from);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k)
+    for (int k = 0; k < M::kAhead; ++k)
       if (from + k < len) {
-        L = here >> k & 1 ? m[k].y : fmaf(m[k].x, L, m[k].y);
-        P *= m[k].x;
+        M now = m[k];
+        now.follow(mine);
+        mine = now;
+        grown = grown || m[k].grown();
       }
-    any = any || here != 0;
   }
   // Inclusive scan of the runs' maps, doubling the reach.
-  maps[0][run][lane] = make_float2(P, L);
-  if (lane == 0) cuts[0][run] = any;
+  S.maps[0][run][lane] = mine;
   __syncthreads();
   int at = 0;
-  for (int reach = 1; reach < kRuns; reach *= 2, at ^= 1) {
-    float2 now = maps[at][run][lane];
-    bool is_cut = cuts[at][run] != 0;
-    if (run >= reach) {
-      const float2 before = maps[at][run - reach][lane];
-      if (!is_cut) now.y = fmaf(now.x, before.y, now.y);
-      now.x *= before.x;
-      is_cut = is_cut || cuts[at][run - reach] != 0;
-    }
-    maps[at ^ 1][run][lane] = now;
-    if (lane == 0) cuts[at ^ 1][run] = is_cut;
-    __syncthreads();
+  for (int reach = 1; reach < kRuns; reach *= 2) {
+    if (run >= reach) mine.follow(S.maps[at][run - reach][lane]);
+    at = (at + 1) % S.kBuffers;
+    if (S.kBuffers == 1) __syncthreads();
+    S.maps[at][run][lane] = mine;
+    if (reach * 2 < kRuns) __syncthreads();
   }
+  grown = __syncthreads_or(grown);
   float h = 0.f;  // the state that enters the block's chunks, then the run's
   if (blocks > 1) {
+    if (threadIdx.x == 0) S.grown = grown;
     cluster_sync();
-    for (int q = 0; q < rank; ++q) {
-      const float2 f = cluster_load2(cluster_addr(&maps[at][kRuns - 1][lane], q));
-      h = cluster_load_u32(cluster_addr(&cuts[at][kRuns - 1], q)) ? f.y : fmaf(f.x, h, f.y);
+    int theirs = 0;
+    if ((int)threadIdx.x < blocks * kCarryChannels) {
+      const int q = threadIdx.x / kCarryChannels;
+      const uint32_t from = cluster_addr(&S.maps[at][kRuns - 1][lane], q);
+      uint32_t w[sizeof(M) / 4];
+#pragma unroll
+      for (int k = 0; k < (int)(sizeof(M) / 4); ++k) w[k] = cluster_load_u32(from + 4 * k);
+      memcpy(&S.others[q][lane], w, sizeof(M));
+      theirs = (int)cluster_load_u32(cluster_addr(&S.grown, q));
     }
     cluster_sync();  // no block leaves while another may read its maps
+    grown = __syncthreads_or(theirs);
+    for (int q = 0; q < rank; ++q) h = S.others[q][lane].through(h);
   }
-  if (!on) return;
-  if (run > 0) {
-    const float2 f = maps[at][run - 1][lane];
-    h = cuts[at][run - 1] ? f.y : fmaf(f.x, h, f.y);
-  }
-  for (int from = 0; from < len; from += kAhead) {
-    if (len > kAhead) load(from);
+  if (grown) return true;
+  if (!on) return false;
+  if (run > 0) h = S.maps[at][run - 1][lane].through(h);
+  for (int from = 0; from < len; from += M::kAhead) {
+    if (len > M::kAhead) load(from);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k)
+    for (int k = 0; k < M::kAhead; ++k)
       if (from + k < len) {
-        to[(from + k) * row] = h;
-        h = here >> k & 1 ? m[k].y : fmaf(m[k].x, h, m[k].y);
+        to[(from + k) * step * A.channels] = h;
+        h = m[k].through(h);
       }
+  }
+  return false;
+}
+
+// Out of line, so that the registers of the usual form stay its own.
+template <bool BACK>
+__device__ __noinline__ void carry_grown_chunks(const Args &A, int blocks, Scanned<Broad> &S) {
+  carry_chunks<BACK>(A, blocks, S);
+}
+
+template <bool BACK>
+__global__ void __launch_bounds__(kCarryChannels *kRuns) carry_kernel(const __grid_constant__ Args A, int blocks) {
+  __shared__ union {
+    Scanned<Narrow> narrow;
+    Scanned<Broad> broad;
+  } shared;
+  start_next();
+  wait_for_previous();
+  if (carry_chunks<BACK>(A, blocks, shared.narrow)) {
+    __syncthreads();  // the narrow form's maps are no longer read
+    carry_grown_chunks<BACK>(A, blocks, shared.broad);
   }
 }
 

@@ -455,3 +455,115 @@ def test_entry_points_refuse_bad_arguments(gs):
     assert lib.gs_gated_scan_scratch_bytes(24, 1, 1, 8, 8, 0, 0, 0) == 0
     assert lib.gs_gated_scan_scratch_bytes(1 << 20, 1, 1, 8, 8, 0, 0, 1) > 0
     assert lib.gs_gated_scan_scratch_bytes(1 << 20, 5, 0, 8, 8, 0, 0, 0) > 0
+
+
+def against(gs, x, gate, init, dh, dfinal, per, dtype, gate_dtype, reverse):
+    """One sequence against its definition, forward and backward; all given in the direction of the recurrence.
+
+    Values may fall below the normal range here, where an operation is off by up to q = 2^-150 besides the
+    relative half step (fp32's smallest step is 2^-149), and later gates multiply that as they multiply the
+    state. A row's product, its sum and a joining that ends there are three such operations, so states are
+    off by at most the recurrence on absolute values with x = 4 q (`low`) more than before (0 where the state
+    is exactly 0, as products and sums of zeros are), the gradients' chain likewise (`back`), and a gate's
+    gradient, a sum of products u h, by the products of the one's size and the other's error, and q a term."""
+    if reverse:
+        x, gate, dh = x.flip(0), gate.flip(0), dh.flip(0)
+    x, gate, dh = x.to(dtype), gate.to(gate_dtype), dh.to(dtype)
+    leaves = [t.to(DEV).requires_grad_(True) for t in (x, gate, init)]
+    h, final = gs.gated_scan(*leaves, reverse=reverse)
+    grads = torch.autograd.grad((h, final), leaves, (dh.to(DEV), dfinal.to(DEV)))
+    rows, bounds = x.shape[0], [(0, x.shape[0])]
+    X, G, DH = x.double(), gate.double().repeat_interleave(per, 1), dh.double()
+    I, DF = init.double(), dfinal.double()
+    H, FIN = walk(X, G, I, bounds, reverse)
+    HA, FA = walk(X.abs(), G.abs(), I.abs(), bounds, reverse)
+    DX, DG, DI = walk_back(G, DH, DF, I, H, bounds, reverse)
+    DXA, DGA, DIA = walk_back(G.abs(), DH.abs(), DF.abs(), I.abs(), HA, bounds, reverse)
+    assert max(float(t.detach().max()) for t in (HA, FA, DXA, DGA, DIA)) < 2.0 ** 127  # nothing overflows
+    q = 2.0 ** -150
+    low, low_end = walk(4 * q * (HA > 0), G.abs(), torch.zeros_like(I), bounds, reverse)
+    back, low_dg, low_di = walk_back(G.abs(), 4 * q * (DXA > 0), torch.zeros_like(I), I.abs(), HA + low,
+                                     bounds, reverse)       # low_dg: the chain's error times |h|
+    low_dg = low_dg + walk_back(G.abs(), DH.abs(), DF.abs(), torch.zeros_like(I), low, bounds, reverse)[1] + 4 * q
+    fold = lambda t: t.reshape(rows, -1, per).sum(2)  # noqa: E731
+
+    def close(name, got, ref, scale, floor, ops, kind):
+        got, half = got.detach().double().cpu(), torch.finfo(kind).eps / 2
+        tol = (1 + half) * (1.01 * ops * U * scale + 1.01 * floor) + half * ref.abs() + torch.finfo(kind).tiny * half * 2
+        bad = ~((got - ref).abs() <= tol)
+        assert not bool(bad.any()), (f"{name}: {int(bad.sum())} of {bad.numel()} off, the first at "
+                                     f"{bad.nonzero()[0].tolist()}: {got[bad][0]} and not {ref[bad][0]}")
+
+    ops = 2 * rows + 16
+    close("h", h, H, HA, low, ops, dtype)
+    close("final", final, FIN, FA, low_end, ops, F32)
+    close("dx", grads[0], DX, DXA, back, ops, dtype)
+    close("dgate", grads[1], fold(DG), fold(DGA), fold(low_dg), 4 * rows + 32 + per, gate_dtype)
+    close("dinitial", grads[2], DI, DIA, low_di, ops, F32)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,gate_dtype", [(F32, F32), (BF16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("rows,per,reverse", [(1000, 1, False), (1000, 1, True), (1000, 3, True), (50000, 1, False)])
+def test_gates_whose_product_leaves_the_range(gs, dtype, gate_dtype, rows, per, reverse):
+    """Gates of 2 and 1/2 over hundreds of rows: their products pass fp32's range (and over 50,000 rows
+    that of 64 bits) while every state and gradient stays inside. Values are powers of 2, so also 16-bit
+    gates hold them."""
+    kinds, at = 6, 700
+    x, gate = torch.zeros(rows, kinds), torch.ones(rows, kinds)
+    dh, init, dfinal = torch.zeros(rows, kinds), torch.zeros(1, kinds), torch.zeros(1, kinds)
+    gate[:, 0] = 2.0                                       # a zero state up to the last row
+    x[-1, 0], dh[0, 0] = 3.0, 1.5                          # and a zero gradient down to the first
+    gate[:, 1] = 2.0                                       # the same up to a reset
+    gate[at, 1], x[at, 1], dh[at, 1] = 0.0, 1.0, 1.0
+    gate[at + 1:, 1] = 0.5
+    gate[at:at + 240, 2], init[0, 2] = 2.0, 2.0 ** -120    # a small state that grows
+    gate[at:at + 200, 3], gate[at + 200:at + 290, 3] = 0.5, 2.0   # a large one that decays and grows again
+    init[0, 3], dh[at + 100, 3] = 2.0 ** 60, 1.0
+    gate[:at, 4], x[at, 4], dh[at, 4] = 2.0, 1.0, 2.0 ** -100     # a gradient between large gates
+    gate[at - 150:at, 5], gate[at:at + 150, 5] = 2.0, 0.5  # up and down again
+    init[0, 5], dfinal[0, 5] = 2.0 ** -60, 1.0
+    gate[:at - 200, 4] = 1.0
+    more = lambda t: t.repeat_interleave(per, 1)  # noqa: E731
+    against(gs, more(x), gate, more(init), more(dh), more(dfinal), per, dtype, gate_dtype, reverse)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,gate_dtype", [(F32, F32), (BF16, BF16), (BF16, F32), (F16, F16), (F16, F32)])
+@pytest.mark.parametrize("channels,gates", [(1, 1), (3, 1), (40, 40), (40, 1), (40, 5), (21, 21), (35, 35), (301, 1), (1040, 2)])
+def test_finite_inputs_give_finite_results(gs, dtype, gate_dtype, channels, gates):
+    gen = torch.Generator(device=DEV).manual_seed(channels)
+    for rows, sequences, offsets in ((700, 7, None), (4100, 1, None), (1283, 6, [0, 0, 700, 700, 701, 1280, 1280])):
+        shape = (rows,) if offsets else (sequences, rows // sequences)
+        leaves = [torch.randn(*shape, channels, generator=gen, device=DEV).to(dtype),
+                  torch.rand(*shape, gates, generator=gen, device=DEV).to(gate_dtype),
+                  torch.randn(sequences, channels, generator=gen, device=DEV)]
+        leaves = [t.requires_grad_(True) for t in leaves]
+        offs = None if offsets is None else torch.tensor(offsets, device=DEV)
+        for reverse in (False, True):
+            h, final = gs.gated_scan(*leaves, offsets=offs, reverse=reverse)
+            grads = torch.autograd.grad((h, final), leaves, (torch.ones_like(h), torch.ones_like(final)))
+            assert all(bool(torch.isfinite(t).all()) for t in (h, final) + grads)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [3000, 60000])
+def test_gates_that_grow_cost_little_more(gs, rows):
+    """Products that leave the range take the chain's other form, not another order of magnitude."""
+    x = torch.randn(rows, 64, device=DEV) * 1e-30
+    times = []
+    for high in (1.0, 1.02):
+        g = torch.where(torch.rand(rows, 64, device=DEV) < 0.01, 0.0, high)
+        for _ in range(3):
+            h, _ = gs.gated_scan(x, g)
+        start, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        best = float("inf")
+        for _ in range(10):
+            start.record()
+            gs.gated_scan(x, g)
+            end.record()
+            end.synchronize()
+            best = min(best, start.elapsed_time(end))
+        times.append(best)
+        assert bool(torch.isfinite(h).all())
+    assert times[1] < 4 * times[0] + 0.1, times
