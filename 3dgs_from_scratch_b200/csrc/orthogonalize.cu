@@ -58,8 +58,7 @@ struct Matrix {        // planes of blocks [row block][column block]
 struct Out {
   void *p;             // the result, or the weights that it updates; null: none
   int type;            // GS_TYPE_*
-  int update;          // p = decay p - step X instead of p = X; skipped like the momentum
-                       // while the device status word is set
+  int update;          // p = decay p - step X instead of p = X, unless the call's gate is closed
   int tall;            // X is the transpose
   int rows, cols;      // of X
   int64_t batch_stride;
@@ -74,7 +73,20 @@ struct Args {
   float a, b, c;
   Out out;
   uint32_t *status;
+  uint32_t *gate;      // of an optimizer step: not 0: nothing is updated; null otherwise
 };
+
+// The optimizers' gate, read once for all launches and blocks of a step: a status
+// word that another stream sets meanwhile skips the next step, never a part of
+// this one. A wait that runs out inside the step closes it as well.
+__global__ void gate_kernel(const uint32_t *status, uint32_t *gate) {
+  start_next();
+  *gate = ld_volatile_u32(status);
+}
+__device__ __forceinline__ void report_timeout(uint32_t *status, uint32_t *gate) {
+  atomicCAS(status, 0u, (uint32_t)GS_ERR_DEVICE_TIMEOUT);
+  if (gate != nullptr) atomicExch(gate, (uint32_t)GS_ERR_DEVICE_TIMEOUT);
+}
 
 __device__ __forceinline__ char *block_at(char *plane, const Matrix &M, int batch, int rb, int cb) {
   return plane + (int64_t)batch * M.batch_bytes + ((int64_t)rb * M.column_blocks + cb) * kBlockBytes;
@@ -474,7 +486,8 @@ __global__ void __launch_bounds__(Shape<BN, KIND, FULL, CTAS>::kThreads, 1)
         }
       }
       if (!good) break;
-      if (A.out.update && ld_volatile_u32(A.status) != 0u) continue;  // the optimizers' gate
+      // One lane reads, so that the warp stays together.
+      if (A.out.update && __shfl_sync(0xffffffffu, lane_id() == 0 ? ld_volatile_u32(A.gate) : 0u, 0) != 0u) continue;
 #pragma unroll
       for (int c = 0; c < S::kHeld; c += 64) {
         if (KIND != kGram && !kAhead) {
@@ -518,7 +531,7 @@ __global__ void __launch_bounds__(Shape<BN, KIND, FULL, CTAS>::kThreads, 1)
   tc::fence_before();
   __syncthreads();
   if (CTAS == 2) cluster_sync();  // neither block leaves while the other may reach into it
-  if (threadIdx.x == 0 && failed) atomicCAS(A.status, 0u, (uint32_t)GS_ERR_DEVICE_TIMEOUT);
+  if (threadIdx.x == 0 && failed) report_timeout(A.status, A.gate);
   if (warp == 1) {
     tc::fence_after();
     tc::tmem_free<CTAS>(tmem, S::kColumns);
@@ -613,10 +626,10 @@ constexpr int kNormThreads = 256, kMaxParts = 296;
 // the range; the momentum is updated on the way. A matrix in one
 // piece is read in 16-byte loads, others a line at a time along the smaller
 // stride. Parts are added in order by the reader.
-__global__ void __launch_bounds__(kNormThreads) norm_kernel(const Source s, double *parts,
-                                                            const uint32_t *status) {
+__global__ void __launch_bounds__(kNormThreads) norm_kernel(const Source s, double *parts, const uint32_t *gate) {
   start_next();
-  if (s.momentum != nullptr && ld_volatile_u32(status) != 0u) return;
+  wait_for_previous();
+  if (gate != nullptr && *gate != 0u) return;
   const int64_t base = (int64_t)blockIdx.y * s.batch_stride;
   const bool cols_fast = s.col_stride <= s.row_stride;
   const int64_t lines = cols_fast ? s.rows : s.cols, len = cols_fast ? s.cols : s.rows;
@@ -767,7 +780,7 @@ struct SmallArgs {
   float a, b, c;
   double eps;
   char *shared;  // of a matrix's blocks: their parts of A, then A's planes
-  uint32_t *status;
+  uint32_t *status, *gate;
 };
 
 // X has up to MC rows. The MMAs' M is 128: what their rows beyond MC hold is
@@ -842,7 +855,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
   if (warp == 0) tc::tmem_alloc<1>(&tmem_base, 2 * S::kTop);
   // Skipped optimizer steps run through, so that the blocks of a cluster stay
   // together, and write nothing.
-  const bool skip = A.out.update && ld_volatile_u32(A.status) != 0u;
+  wait_for_previous();
+  bool skip = A.gate != nullptr && *A.gate != 0u;
 
   // The update, 8 columns of a row at a time, and its sum of squares.
   constexpr int kEach = MC * NC / 8 / kSmallThreads;
@@ -924,6 +938,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
   const bool on = quarter * 32 < MC;  // the warp's rows are X's
   const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
   uint32_t phase = 0;
+  bool timed_out = false;
   const auto run = [&](auto issue) {  // what was written is read by the tensor core
     fence_proxy_async_smem();
     tc::fence_before();
@@ -934,7 +949,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
       tc::commit<1>(&done);
     }
     __syncwarp();
-    if (!mbar_wait(&done, phase)) failed = 1;
+    if (!mbar_wait(&done, phase)) timed_out = true;
     phase ^= 1;
     __syncwarp();
     tc::fence_after();
@@ -1048,6 +1063,16 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
                               smem_addr(x_lo), MC / 64);
     });
     const bool last = step + 1 == A.steps;
+    if (last) {  // whether a wait ran out, in any block of the matrix
+      const int any = __syncthreads_or(timed_out);
+      if (threadIdx.x == 0) failed = any;
+      if (any) skip = true;
+      if (C > 1 && A.gate != nullptr) {
+        cluster_sync();
+        if (__syncthreads_or((int)threadIdx.x < C ? (int)cluster_load_u32(cluster_addr(&failed, threadIdx.x)) : 0))
+          skip = true;
+      }
+    }
     if (on) {
 #pragma unroll 1
       for (int c = group * 32; c < NC; c += 128) {
@@ -1072,7 +1097,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
   tc::fence_before();
   __syncthreads();
   if (C > 1) cluster_sync();  // no block leaves while another may reach into it
-  if (threadIdx.x == 0 && failed) atomicCAS(A.status, 0u, (uint32_t)GS_ERR_DEVICE_TIMEOUT);
+  if (threadIdx.x == 0 && failed) report_timeout(A.status, A.gate);
   if (warp == 0) {
     tc::fence_after();
     tc::tmem_free<1>(tmem, 2 * S::kTop);
@@ -1080,6 +1105,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) small_kernel(const __grid_co
 }
 
 // ---- host -----------------------------------------------------------------------------
+
+constexpr size_t kGateBytes = 256;  // the gate, first in the scratch; what follows keeps its lines
 
 struct Plan {
   int m, n, bn, ctas;       // X is m x n, tiles are 128 ctas x bn
@@ -1157,9 +1184,9 @@ static Plan make_plan(int batch, int rows, int cols, int type) {
   p.parts = (int)(parts < kMaxParts ? parts : kMaxParts);
   p.x_bytes = (size_t)batch * p.row_blocks * p.column_blocks * kBlockBytes;
   p.sq_bytes = (size_t)batch * p.row_blocks * p.sq_column_blocks * kBlockBytes;
-  p.total = 4 * p.x_bytes + (p.full ? 4 : 2) * p.sq_bytes + (size_t)batch * p.parts * 8;
+  p.total = kGateBytes + 4 * p.x_bytes + (p.full ? 4 : 2) * p.sq_bytes + (size_t)batch * p.parts * 8;
   const SmallPlan small = small_plan(p.m, p.n);
-  if (small.columns) p.total = 16 + (size_t)batch * shared_bytes(p.m <= 64 ? 64 : 128, small.cluster);
+  if (small.columns) p.total = kGateBytes + (size_t)batch * shared_bytes(p.m <= 64 ? 64 : 128, small.cluster);
   return p;
 }
 
@@ -1238,12 +1265,13 @@ static int launch_small(const SmallArgs &A, int batch, cudaStream_t st) {
     ready = ctx != 0 ? ctx : current_context_id();
   }
   cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = A.cluster;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = A.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1] = overlapping();
+  cfg.attrs = attr;
+  cfg.numAttrs = A.gate != nullptr ? 2 : 1;
   cfg.gridDim = dim3(batch * A.cluster);
   cfg.blockDim = dim3(kSmallThreads);
   cfg.dynamicSmemBytes = kBytes;
@@ -1290,16 +1318,23 @@ static int run(int batch, const Plan &p, const Source &src, const Out &out, int 
   Args A{};
   A.status = device_status_word();
   if (A.status == nullptr) return GS_ERR_CUDA;
+  char *at = static_cast<char *>(scratch) + kGateBytes;
+  if (out.update) {
+    A.gate = static_cast<uint32_t *>(scratch);
+    gate_kernel<<<1, 1, 0, st>>>(A.status, A.gate);
+    const int rc = launch_status();
+    if (rc) return rc;
+    count_launch();
+  }
   const SmallPlan small = small_plan(p.m, p.n);
   if (small.columns) {
-    const SmallArgs B{src, out, small.cluster, steps, a, b, c, (double)eps, static_cast<char *>(scratch), A.status};
+    const SmallArgs B{src, out, small.cluster, steps, a, b, c, (double)eps, at, A.status, A.gate};
     if (p.m <= 64)
       return small.columns == 64    ? launch_small<64, 64>(B, batch, st)
              : small.columns == 128 ? launch_small<64, 128>(B, batch, st)
                                     : launch_small<64, 256>(B, batch, st);
     return small.columns == 128 ? launch_small<128, 128>(B, batch, st) : launch_small<128, 256>(B, batch, st);
   }
-  char *at = static_cast<char *>(scratch);
   const auto take = [&](size_t n) {
     char *q = at;
     at += n;
@@ -1316,16 +1351,18 @@ static int run(int batch, const Plan &p, const Source &src, const Out &out, int 
   A.a = a;
   A.b = b;
   A.c = c;
-  norm_kernel<<<dim3(p.parts, batch), kNormThreads, 0, st>>>(src, parts, A.status);
-  int rc = launch_status();
-  if (rc) return rc;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr = overlapping();
   cfg.attrs = &attr;
+  cfg.numAttrs = A.gate != nullptr ? 1 : 0;
+  cfg.gridDim = dim3(p.parts, batch);
+  cfg.blockDim = dim3(kNormThreads);
+  cfg.stream = st;
+  int rc = cuda_status(cudaLaunchKernelEx(&cfg, norm_kernel, src, parts, (const uint32_t *)A.gate));
+  if (rc) return rc;
   cfg.numAttrs = 1;
   cfg.gridDim = dim3(p.row_blocks * 2 * p.column_blocks, batch);
   cfg.blockDim = dim3(256);
-  cfg.stream = st;
   rc = cuda_status(cudaLaunchKernelEx(&cfg, split_kernel, src, (const double *)parts, p.parts, (double)eps, A.x));
   if (rc) return rc;
   count_launch(2);

@@ -87,8 +87,8 @@ def muon_step(param: torch.Tensor, grad: torch.Tensor, momentum: torch.Tensor, l
     param and momentum are float32 and contiguous, (rows, cols) or a
     (batch, rows, cols) stack; grad has their shape, of any supported type. The
     three share no memory.
-    Like the Adam step it is skipped while the device status word holds an
-    error of an earlier kernel (gs_check_status)."""
+    Like the Adam step it is skipped, as a whole, while the device status word
+    holds an error of an earlier kernel (gs_check_status)."""
     _check_matrices("muon_step", param)
     _check_matrices("muon_step", grad)
     _check_steps("muon_step", steps, coefficients, eps)

@@ -649,8 +649,12 @@ GS_API int gs_orthogonalize(int batch, int rows, int cols, int type, const void 
 /* One optimizer step of `batch` contiguous fp32 matrices:
  *   M = beta M + (1 - beta) G;  U = nesterov ? beta M + (1 - beta) G : M;
  *   W = (1 - lr weight_decay) W - lr scale orthogonalize(U),
- * G of grad_type, contiguous. Scratch: gs_orthogonalize_scratch_bytes with
- * GS_TYPE_F32. Gated on the device status word like gs_adam_step. */
+ * G of grad_type, contiguous; the three share no memory. Scratch:
+ * gs_orthogonalize_scratch_bytes with GS_TYPE_F32. Gated on the device status
+ * word like gs_adam_step; the word is read once, so that all of the step is
+ * taken or none, whatever other streams record meanwhile. A bounded wait of the
+ * step's own that runs out is recorded there as well; the momentum has been
+ * updated then, weights not yet written stay as they were. */
 GS_API int gs_muon_step(int batch, int rows, int cols, int grad_type, float *params,
                         const void *grads, float *momentum, double lr, double beta, int nesterov,
                         double weight_decay, double scale, int steps, float a, float b, float c,

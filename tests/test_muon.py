@@ -372,3 +372,43 @@ def test_the_largest_values_that_are_accepted(gs, m, n, dtype):
     tol = (23 * 2.0 ** -22 if dtype != BF16 else 16 * 2.0 ** -11) + torch.finfo(dtype).eps / 2
     assert float((got - ref).abs().max()) <= tol * float(ref.max())
     assert int((got != 0).sum()) == 1
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(1024, 2048), (100, 900), (64, 64), (5, 90, 300)])
+def test_a_step_is_taken_or_skipped_as_a_whole(gs, shape):
+    """Another stream records an error before, during or after the step: weights and momentum are both
+    those of the step, or both untouched."""
+    nat = importlib.import_module("3dgs_from_scratch_b200._native")
+    gen = torch.Generator(device=DEV).manual_seed(11)
+    w, g, m = (torch.randn(*shape, generator=gen, device=DEV) for _ in range(3))
+    w1, m1 = w.clone(), m.clone()
+    gs.muon_step(w1, g, m1, 0.1)
+    error = torch.ones(1, dtype=torch.int32, device=DEV)
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    assert nat.query("gs_check_status", nat.stream_ptr()) == 0
+    taken = []
+    for delay in range(0, 420, 20):                 # microseconds, at about 1.9 GHz
+        w2, m2 = w.clone(), m.clone()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(other):
+            torch.cuda._sleep(1 + 1900 * delay)
+            nat.call("gs_status_merge", error.data_ptr(), other.cuda_stream)
+        gs.muon_step(w2, g, m2, 0.1)
+        torch.cuda.synchronize()
+        assert nat.query("gs_check_status", nat.stream_ptr()) == nat.GS_ERR_PEER
+        taken.append(torch.equal(m2, m1))
+        if taken[-1]:
+            assert torch.equal(w2, w1), delay
+        else:
+            assert torch.equal(w2, w) and torch.equal(m2, m), delay
+    with torch.cuda.stream(other):                  # and before it
+        nat.call("gs_status_merge", error.data_ptr(), other.cuda_stream)
+    torch.cuda.synchronize()
+    w2, m2 = w.clone(), m.clone()
+    gs.muon_step(w2, g, m2, 0.1)
+    torch.cuda.synchronize()
+    assert nat.query("gs_check_status", nat.stream_ptr()) == nat.GS_ERR_PEER
+    assert torch.equal(w2, w) and torch.equal(m2, m)
+    assert any(taken)
