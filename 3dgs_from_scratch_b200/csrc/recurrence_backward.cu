@@ -138,15 +138,10 @@ __global__ void __launch_bounds__(kThreads) backward_kernel(const __grid_constan
 #pragma unroll
         for (int k = kBatch - 1; k >= 0; --k) {
           if (k >= n) continue;
-          if (lasts >> k & 1) {
-            q.seek(A, row + k * one);
-            load_state(A.dfinal, A, q.s, p, v_in);
-          }
+          if ((firsts | lasts) >> k & 1) q.seek(A, row + k * one);
+          if (lasts >> k & 1) load_state(A.dfinal, A, q.s, p, v_in);
           finish(k, !(outside >> k & 1));
-          if ((firsts >> k & 1) && A.dinitial != nullptr) {
-            q.seek(A, row + k * one);
-            store_state(A.dinitial, A, q.s, p, v_in);
-          }
+          if ((firsts >> k & 1) && A.dinitial != nullptr) store_state(A.dinitial, A, q.s, p, v_in);
         }
       }
     }
