@@ -16,6 +16,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
@@ -48,6 +49,9 @@ def _rows_of(t, channels):
 
 
 def _check(x, gate, initial, offsets):
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (x, gate, initial)):
+        raise NotImplementedError("gated_scan has no forward-mode derivative")
     if x.dim() != 2 and (x.dim() != 3 or offsets is not None):
         raise ValueError("gated_scan expects x of shape (rows, channels), with offsets or as one "
                          "sequence, or (batch, rows, channels)")
@@ -192,7 +196,7 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, initial: torch.Tensor | None
 
     float32, bfloat16 or float16; gates of x's type or float32. The recurrence
     runs in fp32 and h is rounded once. Differentiable w.r.t. x, gate and
-    initial (once), through h and final."""
+    initial (once, in reverse mode), through h and final."""
     sequences = _check(x, gate, initial, offsets)
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or
                                     initial is not None and initial.requires_grad):

@@ -617,3 +617,29 @@ def test_a_long_run_of_empty_sequences(gs, rows, lists, reverse):
     for kind in ("run", "scattered"):
         assert all(torch.equal(a, b) for a, b in zip(out["none"], out[kind])), kind
     assert times["run"] < 3 * times["scattered"] + 0.2, times
+
+
+def test_forward_mode_derivatives_are_refused(gs):
+    """A tangent would be lost without a word, as if the derivative were zero."""
+    fw = torch.autograd.forward_ad
+    x, g, init = torch.randn(4, 6), torch.rand(4, 6), torch.randn(1, 6)
+    with fw.dual_level():
+        duals = [fw.make_dual(t, torch.ones_like(t)) for t in (x, g, init)]
+        for args in ((duals[0], g, init), (x, duals[1], init), (x, g, duals[2])):
+            with pytest.raises(NotImplementedError):
+                gs.gated_scan(*args)
+    with pytest.raises(NotImplementedError):
+        torch.func.jvp(lambda t: gs.gated_scan(t, g)[0], (x,), (x,))
+
+
+@gpu
+def test_forward_mode_levels_without_tangents(gs):
+    fw = torch.autograd.forward_ad
+    x, g = torch.randn(4, 6, device=DEV), torch.rand(4, 6, device=DEV)
+    ref = gs.gated_scan(x, g)[0]
+    with fw.dual_level():
+        assert torch.equal(gs.gated_scan(x, g)[0], ref)
+        for wanted in (False, True):
+            leaf = x.clone().requires_grad_(wanted)
+            with pytest.raises(NotImplementedError):
+                gs.gated_scan(fw.make_dual(leaf, torch.ones_like(x)), g)
