@@ -17,6 +17,8 @@
 //     grows with the number of additions (2.6e-5 of the result at 4096 x 4096
 //     with one accumulator for all of K); so each 256 elements of K start a
 //     fresh accumulator, and these parts are added in registers, rounded.
+//     half products start one every 8192 elements (a bias of 2e-5), which also
+//     keeps the longest wait for an accumulator short.
 //   half (bf16 results, 2^-9 a rounding): A and B are computed from and held
 //     as hi alone. Their errors (2^-12) multiply each singular direction by
 //     1 + small and mix left directions only, so a small singular value keeps
@@ -260,7 +262,7 @@ struct Shape {
   static constexpr int kPlaneA = 128 * 128, kPlaneB = kRowsB * 128;  // bytes
   static constexpr int kStage = kPlanesA * kPlaneA + kPlanesB * kPlaneB;
   static constexpr int kTri = BN > 128 * CTAS ? BN : 128 * CTAS;
-  static constexpr int kChunk = FULL ? 4 : 1 << 30;        // K blocks of an accumulator
+  static constexpr int kChunk = FULL ? 4 : 128;            // K blocks of an accumulator
   // Where there is room, hi lo + lo hi have an accumulator of their own: far
   // fewer cut-off additions to the large one (128 x 64 in fp32: the result's
   // error 2.3e-6 -> 1.2e-6, as fp32 products have).

@@ -412,3 +412,22 @@ def test_a_step_is_taken_or_skipped_as_a_whole(gs, shape):
     assert nat.query("gs_check_status", nat.stream_ptr()) == nat.GS_ERR_PEER
     assert torch.equal(w2, w) and torch.equal(m2, m)
     assert any(taken)
+
+
+@gpu
+def test_very_wide_bf16_matrices(gs):
+    """Rows of equal size and orthogonal signs (Walsh functions), X = c S with S S^T = n I: one step with
+    (0, 1, 0) gives X / m. Held to 2^-11 are X in A, twice, and A; the result is rounded to half a step.
+    Sums of 8192 elements are cut off at 2^-23 in each of 512 additions of a growing sum, and 768 of
+    them added at 2^-24: below 1e-4. One sum over all of K, cut off 393,216 times, would be 1.3% low."""
+    m, n = 130, 3 << 21
+    k = torch.arange(256, device=DEV)
+    parity = k[:, None] & k
+    for shift in (4, 2, 1):
+        parity = parity ^ (parity >> shift)
+    signs = (1 - 2 * (parity & 1))[:m].to(BF16)
+    u = (signs * 1e-3).repeat(1, n // 256)
+    got = gs.orthogonalize(u, steps=1, coefficients=(0.0, 1.0, 0.0))
+    ref = 1 / math.sqrt(m * n) / m
+    off = (got.reshape(m, n // 256, 256).float() * signs[:, None].float()).sub_(ref).abs_().max()
+    assert float(off) <= (3 * 2.0 ** -11 + 2.0 ** -8 + 1e-4) * ref
