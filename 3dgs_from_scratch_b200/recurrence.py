@@ -111,9 +111,10 @@ def _forward(x, gate, initial, offsets, reverse, sequences, keep):
     h = torch.empty_like(x, memory_format=torch.contiguous_format)
     final = _states_like(initial, (sequences, channels), x)
     rows = x.numel() // channels
-    if rows == 0 or sequences == 0:
+    if sequences == 0 or rows == 0 and offsets is None:
         final.zero_() if initial is None else final.copy_(initial)
         return h, final, None, None
+    # (without rows the offsets are still looked at)
     (xr, x_step), (gr, g_step) = _rows_of(x, channels), _rows_of(gate, gates)
     init, offs = _states(initial), offsets
     if offs is not None:

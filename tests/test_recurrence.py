@@ -643,3 +643,23 @@ def test_forward_mode_levels_without_tangents(gs):
             leaf = x.clone().requires_grad_(wanted)
             with pytest.raises(NotImplementedError):
                 gs.gated_scan(fw.make_dual(leaf, torch.ones_like(x)), g)
+
+
+@gpu
+def test_offsets_are_looked_at_without_rows(gs):
+    nat = importlib.import_module("3dgs_from_scratch_b200._native")
+    init = torch.randn(2, 6, device=DEV, requires_grad=True)
+    for kind, layout in ((F32, torch.zeros(0, 6, device=DEV)), (F32, torch.zeros(9, 12, device=DEV)[9:, 3:9])):
+        x = layout.to(kind)
+        for offsets, error in (([0, 0, 0], nat.GS_OK), ([0, 0, 5], nat.GS_ERR_INVALID_ARGUMENT),
+                               ([0, -1, 0], nat.GS_ERR_INVALID_ARGUMENT)):
+            assert nat.query("gs_check_status", nat.stream_ptr()) == nat.GS_OK
+            offs = torch.tensor(offsets, device=DEV)
+            h, final = gs.gated_scan(x, x, initial=init, offsets=offs)
+            assert nat.query("gs_check_status", nat.stream_ptr()) == error
+            assert h.shape == (0, 6)
+            if error == nat.GS_OK:
+                assert torch.equal(final, init)
+                (dinit,) = torch.autograd.grad(final.square().sum(), init)
+                assert torch.equal(dinit, 2 * init.detach())
+                assert float(gs.gated_scan(x, x, offsets=offs)[1].abs().max()) == 0.0
