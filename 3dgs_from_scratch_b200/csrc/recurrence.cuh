@@ -376,8 +376,8 @@ __device__ __forceinline__ Wide normal(float v, int e) {
 // rows of the sequence that reaches over the chunk's end, from that sequence's
 // first row along the chain where the chunk holds it (the chain is cut there).
 
-// p times the gates of n rows, one by one: where their product leaves the range,
-// or one is 0. What is not finite needs no care here: the run's result is
+// p times the gates of n rows, one by one: where their product leaves the range.
+// What is not finite needs no care here: the run's result is
 // not finite then.
 template <typename GT>
 __device__ __forceinline__ void multiply_rows(Wide &p, const GT *gate, int64_t step, int n) {
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, ST || (V == 4 && !SHARED) ? 2 : 4) m
         }
       // Cut runs need no product. Where threads are bound by their loads alone, a
       // branch around it costs more than it (bf16 with fp32 gates, 8 x 2048 x 1024:
-      // forward 57 us with, 51 without; bf16, 49,152 x 333: 55 and 59).
+      // forward 57 us with, 48 without; bf16, 49,152 x 333: 55 and 59).
       if (!ST || !cut) {
 #pragma unroll
         for (int k = 0; k < kAhead; ++k)
@@ -476,8 +476,13 @@ __global__ void __launch_bounds__(kThreads, ST || (V == 4 && !SHARED) ? 2 : 4) m
         for (int v = 0; v < kGates; ++v) {
           if (fabsf(product[v]) >= 0x1p-110f && fabsf(product[v]) <= 0x1p110f)
             P[v] = normal(product[v], P[v].e);
-          else if (!cut && P[v].m != 0.f)
-            multiply_rows(P[v], gate + p.at(v), gstep, left < kAhead ? left : kAhead);
+          else if (!cut && P[v].m != 0.f) {
+            bool zero = false;  // most often a reset
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) zero = zero || (k < left && g[k](v) == 0.f);
+            if (zero) P[v] = Wide{0.f, 0};
+            else multiply_rows(P[v], gate + p.at(v), gstep, left < kAhead ? left : kAhead);
+          }
           peak = max(peak, P[v].e);
         }
       }
