@@ -110,9 +110,6 @@ SIGNATURES = {
                                          P, I, P, P, P, P, P, P, P]),
 }
 
-# GS_TYPE_* by torch dtype name
-TYPES = {"float32": 0, "bfloat16": 1, "float16": 2}
-
 _lib = None
 _lock = threading.Lock()
 

@@ -48,6 +48,11 @@ Plan make_plan(int64_t rows, int sequences, bool even, int channels, int gates, 
   // Rows of a chunk: about kFill threads on each of 148 SMs.
   const int64_t want = rows * vectors / (148 * kFill);
   const int64_t period = even ? rows / sequences : 0;
+  // Sequences stay whole, without the chain's launches, where they are short or
+  // enough to give 256 threads an SM: fewer lose more by the threads that are
+  // missing (512 rows x 64 channels fp32, forward and backward: 137 us whole and 92
+  // cut at 64 threads an SM, 156 and 168 at 128, 217 and 300 at 256, 513 and 694 at
+  // 640; 2048 rows 816 and 1125 at 256).
   p.whole = even && period > 0 && (period <= kShort || (int64_t)sequences * vectors >= 148 * 256);
   if (p.whole) {
     const int64_t k = want / period;
@@ -69,7 +74,7 @@ Plan make_plan(int64_t rows, int sequences, bool even, int channels, int gates, 
 // 128 threads a channel with a run of chunks each. The runs' maps are scanned in
 // shared memory, then each thread goes through its run once more from the state
 // before it. Many chunks are shared out over a cluster of blocks, which read
-// each other's maps: one SM alone takes 14 us for 4096 chunks.
+// each other's maps.
 constexpr int kCarryChannels = 4, kRuns = 128, kCarryBlocks = 8;
 
 // A run's map with P in fp32, for products of at most 1, and in the form that
@@ -227,7 +232,10 @@ __global__ void __launch_bounds__(kCarryChannels *kRuns) carry_kernel(const __gr
 }
 
 int launch_carry(const Args &A, bool back, cudaStream_t st) {
-  // 941 chunks take 8 us in one block and 20 in a cluster, 2048 take 19 and 9.
+  // The whole forward in fp32 with one block, and with a cluster: 941 chunks of 32
+  // rows x 64 channels 12.1 and 16.2 us, x 200 19.6 and 26.7; 4096 x 64 33.0 and
+  // 27.8, 4096 x 4 25.9 and 20.0. Between, few channels gain by a cluster (2048 x 4
+  // 20.5 and 19.8) and more lose (2048 x 64 15.6 and 18.8).
   const int blocks = A.plan.chunks > 12 * kRuns ? kCarryBlocks : 1;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2];

@@ -586,10 +586,10 @@ GS_API int gs_reset_opacities(int n, float *opacity_logits, float *exp_avg, floa
  * (sequences, channels); the recurrence is computed in fp32 and h rounded
  * once. x, gate and grad_h have a stride of elements from row to row; outputs
  * are contiguous. Rows outside every sequence are not read into a result and
- * are written as zeros. Pointers and row strides are multiples of 16 bytes
- * (8 where an 16-bit x goes with fp32 gates of one per channel) when the
- * channels (with shared gates: the channels per gate) fill whole vectors of
- * that size, otherwise of the element. rows <= INT32_MAX,
+ * are written as zeros. Pointers and row strides are multiples of 8 bytes (4
+ * for a 16-bit x that goes with fp32 gates of one per channel) when the channels
+ * (with shared gates: the channels per gate) fill whole vectors of that size,
+ * otherwise, and for shared gates, of the element. rows <= INT32_MAX,
  * sequences <= 2^28. Offsets that do not ascend within [0, rows] record
  * GS_ERR_INVALID_ARGUMENT in the device status word; what is written then is
  * undefined, but within the buffers. */
@@ -630,8 +630,10 @@ GS_API int gs_gated_scan_backward(int64_t rows, int sequences, int channels, int
  *   A = X X^T;  B = b A + c A A;  X = a X + B X,
  * which brings X near the orthogonal factor of U: every singular value s
  * follows p(s) = a s + b s^3 + c s^5. Products run on the tensor cores with
- * fp32 accumulation; results of type fp32 and fp16 carry fp32's accuracy, bf16
- * results that of their type.
+ * fp32 accumulation. Results of type fp32 and fp16 carry about fp32's accuracy;
+ * bf16 results are computed with 11-bit operands in A and A A, which adds about a
+ * quarter to the error of the final rounding. X is held to 2^-37 absolutely at
+ * best, so where |U|_F lies far below eps its last bits go first.
  *
  * 1 <= batch <= 65535, rows and cols <= 2^24, the smaller <= 2^15;
  * 1 <= steps <= 100; eps > 0. The coefficients have to keep |X|_2 and |B|_2
