@@ -431,3 +431,31 @@ def test_very_wide_bf16_matrices(gs):
     ref = 1 / math.sqrt(m * n) / m
     off = (got.reshape(m, n // 256, 256).float() * signs[:, None].float()).sub_(ref).abs_().max()
     assert float(off) <= (3 * 2.0 ** -11 + 2.0 ** -8 + 1e-4) * ref
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(64, 64), (100, 900), (5, 90, 300), (600, 700)])
+def test_captured_steps_replay(gs, shape):
+    """On chip, in clusters, in stacks and in tiles: two replayed steps are the two steps, and a replay
+    that finds an error recorded is skipped."""
+    nat = importlib.import_module("3dgs_from_scratch_b200._native")
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    w, g, m = (torch.randn(*shape, generator=gen, device=DEV) for _ in range(3))
+    w1, m1 = w.clone(), m.clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        gs.muon_step(w1, g, m1, 0.1, weight_decay=0.1)
+    assert torch.equal(w1, w)
+    for _ in range(2):
+        graph.replay()
+        gs.muon_step(w, g, m, 0.1, weight_decay=0.1)
+    torch.cuda.synchronize()
+    assert torch.equal(w1, w) and torch.equal(m1, m)
+    assert nat.query("gs_check_status", nat.stream_ptr()) == 0
+    error = torch.ones(1, dtype=torch.int32, device=DEV)
+    nat.call("gs_status_merge", error.data_ptr(), nat.stream_ptr())
+    graph.replay()
+    torch.cuda.synchronize()
+    assert nat.query("gs_check_status", nat.stream_ptr()) == nat.GS_ERR_PEER
+    assert torch.equal(w1, w) and torch.equal(m1, m)
