@@ -125,8 +125,9 @@ struct Broad {
   __device__ bool grown() const { return false; }
 };
 
-// What a block keeps in shared memory. More than these 9 KB would keep it from
-// running next to the walk, which starts before the scan has ended.
+// What a block keeps in shared memory. More than these 9 KB keep the walk, which
+// starts before the scan has ended, off the same SM for longer (25 KB: 1,300
+// chunks x 200 channels 36 us in place of 34).
 template <class M>
 struct Scanned {
   static constexpr int kBuffers = sizeof(M) == 8 ? 2 : 1;
